@@ -313,6 +313,129 @@ b2vx_status b2vx_conv2d_first_layer_noalloc(const b2vx_conv2d_noalloc_desc* d, c
                                             const int32_t* bias_full, const float* acc_scale, void* y_cl,
                                             void* cuda_stream, char* err, size_t err_len);
 
+/* ---- operators on device tensors: 4-bit block floating point and experts -------
+ * No counterpart in the reference.  For programs whose tensors already live on the
+ * GPU (a language model's decode loop): every argument is a device pointer of the
+ * current device, results are queued on `cuda_stream` (NULL: the default stream)
+ * and the call returns without waiting.  Nothing is allocated: intermediates go to
+ * a workspace of the caller's, whose size the _workspace_ calls tell.  A call may
+ * be captured into a CUDA graph, after the first call on that GPU; calls or
+ * captured graphs that may overlap need a workspace each.  Arguments are checked
+ * before anything is launched; refusals return a status and write a message to err
+ * (err may be NULL).  Counts of zero are fine: nothing is launched.
+ *
+ * 4-bit values are e2m1: codes 0..7 stand for 0, 0.5, 1, 1.5, 2, 3, 4, 6, bit 3 is
+ * the sign; two to a byte, the even column in the low half.
+ *   B2VX_FP4_BLOCK32  one scale byte per 32 columns, e8m0: byte b stands for
+ *                     2^(b-127), 255 for NaN.  Quantization: 2^(floor(log2(amax))-2),
+ *                     not below 2^-127
+ *   B2VX_FP4_BLOCK16  one scale byte per 16 columns, e4m3 without sign (127 is NaN),
+ *                     times one positive float for the tensor.  Quantization: amax / 6 /
+ *                     tensor scale, rounded to nearest even, at most 448
+ * Numbers are divided by their scale exactly, rounded to nearest even and cut to
+ * +-6.  A block that holds a NaN or an infinity gets the scale NaN and codes 0.
+ * Scales come in two layouts: B2VX_SCALES_ROWS, [rows][blocks of a row], and
+ * B2VX_SCALES_PACKED, the operand layout of the products (tiles of 128 rows x 4
+ * blocks), whose size b2vx_fp4_packed_scales_size_noalloc tells. */
+#define B2VX_DT_BFLOAT16 16
+enum { B2VX_FP4_BLOCK32 = 1, B2VX_FP4_BLOCK16 = 2 };
+enum { B2VX_SCALES_ROWS = 0, B2VX_SCALES_PACKED = 1 };
+
+/* x [x_rows][x_stride] (float32, float16 or bfloat16) to codes [rows][codes_pitch]
+ * and scales.  codes_pitch (bytes): a multiple of 4, at least k rounded up to 32,
+ * over 2; columns from k to there get code 0.  scales_pitch (bytes, layout ROWS): at
+ * least ceil(k / block).  row_index (int32 [rows], may be NULL): output row i is
+ * row row_index[i] of x, a row of zeros where that is outside 0..x_rows-1.
+ * tensor_scale: one float, BLOCK16 only; a scale that is not positive and finite
+ * makes every block NaN. */
+typedef struct b2vx_fp4_quantize_desc {
+  int32_t format, scales_layout, x_dtype;
+  uint64_t x_rows, rows, k;
+  uint64_t x_stride;        /* elements between rows of x */
+  uint64_t codes_pitch, scales_pitch;
+} b2vx_fp4_quantize_desc;
+b2vx_status b2vx_fp4_quantize_noalloc(const b2vx_fp4_quantize_desc* d, const void* x, const int32_t* row_index,
+                                      const float* tensor_scale, void* codes, void* scales,
+                                      void* cuda_stream, char* err, size_t err_len);
+/* The values that codes and scales (layout ROWS) stand for, times the tensor scale, rounded once to y_dtype. */
+typedef struct b2vx_fp4_dequantize_desc {
+  int32_t format, y_dtype;
+  uint64_t rows, k;
+  uint64_t codes_pitch, scales_pitch;
+  uint64_t y_stride;        /* elements */
+} b2vx_fp4_dequantize_desc;
+b2vx_status b2vx_fp4_dequantize_noalloc(const b2vx_fp4_dequantize_desc* d, const void* codes, const void* scales,
+                                        const float* tensor_scale, void* y, void* cuda_stream, char* err, size_t err_len);
+/* Scales [matrices][rows][ceil(k / block)] to the packed layout, matrix after matrix. */
+b2vx_status b2vx_fp4_packed_scales_size_noalloc(int32_t format, uint64_t matrices, uint64_t rows, uint64_t k, size_t* bytes);
+b2vx_status b2vx_fp4_pack_scales_noalloc(int32_t format, uint64_t matrices, uint64_t rows, uint64_t k, const void* scales,
+                                         void* packed, void* cuda_stream, char* err, size_t err_len);
+
+/* Products with one matrix (FullyConnected on device tensors) or one per group of rows (experts):
+ *   y[m][f] = alpha * sum_k x[m][k] w_e[f][k] + bias_e[f]
+ *   gated:    silu(that with rows f of w_e) * (that with rows n + f)
+ * experts == 0: one matrix w [n][k], offsets NULL.  Otherwise w is [experts][n][k]
+ * and rows offsets[e] .. offsets[e+1]-1 (int32 [experts + 1], rising, at most rows) belong to
+ * expert e; other rows of y are left as they are.  Offsets that fall or lie outside 0..rows are cut to rising values in
+ * there; no access leaves the buffers.  gated doubles the rows of w and bias ([2n], gate first).
+ *   w_format 0: w and x are 16-bit floats of x_dtype, k a multiple of 8
+ *   w_format B2VX_FP4_*: w is codes [..][k/2], k a multiple of 32; w_scales packed (gated: 2 * experts matrices of n rows);
+ *     x (float32, float16, bfloat16) is quantized to the same format on the way in.
+ *     BLOCK16: alpha = x_scale * w_scale[e], the tensors' scales; required then, NULL otherwise
+ * row_index (int32 [rows] or NULL): row m of the product is row row_index[m] of x (zeros where out of range).
+ * bias: float32 or NULL.  y_dtype: float32, float16 or bfloat16; sums are float32, rounded once.
+ * w: 16-byte aligned.  experts <= 1024.  The values of w's rows and scales are used as they are: NaN scales give NaN. */
+typedef struct b2vx_linear_desc {
+  int32_t w_format, x_dtype, y_dtype, gated;
+  uint32_t experts;
+  uint64_t x_rows, rows, n, k;
+  uint64_t x_stride, y_stride;   /* elements */
+} b2vx_linear_desc;
+typedef struct b2vx_linear_args {
+  const void* x;
+  const void* w;
+  const void* w_scales;
+  const float* x_scale;
+  const float* w_scale;
+  const float* bias;
+  const int32_t* offsets;
+  const int32_t* row_index;
+  void* y;
+  void* workspace;               /* 256-byte aligned */
+  size_t workspace_bytes;
+} b2vx_linear_args;
+b2vx_status b2vx_linear_workspace_size_noalloc(const b2vx_linear_desc* d, size_t* bytes, char* err, size_t err_len);
+b2vx_status b2vx_linear_noalloc(const b2vx_linear_desc* d, const b2vx_linear_args* a, void* cuda_stream, char* err, size_t err_len);
+
+/* The experts of each token: ids[t][j] (int32) = the top_k largest of logits[t][0..experts-1], largest first, ties to the
+ * lowest index; weights[t][j] (float32) = exp(logit - max) over the sum of all experts' (normalize 0) or of the chosen (1).
+ * A NaN logit counts as -infinity; a row without anything above -infinity gets weights 0.
+ * offsets (int32 [experts + 1]): first row of each expert when the pairs (t, j) are sorted by expert, then t;
+ * row_index (int32 [tokens * top_k]): the token of each sorted row; slots (int32 [tokens][top_k]): the sorted row of a pair.
+ * experts <= 1024, top_k <= min(32, experts), tokens * top_k < 2^31. */
+typedef struct b2vx_route_desc {
+  int32_t logits_dtype, normalize;
+  uint32_t experts, top_k;
+  uint64_t tokens, logits_stride;  /* elements */
+} b2vx_route_desc;
+b2vx_status b2vx_route_workspace_size_noalloc(const b2vx_route_desc* d, size_t* bytes, char* err, size_t err_len);
+b2vx_status b2vx_route_noalloc(const b2vx_route_desc* d, const void* logits, int32_t* ids, float* weights, int32_t* offsets,
+                               int32_t* row_index, int32_t* slots, void* workspace, size_t workspace_bytes,
+                               void* cuda_stream, char* err, size_t err_len);
+/* y[t] = residual[t] + sum_j weights[t][j] z[slots[t][j]], sums in float32 in the order of j, rounded once; a slot outside
+ * 0..z_rows-1 adds nothing.  z, residual (may be NULL) and y have one dtype; y may be residual. */
+typedef struct b2vx_combine_desc {
+  int32_t dtype;
+  uint32_t top_k;
+  uint64_t tokens, n, z_rows;
+  uint64_t z_stride, residual_stride, y_stride;  /* elements */
+} b2vx_combine_desc;
+b2vx_status b2vx_combine_noalloc(const b2vx_combine_desc* d, const void* z, const int32_t* slots, const float* weights,
+                                 const void* residual, void* y, void* cuda_stream, char* err, size_t err_len);
+/* Waits for the stream and tells whether a product on the current GPU gave up on a barrier since the last such call
+ * (B2VX_DEVICE_TIMEOUT; its y is incomplete).  Later calls on that GPU are refused until this one is made. */
+b2vx_status b2vx_device_check_noalloc(void* cuda_stream, char* err, size_t err_len);
+
 /* Measurement aid with no counterpart in the reference: the dense int8 rate of
  * the tensor pipe of GPU `device_id`, in TOP/s (2 x multiply-accumulate), from
  * an issue-rate microbenchmark (tcgen05.mma.kind::i8 on operands resident in

@@ -1,0 +1,201 @@
+"""Refusals of the operators on device tensors, and the sizes they tell: host-side rules, no GPU needed.
+
+Every refusal comes before the first CUDA call, so the pointers here are only numbers."""
+import ctypes as C
+
+import pytest
+
+import deviceops as D
+
+PTR = 1 << 20   # an address that is aligned to everything; never read
+
+
+def desc(cls, base, **change):
+    d = cls()
+    for name, value in dict(base, **change).items():
+        setattr(d, name, value)
+    return d
+
+
+QUANTIZE = dict(format=1, scales_layout=0, x_dtype=16, x_rows=8, rows=8, k=96, x_stride=96, codes_pitch=48, scales_pitch=3)
+DEQUANTIZE = dict(format=1, y_dtype=16, rows=8, k=96, codes_pitch=48, scales_pitch=3, y_stride=96)
+LINEAR = dict(w_format=1, x_dtype=16, y_dtype=16, gated=0, experts=0, x_rows=8, rows=8, n=64, k=96, x_stride=96, y_stride=64)
+ROUTE = dict(logits_dtype=9, normalize=1, experts=16, top_k=4, tokens=8, logits_stride=16)
+COMBINE = dict(dtype=16, top_k=2, tokens=8, n=64, z_rows=16, z_stride=64, residual_stride=64, y_stride=64)
+
+
+def refused(fn, *args):
+    err = C.create_string_buffer(256)
+    st = fn(*args, err, 256)
+    assert st == 1, (st, err.value)
+    assert err.value
+    assert fn(*args, None, 0) == 1      # without a place for the message
+    return err.value.decode()
+
+
+@pytest.mark.parametrize("change,scale,words", [
+    (dict(format=0), None, "format"), (dict(format=3), None, "format"), (dict(scales_layout=2), None, "layout"), (dict(x_dtype=2), None, "float32"),
+    (dict(k=1 << 30), None, "range"), (dict(rows=1 << 30), None, "range"), (dict(x_stride=95), None, "x_stride"), (dict(x_stride=1 << 41), None, "x_stride"),
+    (dict(codes_pitch=44), None, "codes_pitch"), (dict(codes_pitch=49), None, "codes_pitch"), (dict(scales_pitch=2), None, "scales_pitch"),
+    (dict(format=2, scales_pitch=6), None, "tensor scale"), (dict(), PTR, "tensor scale"), (dict(rows=9), None, "row_index")])
+def test_quantize_refuses(change, scale, words):
+    fn = D.library().b2vx_fp4_quantize_noalloc
+    assert words in refused(fn, C.byref(desc(D.QuantizeDesc, QUANTIZE, **change)), PTR, None, scale, PTR, PTR, None)
+
+
+def test_quantize_refuses_pointers():
+    fn = D.library().b2vx_fp4_quantize_noalloc
+    d = C.byref(desc(D.QuantizeDesc, QUANTIZE))
+    assert "null" in refused(fn, None, PTR, None, None, PTR, PTR, None)
+    for args in ((None, None, None, PTR, PTR, None), (PTR, None, None, None, PTR, None), (PTR, None, None, PTR, None, None)):
+        assert "null" in refused(fn, d, *args)
+    assert "aligned" in refused(fn, d, PTR + 1, None, None, PTR, PTR, None)
+    assert "aligned" in refused(fn, d, PTR, None, None, PTR + 2, PTR, None)
+    packed = C.byref(desc(D.QuantizeDesc, QUANTIZE, scales_layout=1))
+    assert "aligned" in refused(fn, packed, PTR, None, None, PTR, PTR + 4, None)
+
+
+@pytest.mark.parametrize("change,scale,words", [
+    (dict(format=0), None, "format"), (dict(y_dtype=1), None, "float32"), (dict(rows=1 << 30), None, "range"), (dict(codes_pitch=40), None, "codes_pitch"),
+    (dict(scales_pitch=1), None, "scales_pitch"), (dict(y_stride=95), None, "y_stride"), (dict(format=2, scales_pitch=6), None, "tensor scale"),
+    (dict(), PTR, "tensor scale")])
+def test_dequantize_refuses(change, scale, words):
+    fn = D.library().b2vx_fp4_dequantize_noalloc
+    assert words in refused(fn, C.byref(desc(D.DequantizeDesc, DEQUANTIZE, **change)), PTR, PTR, scale, PTR, None)
+
+
+def test_dequantize_refuses_pointers():
+    fn = D.library().b2vx_fp4_dequantize_noalloc
+    d = C.byref(desc(D.DequantizeDesc, DEQUANTIZE))
+    for args in ((None, PTR, None, PTR, None), (PTR, None, None, PTR, None), (PTR, PTR, None, None, None)):
+        assert "null" in refused(fn, d, *args)
+    assert "aligned" in refused(fn, d, PTR, PTR, None, PTR + 1, None)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(w_format=4), "w_format"), (dict(x_dtype=1), "float32"), (dict(y_dtype=2), "float32"), (dict(w_format=0, x_dtype=9), "16-bit"),
+    (dict(gated=2), "gated"), (dict(experts=1025), "1024"), (dict(n=1 << 30), "range"), (dict(k=0, x_stride=0), "zero"), (dict(k=100, x_stride=100), "multiple"),
+    (dict(w_format=0, k=100, x_stride=100), "multiple"), (dict(x_stride=95), "x_stride"), (dict(y_stride=63), "y_stride"),
+    (dict(rows=1 << 28, x_rows=1 << 28, n=1 << 20, y_stride=1 << 20), "tiles")])
+def test_linear_refuses(change, words):
+    size = C.c_size_t()
+    d = desc(D.LinearDesc, LINEAR, **change)
+    assert words in refused(D.library().b2vx_linear_workspace_size_noalloc, C.byref(d), C.byref(size))
+    args = D.LinearArgs(PTR, PTR, PTR, None, None, None, None, None, PTR, PTR, 1 << 30)
+    assert words in refused(D.library().b2vx_linear_noalloc, C.byref(d), C.byref(args), None)
+
+
+@pytest.mark.parametrize("change,args,words", [
+    (dict(), dict(offsets=PTR), "offsets"), (dict(experts=4), dict(), "offsets"), (dict(w_format=2), dict(), "tensor scales"),
+    (dict(w_format=2), dict(x_scale=PTR), "tensor scales"), (dict(), dict(w_scale=PTR), "tensor scales"), (dict(rows=9), dict(), "row_index"),
+    (dict(), dict(x=None), "null"), (dict(), dict(w=None), "null"), (dict(), dict(y=None), "null"), (dict(), dict(w_scales=None), "null"),
+    (dict(), dict(w=PTR + 8), "aligned"), (dict(), dict(w_scales=PTR + 8), "aligned"), (dict(), dict(y=PTR + 1), "aligned"), (dict(), dict(x=PTR + 1), "aligned"),
+    (dict(), dict(workspace=None), "workspace"), (dict(), dict(workspace=PTR + 16), "workspace"), (dict(), dict(workspace_bytes=100), "workspace"),
+    (dict(w_format=0), dict(row_index=PTR, workspace_bytes=0), "workspace"), (dict(w_format=0, x_stride=100), dict(workspace=None), "workspace")])
+def test_linear_refuses_arguments(change, args, words):
+    d = desc(D.LinearDesc, LINEAR, **change)
+    a = desc(D.LinearArgs, dict(x=PTR, w=PTR, w_scales=PTR, y=PTR, workspace=PTR, workspace_bytes=1 << 30), **args)
+    assert words in refused(D.library().b2vx_linear_noalloc, C.byref(d), C.byref(a), None)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(experts=0), "experts"), (dict(experts=1025, logits_stride=1025), "experts"), (dict(top_k=0), "top_k"), (dict(top_k=17), "top_k"),
+    (dict(experts=64, logits_stride=64, top_k=33), "top_k"), (dict(tokens=1 << 29), "tokens"), (dict(logits_dtype=1), "float32"), (dict(normalize=2), "normalize"),
+    (dict(logits_stride=15), "logits_stride")])
+def test_route_refuses(change, words):
+    d = C.byref(desc(D.RouteDesc, ROUTE, **change))
+    assert words in refused(D.library().b2vx_route_noalloc, d, PTR, PTR, PTR, PTR, PTR, PTR, PTR, 1 << 30, None)
+
+
+def test_route_refuses_pointers():
+    fn, d = D.library().b2vx_route_noalloc, C.byref(desc(D.RouteDesc, ROUTE))
+    for i in range(6):
+        args = [PTR] * 6
+        args[i] = None
+        assert "null" in refused(fn, d, *args, PTR, 1 << 20, None)
+    assert "workspace" in refused(fn, d, *[PTR] * 6, None, 1 << 20, None)
+    assert "workspace" in refused(fn, d, *[PTR] * 6, PTR + 8, 1 << 20, None)
+    assert "workspace" in refused(fn, d, *[PTR] * 6, PTR, 8, None)
+    assert "aligned" in refused(fn, d, PTR + 2, *[PTR] * 5, PTR, 1 << 20, None)
+
+
+@pytest.mark.parametrize("change,words", [
+    (dict(dtype=2), "float32"), (dict(tokens=1 << 30), "range"), (dict(z_stride=63), "stride"), (dict(y_stride=63), "stride"), (dict(residual_stride=63), "stride"),
+    (dict(z_stride=1 << 41), "stride")])
+def test_combine_refuses(change, words):
+    d = C.byref(desc(D.CombineDesc, COMBINE, **change))
+    assert words in refused(D.library().b2vx_combine_noalloc, d, PTR, PTR, PTR, PTR, PTR, None)
+
+
+def test_combine_refuses_pointers():
+    fn, d = D.library().b2vx_combine_noalloc, C.byref(desc(D.CombineDesc, COMBINE))
+    for args in ((None, PTR, PTR, PTR, PTR), (PTR, None, PTR, PTR, PTR), (PTR, PTR, None, PTR, PTR), (PTR, PTR, PTR, PTR, None)):
+        assert "null" in refused(fn, d, *args, None)
+    assert "aligned" in refused(fn, d, PTR + 1, PTR, PTR, PTR, PTR, None)
+
+
+def test_empty_calls_launch_nothing():
+    lib = D.library()
+    assert lib.b2vx_fp4_quantize_noalloc(C.byref(desc(D.QuantizeDesc, QUANTIZE, rows=0)), None, None, None, None, None, None, None, 0) == 0
+    assert lib.b2vx_fp4_dequantize_noalloc(C.byref(desc(D.DequantizeDesc, DEQUANTIZE, rows=0)), None, None, None, None, None, None, 0) == 0
+    assert lib.b2vx_linear_noalloc(C.byref(desc(D.LinearDesc, LINEAR, rows=0)), C.byref(D.LinearArgs()), None, None, 0) == 0
+    assert lib.b2vx_linear_noalloc(C.byref(desc(D.LinearDesc, LINEAR, n=0)), C.byref(D.LinearArgs()), None, None, 0) == 0
+    assert lib.b2vx_combine_noalloc(C.byref(desc(D.CombineDesc, COMBINE, tokens=0)), None, None, None, None, None, None, None, 0) == 0
+
+
+def packed_size(fmt, matrices, rows, k):
+    size = C.c_size_t()
+    assert D.library().b2vx_fp4_packed_scales_size_noalloc(fmt, matrices, rows, k, C.byref(size)) == 0
+    return size.value
+
+
+def test_sizes():
+    # tiles of 128 rows x 4 blocks of 512 bytes, K in steps of 256 columns
+    assert packed_size(1, 1, 128, 256) == 2 * 512
+    assert packed_size(2, 1, 128, 256) == 4 * 512
+    assert packed_size(1, 3, 129, 257) == 3 * 2 * 4 * 512
+    assert packed_size(1, 0, 5, 64) == 0
+    assert D.library().b2vx_fp4_packed_scales_size_noalloc(0, 1, 1, 1, C.byref(C.c_size_t())) == 1
+    size = C.c_size_t()
+    lib = D.library()
+    # codes of 8 rows, 48 bytes each, and scales of one tile for the rows and one for the group's own start
+    assert lib.b2vx_linear_workspace_size_noalloc(C.byref(desc(D.LinearDesc, LINEAR)), C.byref(size), None, 0) == 0
+    assert size.value == 512 + 2 * 2 * 512
+    assert lib.b2vx_linear_workspace_size_noalloc(C.byref(desc(D.LinearDesc, LINEAR, experts=5)), C.byref(size), None, 0) == 0
+    assert size.value == 512 + 6 * 2 * 512
+
+
+def test_group_scale_rows_do_not_overlap():
+    """The rule that gives every group of rows its own scale tiles: group e starts at roundup128(lo) + 128 e."""
+    import random
+    rng = random.Random(5)
+    up = lambda v: (v + 127) // 128 * 128
+    for _ in range(300):
+        counts = [rng.choice([0, 0, 1, 63, 127, 128, 129, rng.randrange(2000)]) for _ in range(rng.randrange(1, 40))]
+        lo, end = 0, 0
+        for e, n in enumerate(counts):
+            first = up(lo) + 128 * e
+            assert first >= end
+            end = first + up(n)
+            lo += n
+        assert end <= up(lo) + 128 * len(counts)
+
+
+def test_tensors_must_be_on_a_gpu():
+    torch = pytest.importorskip("torch")
+    with pytest.raises(ValueError, match="GPU"):
+        D.quantize_fp4(torch.zeros(2, 32))
+    with pytest.raises(ValueError, match="type"):
+        D.quantize_fp4(torch.zeros(2, 32, dtype=torch.float64))
+    with pytest.raises(ValueError, match="format"):
+        D.quantize_fp4(torch.zeros(2, 32), "block8")
+    with pytest.raises(ValueError, match="scale"):
+        D.quantize_fp4(torch.zeros(2, 32), "block16")
+    with pytest.raises(ValueError, match="last dimension"):
+        D.quantize_fp4(torch.zeros(32, 2).t())
+    with pytest.raises(ValueError, match="offsets"):
+        D.expert_linear(torch.zeros(2, 32, dtype=torch.bfloat16), torch.zeros(3, 8, 32, dtype=torch.bfloat16), None)
+    with pytest.raises(ValueError, match="columns"):
+        D.linear(torch.zeros(2, 32, dtype=torch.bfloat16), torch.zeros(8, 64, dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="two dimensions"):
+        D.combine_experts(torch.zeros(4, 8), torch.zeros(4, dtype=torch.int32), torch.zeros(4))

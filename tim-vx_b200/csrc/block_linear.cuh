@@ -1,0 +1,85 @@
+// What the host entry points (device_ops.cu) and the kernels of the operators on device tensors share: formats, layouts, launchers.
+#ifndef B2VX_BLOCK_LINEAR_CUH_
+#define B2VX_BLOCK_LINEAR_CUH_
+
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "b2vx.h"
+
+namespace b2vx {
+
+// Columns that share a scale.
+__host__ __device__ constexpr int fp4_block(int format) { return format == B2VX_FP4_BLOCK16 ? 16 : 32; }
+
+// Scales of a product's operand ("packed"): tiles of 128 rows x 4 blocks, 512 bytes each, which is the form the tensor pipe takes
+// its scales in.  Row r's four bytes of a tile lie at (r % 32) * 16 + (r / 32) * 4: a copy of the tile into tensor memory puts rows
+// 32 c .. 32 c + 31 into its column c.  Tiles run along K first, padded to whole pipeline stages of 256 columns.
+constexpr int kScaleTile = 512;
+constexpr int kStageBytes = 128;                       // bytes of K per row and pipeline stage
+constexpr int kMaxExperts = 1024;
+__host__ __device__ constexpr int scale_words_per_stage(int format) { return 256 / (4 * fp4_block(format)); }   // 2 or 4
+__host__ __device__ inline long long scale_words(long long k, int format) {
+  return (k + 255) / 256 * scale_words_per_stage(format);
+}
+__host__ __device__ inline size_t packed_scale_bytes(long long matrices, long long rows, long long k, int format) {
+  return static_cast<size_t>(matrices) * ((rows + 127) / 128) * scale_words(k, format) * kScaleTile;
+}
+// Rows of the packed scales of an operand whose rows belong to `experts` groups: each group starts on a tile of its own.  Group e,
+// whose first row is lo, starts at scale row expert_scale_row(lo, e); since roundup(a) + roundup(b) <= roundup(a + b) + 128, groups do
+// not overlap and the space ends at expert_scale_rows.
+__host__ __device__ inline long long expert_scale_row(long long lo, long long e) { return (lo + 127) / 128 * 128 + 128 * e; }
+__host__ __device__ inline long long expert_scale_rows(long long rows, long long experts) { return (rows + 127) / 128 * 128 + 128 * experts; }
+
+struct QuantizeArgs {
+  const void* x;
+  int x_dtype;
+  long long x_stride;          // elements
+  long long x_rows;            // rows of x (bound of row_index)
+  long long rows, k;
+  const int32_t* row_index;    // or null
+  const float* tensor_scale;   // block16
+  int format;
+  uint8_t* codes;
+  long long codes_pitch;       // bytes
+  uint8_t* scales;
+  long long scales_pitch;      // bytes; 0: packed
+  const int32_t* offsets;      // packed: the groups, or null for one group of all rows
+  int experts;
+};
+cudaError_t launch_fp4_quantize(const QuantizeArgs& a, cudaStream_t s);
+cudaError_t launch_fp4_dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
+                                  const float* tensor_scale, int format, long long rows, long long k, void* y, int y_dtype,
+                                  long long y_stride, cudaStream_t s);
+cudaError_t launch_fp4_pack_scales(const uint8_t* scales, int format, long long matrices, long long n, long long k, uint8_t* packed, cudaStream_t s);
+// rows of 16-bit numbers, gathered: y[i] = x[row_index[i]] (zeros where the index is out of range), K contiguous in y
+cudaError_t launch_gather_rows(const void* x, long long x_stride, long long x_rows, const int32_t* row_index, long long rows, long long k,
+                               void* y, cudaStream_t s);
+
+struct LinearArgs {
+  int format;                  // 0: 16-bit numbers of x_dtype, else B2VX_FP4_*
+  int x_dtype, y_dtype;
+  long long rows;              // rows of the operand x and of y
+  long long n, k;
+  int experts;                 // groups; 1 with offsets == null: one product
+  int gated;
+  const void* x;               // codes or 16-bit numbers
+  long long x_pitch;           // bytes
+  const uint8_t* x_scales;     // packed
+  const void* w;
+  const uint8_t* w_scales;     // packed
+  const float* x_scale;        // tensor scales, or null
+  const float* w_scale;
+  const float* bias;
+  const int32_t* offsets;
+  void* y;
+  long long y_stride;          // elements
+  int* status;
+  int sm_count;
+};
+cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why);
+
+}  // namespace b2vx
+#endif  // B2VX_BLOCK_LINEAR_CUH_

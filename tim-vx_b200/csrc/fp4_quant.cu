@@ -1,0 +1,237 @@
+// Rows of numbers to 4-bit block floating point and back, packing of scales, gathering of rows.
+//
+// Quantization reads every number once and writes half a byte and a scale's share for it; it is bound by memory (a block is 16 or 32
+// neighbouring columns, 2 or 4 lanes of eight columns each, so its maximum costs one or two shuffles).  Eight numbers a lane:
+// one 16-byte load of 16-bit numbers, one 4-byte store of codes, 128 bytes a warp.
+#include <algorithm>
+
+#include "block_linear.cuh"
+#include "fp4.cuh"
+#include "pdl.cuh"
+
+namespace b2vx {
+namespace {
+
+constexpr int kWarps = 8;
+constexpr int kChunk = 256;   // columns of a warp per step, one pipeline stage of the products
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
+  else return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_float(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
+
+// Eight numbers from column c on, zeros from column k on.  VEC: rows start on 16 bytes, so whole pieces load in 16 bytes.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_8(const T* row, long long c, long long k, float (&v)[8]) {
+  if (VEC && c + 8 <= k) {
+    alignas(16) T t[8];
+    const uint4* src = reinterpret_cast<const uint4*>(row + c);
+    *reinterpret_cast<uint4*>(t) = __ldg(src);
+    if (sizeof(T) == 4) *reinterpret_cast<uint4*>(t + 4) = __ldg(src + 1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_float(t[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c + i < k ? to_float(row[c + i]) : 0.0f;
+  }
+}
+
+// The group of a row: how many groups end at or before it.
+__device__ __forceinline__ int group_of(const int32_t* offsets, int experts, long long row, int lane) {
+  int n = 0;
+  for (int e = lane; e < experts; e += 32) n += offsets[e + 1] <= row;
+  return __reduce_add_sync(0xffffffffu, n);
+}
+
+// `split` warps share a row, each taking every split-th chunk.
+template <typename T, int FORMAT, bool VEC, bool PACKED>
+__global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArgs a, int chunks, int split) {
+  constexpr int B = fp4_block(FORMAT), LANES = B / 8;
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const long long warps = static_cast<long long>(gridDim.x) * kWarps;
+  const float g = FORMAT == B2VX_FP4_BLOCK16 ? __ldg(a.tensor_scale) : 1.0f;
+  const long long k32 = (a.k + 31) / 32 * 32, blocks = (a.k + B - 1) / B;
+  const T* x = static_cast<const T*>(a.x);
+  for (long long unit = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5); unit < a.rows * split; unit += warps) {
+    const long long row = split == 1 ? unit : unit / split;
+    const int part = split == 1 ? 0 : static_cast<int>(unit - row * split);
+    const long long src = a.row_index ? a.row_index[row] : row;
+    const bool there = src >= 0 && src < a.x_rows;
+    const T* from = x + (there ? src : 0) * a.x_stride;
+    const long long k_here = there ? a.k : 0;
+    uint8_t* tile = nullptr;      // PACKED: where the row's words of the first scale tile lie; null: the row belongs to no group
+    if (PACKED) {
+      long long at = row;
+      if (a.offsets) {
+        const int e = group_of(a.offsets, a.experts, row, lane);
+        const long long lo = e < a.experts ? a.offsets[e] : -1;
+        at = lo >= 0 && lo <= row ? expert_scale_row(lo, e) + row - lo : -1;
+      }
+      if (at >= 0) tile = a.scales + (at / 128) * scale_words(a.k, FORMAT) * kScaleTile + (at % 32) * 16 + (at % 128 / 32) * 4;
+    }
+    for (int chunk = part; chunk < chunks; chunk += split) {
+      const long long c = static_cast<long long>(chunk) * kChunk + lane * 8;
+      float v[8];
+      load_8<T, VEC>(from, c, k_here, v);
+      uint32_t byte;
+      const uint32_t codes = quantize_8<FORMAT>(v, g, byte);
+      if (c < k32) *reinterpret_cast<uint32_t*>(a.codes + row * a.codes_pitch + c / 2) = codes;
+      if (PACKED) {
+        if (c >= a.k) byte = 0;
+        uint32_t word = byte | __shfl_down_sync(0xffffffffu, byte, LANES) << 8;
+        word |= __shfl_down_sync(0xffffffffu, word, 2 * LANES) << 16;
+        if (lane % (4 * LANES) == 0 && tile)
+          *reinterpret_cast<uint32_t*>(tile + (static_cast<long long>(chunk) * scale_words_per_stage(FORMAT) + lane / (4 * LANES)) * kScaleTile) = word;
+      } else if (lane % LANES == 0 && c / B < blocks) {
+        a.scales[row * a.scales_pitch + c / B] = static_cast<uint8_t>(byte);
+      }
+    }
+  }
+}
+
+template <typename T, int FORMAT>
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
+                                                         const float* tensor_scale, long long rows, long long k, T* y, long long y_stride,
+                                                         int pieces, int vec) {
+  constexpr int B = fp4_block(FORMAT);
+  pdl_trigger();
+  pdl_wait();
+  const float g = FORMAT == B2VX_FP4_BLOCK16 ? __ldg(tensor_scale) : 1.0f;
+  const long long total = rows * pieces, step = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
+    const long long row = i / pieces, c = (i - row * pieces) * 8;
+    const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(codes + row * codes_pitch + c / 2));
+    const float s = scale_value<FORMAT>(__ldg(scales + row * scales_pitch + c / B));
+    float v[8];
+    e2m1_values(word, v);
+    alignas(16) T out[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) out[j] = from_float<T>(FORMAT == B2VX_FP4_BLOCK16 ? v[j] * s * g : v[j] * s);
+    T* dst = y + row * y_stride + c;
+    if (vec && c + 8 <= k) {
+      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(out);
+      if (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + 4) = *reinterpret_cast<const uint4*>(out + 4);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < k) dst[j] = out[j];
+    }
+  }
+}
+
+// One thread per word (four blocks of a row) of the packed layout.
+__global__ void __launch_bounds__(256) pack_scales_kernel(const uint8_t* scales, long long matrices, long long n, long long blocks, long long words,
+                                                          uint32_t* packed) {
+  pdl_trigger();
+  pdl_wait();
+  const long long tiles = (n + 127) / 128, total = matrices * tiles * words * 128, step = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
+    const int in = static_cast<int>(i & 127);
+    const long long w = (i >> 7) % words, t = (i >> 7) / words % tiles, m = (i >> 7) / words / tiles;
+    const long long row = t * 128 + (in & 3) * 32 + (in >> 2);
+    uint32_t word = 0;
+    if (row < n)
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (w * 4 + b < blocks) word |= static_cast<uint32_t>(scales[(m * n + row) * blocks + w * 4 + b]) << (8 * b);
+    packed[i] = word;
+  }
+}
+
+__global__ void __launch_bounds__(256) gather_rows_kernel(const uint16_t* x, long long x_stride, long long x_rows, const int32_t* row_index,
+                                                          long long rows, long long k, int pieces, uint4* y, int vec) {
+  pdl_trigger();
+  pdl_wait();
+  const long long total = rows * pieces, step = static_cast<long long>(gridDim.x) * blockDim.x;
+  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
+    const long long row = i / pieces, c = (i - row * pieces) * 8;
+    const long long src = row_index ? row_index[row] : row;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (src >= 0 && src < x_rows) {
+      const uint16_t* from = x + src * x_stride + c;
+      if (vec) {
+        v = __ldg(reinterpret_cast<const uint4*>(from));
+      } else {
+        alignas(16) uint16_t t[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = from[j];
+        v = *reinterpret_cast<const uint4*>(t);
+      }
+    }
+    y[i] = v;
+  }
+}
+
+int blocks_for(long long threads, int per_block) {
+  return static_cast<int>(std::max<long long>(1, std::min<long long>((threads + per_block - 1) / per_block, 148 * 8)));
+}
+
+template <typename T, int FORMAT, bool VEC>
+cudaError_t quantize(const QuantizeArgs& a, cudaStream_t s) {
+  const int chunks = static_cast<int>((a.k + kChunk - 1) / kChunk);
+  // a row to a warp where the rows fill the GPU (8 blocks an SM), else shared by up to as many warps as it has chunks
+  const long long fill = 148 * 8 * kWarps;
+  const int split = static_cast<int>(std::max<long long>(1, std::min<long long>(chunks, fill / std::max<long long>(1, a.rows))));
+  const int grid = blocks_for(a.rows * split, kWarps);
+  if (a.scales_pitch == 0) return launch_pdl(quantize_kernel<T, FORMAT, VEC, true>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
+  return launch_pdl(quantize_kernel<T, FORMAT, VEC, false>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
+}
+template <typename T, int FORMAT>
+cudaError_t quantize_vec(const QuantizeArgs& a, cudaStream_t s) {
+  const bool vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && (a.x_stride * sizeof(T)) % 16 == 0;
+  return vec ? quantize<T, FORMAT, true>(a, s) : quantize<T, FORMAT, false>(a, s);
+}
+template <typename T>
+cudaError_t quantize_format(const QuantizeArgs& a, cudaStream_t s) {
+  return a.format == B2VX_FP4_BLOCK32 ? quantize_vec<T, B2VX_FP4_BLOCK32>(a, s) : quantize_vec<T, B2VX_FP4_BLOCK16>(a, s);
+}
+template <typename T>
+cudaError_t dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch, const float* tensor_scale, int format,
+                       long long rows, long long k, void* y, long long y_stride, cudaStream_t s) {
+  const int pieces = static_cast<int>((k + 7) / 8);
+  const int vec = reinterpret_cast<uintptr_t>(y) % 16 == 0 && (y_stride * sizeof(T)) % 16 == 0;
+  const int grid = blocks_for(rows * pieces, 256);
+  auto* kernel = format == B2VX_FP4_BLOCK32 ? dequantize_kernel<T, B2VX_FP4_BLOCK32> : dequantize_kernel<T, B2VX_FP4_BLOCK16>;
+  return launch_pdl(kernel, dim3(grid), dim3(256), 0, s, codes, codes_pitch, scales, scales_pitch, tensor_scale, rows, k, static_cast<T*>(y), y_stride,
+                    pieces, vec);
+}
+
+}  // namespace
+
+cudaError_t launch_fp4_quantize(const QuantizeArgs& a, cudaStream_t s) {
+  if (a.x_dtype == B2VX_DT_FLOAT32) return quantize_format<float>(a, s);
+  if (a.x_dtype == B2VX_DT_FLOAT16) return quantize_format<__half>(a, s);
+  return quantize_format<__nv_bfloat16>(a, s);
+}
+cudaError_t launch_fp4_dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
+                                  const float* tensor_scale, int format, long long rows, long long k, void* y, int y_dtype,
+                                  long long y_stride, cudaStream_t s) {
+  if (y_dtype == B2VX_DT_FLOAT32) return dequantize<float>(codes, codes_pitch, scales, scales_pitch, tensor_scale, format, rows, k, y, y_stride, s);
+  if (y_dtype == B2VX_DT_FLOAT16) return dequantize<__half>(codes, codes_pitch, scales, scales_pitch, tensor_scale, format, rows, k, y, y_stride, s);
+  return dequantize<__nv_bfloat16>(codes, codes_pitch, scales, scales_pitch, tensor_scale, format, rows, k, y, y_stride, s);
+}
+cudaError_t launch_fp4_pack_scales(const uint8_t* scales, int format, long long matrices, long long n, long long k, uint8_t* packed, cudaStream_t s) {
+  const long long blocks = (k + fp4_block(format) - 1) / fp4_block(format), words = scale_words(k, format);
+  const long long total = static_cast<long long>(packed_scale_bytes(matrices, n, k, format) / 4);
+  return launch_pdl(pack_scales_kernel, dim3(blocks_for(total, 256)), dim3(256), 0, s, scales, matrices, n, blocks, words,
+                    reinterpret_cast<uint32_t*>(packed));
+}
+cudaError_t launch_gather_rows(const void* x, long long x_stride, long long x_rows, const int32_t* row_index, long long rows, long long k, void* y,
+                               cudaStream_t s) {
+  const int pieces = static_cast<int>(k / 8);
+  const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && x_stride % 8 == 0;
+  return launch_pdl(gather_rows_kernel, dim3(blocks_for(rows * pieces, 256)), dim3(256), 0, s, static_cast<const uint16_t*>(x), x_stride, x_rows,
+                    row_index, rows, k, pieces, static_cast<uint4*>(y), vec);
+}
+
+}  // namespace b2vx
