@@ -5,6 +5,7 @@ import ctypes as C
 
 import pytest
 
+import device_ops_abi as ABI
 import deviceops as D
 
 PTR = 1 << 20   # an address that is aligned to everything; never read
@@ -39,19 +40,19 @@ def refused(fn, *args):
     (dict(codes_pitch=44), None, "codes_pitch"), (dict(codes_pitch=49), None, "codes_pitch"), (dict(scales_pitch=2), None, "scales_pitch"),
     (dict(format=2, scales_pitch=6), None, "tensor scale"), (dict(), PTR, "tensor scale"), (dict(rows=9), None, "row_index")])
 def test_quantize_refuses(change, scale, words):
-    fn = D.library().b2vx_fp4_quantize_noalloc
-    assert words in refused(fn, C.byref(desc(D.QuantizeDesc, QUANTIZE, **change)), PTR, None, scale, PTR, PTR, None)
+    fn = ABI.library().b2vx_fp4_quantize_noalloc
+    assert words in refused(fn, C.byref(desc(ABI.QuantizeDesc, QUANTIZE, **change)), PTR, None, scale, PTR, PTR, None)
 
 
 def test_quantize_refuses_pointers():
-    fn = D.library().b2vx_fp4_quantize_noalloc
-    d = C.byref(desc(D.QuantizeDesc, QUANTIZE))
+    fn = ABI.library().b2vx_fp4_quantize_noalloc
+    d = C.byref(desc(ABI.QuantizeDesc, QUANTIZE))
     assert "null" in refused(fn, None, PTR, None, None, PTR, PTR, None)
     for args in ((None, None, None, PTR, PTR, None), (PTR, None, None, None, PTR, None), (PTR, None, None, PTR, None, None)):
         assert "null" in refused(fn, d, *args)
     assert "aligned" in refused(fn, d, PTR + 1, None, None, PTR, PTR, None)
     assert "aligned" in refused(fn, d, PTR, None, None, PTR + 2, PTR, None)
-    packed = C.byref(desc(D.QuantizeDesc, QUANTIZE, scales_layout=1))
+    packed = C.byref(desc(ABI.QuantizeDesc, QUANTIZE, scales_layout=1))
     assert "aligned" in refused(fn, packed, PTR, None, None, PTR, PTR + 4, None)
 
 
@@ -60,13 +61,13 @@ def test_quantize_refuses_pointers():
     (dict(scales_pitch=1), None, "scales_pitch"), (dict(y_stride=95), None, "y_stride"), (dict(format=2, scales_pitch=6), None, "tensor scale"),
     (dict(), PTR, "tensor scale")])
 def test_dequantize_refuses(change, scale, words):
-    fn = D.library().b2vx_fp4_dequantize_noalloc
-    assert words in refused(fn, C.byref(desc(D.DequantizeDesc, DEQUANTIZE, **change)), PTR, PTR, scale, PTR, None)
+    fn = ABI.library().b2vx_fp4_dequantize_noalloc
+    assert words in refused(fn, C.byref(desc(ABI.DequantizeDesc, DEQUANTIZE, **change)), PTR, PTR, scale, PTR, None)
 
 
 def test_dequantize_refuses_pointers():
-    fn = D.library().b2vx_fp4_dequantize_noalloc
-    d = C.byref(desc(D.DequantizeDesc, DEQUANTIZE))
+    fn = ABI.library().b2vx_fp4_dequantize_noalloc
+    d = C.byref(desc(ABI.DequantizeDesc, DEQUANTIZE))
     for args in ((None, PTR, None, PTR, None), (PTR, None, None, PTR, None), (PTR, PTR, None, None, None)):
         assert "null" in refused(fn, d, *args)
     assert "aligned" in refused(fn, d, PTR, PTR, None, PTR + 1, None)
@@ -79,10 +80,10 @@ def test_dequantize_refuses_pointers():
     (dict(rows=1 << 28, x_rows=1 << 28, n=1 << 20, y_stride=1 << 20), "tiles")])
 def test_linear_refuses(change, words):
     size = C.c_size_t()
-    d = desc(D.LinearDesc, LINEAR, **change)
-    assert words in refused(D.library().b2vx_linear_workspace_size_noalloc, C.byref(d), C.byref(size))
-    args = D.LinearArgs(PTR, PTR, PTR, None, None, None, None, None, PTR, PTR, 1 << 30)
-    assert words in refused(D.library().b2vx_linear_noalloc, C.byref(d), C.byref(args), None)
+    d = desc(ABI.LinearDesc, LINEAR, **change)
+    assert words in refused(ABI.library().b2vx_linear_workspace_size_noalloc, C.byref(d), C.byref(size))
+    args = ABI.LinearArgs(PTR, PTR, PTR, None, None, None, None, None, PTR, PTR, 1 << 30)
+    assert words in refused(ABI.library().b2vx_linear_noalloc, C.byref(d), C.byref(args), None)
 
 
 @pytest.mark.parametrize("change,args,words", [
@@ -93,9 +94,9 @@ def test_linear_refuses(change, words):
     (dict(), dict(workspace=None), "workspace"), (dict(), dict(workspace=PTR + 16), "workspace"), (dict(), dict(workspace_bytes=100), "workspace"),
     (dict(w_format=0), dict(row_index=PTR, workspace_bytes=0), "workspace"), (dict(w_format=0, x_stride=100), dict(workspace=None), "workspace")])
 def test_linear_refuses_arguments(change, args, words):
-    d = desc(D.LinearDesc, LINEAR, **change)
-    a = desc(D.LinearArgs, dict(x=PTR, w=PTR, w_scales=PTR, y=PTR, workspace=PTR, workspace_bytes=1 << 30), **args)
-    assert words in refused(D.library().b2vx_linear_noalloc, C.byref(d), C.byref(a), None)
+    d = desc(ABI.LinearDesc, LINEAR, **change)
+    a = desc(ABI.LinearArgs, dict(x=PTR, w=PTR, w_scales=PTR, y=PTR, workspace=PTR, workspace_bytes=1 << 30), **args)
+    assert words in refused(ABI.library().b2vx_linear_noalloc, C.byref(d), C.byref(a), None)
 
 
 @pytest.mark.parametrize("change,words", [
@@ -103,12 +104,12 @@ def test_linear_refuses_arguments(change, args, words):
     (dict(experts=64, logits_stride=64, top_k=33), "top_k"), (dict(tokens=1 << 29), "tokens"), (dict(logits_dtype=1), "float32"), (dict(normalize=2), "normalize"),
     (dict(logits_stride=15), "logits_stride")])
 def test_route_refuses(change, words):
-    d = C.byref(desc(D.RouteDesc, ROUTE, **change))
-    assert words in refused(D.library().b2vx_route_noalloc, d, PTR, PTR, PTR, PTR, PTR, PTR, PTR, 1 << 30, None)
+    d = C.byref(desc(ABI.RouteDesc, ROUTE, **change))
+    assert words in refused(ABI.library().b2vx_route_noalloc, d, PTR, PTR, PTR, PTR, PTR, PTR, PTR, 1 << 30, None)
 
 
 def test_route_refuses_pointers():
-    fn, d = D.library().b2vx_route_noalloc, C.byref(desc(D.RouteDesc, ROUTE))
+    fn, d = ABI.library().b2vx_route_noalloc, C.byref(desc(ABI.RouteDesc, ROUTE))
     for i in range(6):
         args = [PTR] * 6
         args[i] = None
@@ -123,29 +124,29 @@ def test_route_refuses_pointers():
     (dict(dtype=2), "float32"), (dict(tokens=1 << 30), "range"), (dict(z_stride=63), "stride"), (dict(y_stride=63), "stride"), (dict(residual_stride=63), "stride"),
     (dict(z_stride=1 << 41), "stride")])
 def test_combine_refuses(change, words):
-    d = C.byref(desc(D.CombineDesc, COMBINE, **change))
-    assert words in refused(D.library().b2vx_combine_noalloc, d, PTR, PTR, PTR, PTR, PTR, None)
+    d = C.byref(desc(ABI.CombineDesc, COMBINE, **change))
+    assert words in refused(ABI.library().b2vx_combine_noalloc, d, PTR, PTR, PTR, PTR, PTR, None)
 
 
 def test_combine_refuses_pointers():
-    fn, d = D.library().b2vx_combine_noalloc, C.byref(desc(D.CombineDesc, COMBINE))
+    fn, d = ABI.library().b2vx_combine_noalloc, C.byref(desc(ABI.CombineDesc, COMBINE))
     for args in ((None, PTR, PTR, PTR, PTR), (PTR, None, PTR, PTR, PTR), (PTR, PTR, None, PTR, PTR), (PTR, PTR, PTR, PTR, None)):
         assert "null" in refused(fn, d, *args, None)
     assert "aligned" in refused(fn, d, PTR + 1, PTR, PTR, PTR, PTR, None)
 
 
 def test_empty_calls_launch_nothing():
-    lib = D.library()
-    assert lib.b2vx_fp4_quantize_noalloc(C.byref(desc(D.QuantizeDesc, QUANTIZE, rows=0)), None, None, None, None, None, None, None, 0) == 0
-    assert lib.b2vx_fp4_dequantize_noalloc(C.byref(desc(D.DequantizeDesc, DEQUANTIZE, rows=0)), None, None, None, None, None, None, 0) == 0
-    assert lib.b2vx_linear_noalloc(C.byref(desc(D.LinearDesc, LINEAR, rows=0)), C.byref(D.LinearArgs()), None, None, 0) == 0
-    assert lib.b2vx_linear_noalloc(C.byref(desc(D.LinearDesc, LINEAR, n=0)), C.byref(D.LinearArgs()), None, None, 0) == 0
-    assert lib.b2vx_combine_noalloc(C.byref(desc(D.CombineDesc, COMBINE, tokens=0)), None, None, None, None, None, None, None, 0) == 0
+    lib = ABI.library()
+    assert lib.b2vx_fp4_quantize_noalloc(C.byref(desc(ABI.QuantizeDesc, QUANTIZE, rows=0)), None, None, None, None, None, None, None, 0) == 0
+    assert lib.b2vx_fp4_dequantize_noalloc(C.byref(desc(ABI.DequantizeDesc, DEQUANTIZE, rows=0)), None, None, None, None, None, None, 0) == 0
+    assert lib.b2vx_linear_noalloc(C.byref(desc(ABI.LinearDesc, LINEAR, rows=0)), C.byref(ABI.LinearArgs()), None, None, 0) == 0
+    assert lib.b2vx_linear_noalloc(C.byref(desc(ABI.LinearDesc, LINEAR, n=0)), C.byref(ABI.LinearArgs()), None, None, 0) == 0
+    assert lib.b2vx_combine_noalloc(C.byref(desc(ABI.CombineDesc, COMBINE, tokens=0)), None, None, None, None, None, None, None, 0) == 0
 
 
 def packed_size(fmt, matrices, rows, k):
     size = C.c_size_t()
-    assert D.library().b2vx_fp4_packed_scales_size_noalloc(fmt, matrices, rows, k, C.byref(size)) == 0
+    assert ABI.library().b2vx_fp4_packed_scales_size_noalloc(fmt, matrices, rows, k, C.byref(size)) == 0
     return size.value
 
 
@@ -155,13 +156,13 @@ def test_sizes():
     assert packed_size(2, 1, 128, 256) == 4 * 512
     assert packed_size(1, 3, 129, 257) == 3 * 2 * 4 * 512
     assert packed_size(1, 0, 5, 64) == 0
-    assert D.library().b2vx_fp4_packed_scales_size_noalloc(0, 1, 1, 1, C.byref(C.c_size_t())) == 1
+    assert ABI.library().b2vx_fp4_packed_scales_size_noalloc(0, 1, 1, 1, C.byref(C.c_size_t())) == 1
     size = C.c_size_t()
-    lib = D.library()
+    lib = ABI.library()
     # codes of 8 rows, 48 bytes each, and scales of one tile for the rows and one for the group's own start
-    assert lib.b2vx_linear_workspace_size_noalloc(C.byref(desc(D.LinearDesc, LINEAR)), C.byref(size), None, 0) == 0
+    assert lib.b2vx_linear_workspace_size_noalloc(C.byref(desc(ABI.LinearDesc, LINEAR)), C.byref(size), None, 0) == 0
     assert size.value == 512 + 2 * 2 * 512
-    assert lib.b2vx_linear_workspace_size_noalloc(C.byref(desc(D.LinearDesc, LINEAR, experts=5)), C.byref(size), None, 0) == 0
+    assert lib.b2vx_linear_workspace_size_noalloc(C.byref(desc(ABI.LinearDesc, LINEAR, experts=5)), C.byref(size), None, 0) == 0
     assert size.value == 512 + 6 * 2 * 512
 
 

@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 import torch
 
+import device_ops_abi as ABI
 import deviceops as D
 
 pytestmark = pytest.mark.gpu
@@ -217,14 +218,14 @@ def test_packed_layout(fmt, rows, k):
     s = scale_for(f64(x), fmt)
     q = D.quantize_fp4(x, fmt, scale=s)
     size = C.c_size_t()
-    lib, f, b = D.library(), D.FORMATS[fmt], D.BLOCK[fmt]
+    lib, f, b = ABI.library(), D.FORMATS[fmt], D.BLOCK[fmt]
     assert lib.b2vx_fp4_packed_scales_size_noalloc(f, 1, rows, k, C.byref(size)) == 0
     direct = torch.full((size.value,), 0xAB, dtype=torch.uint8, device="cuda")
     later = torch.full((size.value,), 0xCD, dtype=torch.uint8, device="cuda")
     codes = torch.empty_like(q.codes)
-    d = D.QuantizeDesc(f, 1, 16, rows, rows, k, k, codes.shape[1], 0)
-    D._call(lib.b2vx_fp4_quantize_noalloc, C.byref(d), x.data_ptr(), None, None if s is None else s.data_ptr(), codes.data_ptr(), direct.data_ptr(), None)
-    D._call(lib.b2vx_fp4_pack_scales_noalloc, f, 1, rows, k, q.scales.data_ptr(), later.data_ptr(), None)
+    d = ABI.QuantizeDesc(f, 1, 16, rows, rows, k, k, codes.shape[1], 0)
+    ABI.call(lib.b2vx_fp4_quantize_noalloc, C.byref(d), x.data_ptr(), None, None if s is None else s.data_ptr(), codes.data_ptr(), direct.data_ptr(), None)
+    ABI.call(lib.b2vx_fp4_pack_scales_noalloc, f, 1, rows, k, q.scales.data_ptr(), later.data_ptr(), None)
     torch.cuda.synchronize()
     assert torch.equal(codes, q.codes)
     words = (k + 255) // 256 * (256 // (4 * b))

@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "block_linear.cuh"
 #include "pdl.cuh"
@@ -33,6 +34,8 @@ constexpr int kEpilogueWarps = 8;
 constexpr int kMaxStages = 10;
 constexpr int kBoxRows = 32;
 constexpr int kSmemBudget = 224 * 1024;
+constexpr int kMaxDynSmem = 227 * 1024;
+constexpr int kMaxDevices = 64;
 constexpr int kMinDynSmem = 120 * 1024;   // keeps two CTAs from sharing an SM and its tensor memory
 
 struct LinearParams {
@@ -411,8 +414,16 @@ bool encode_rows(CUtensorMap* map, const void* base, int rank, uint64_t kbytes, 
 template <int KIND, int P, typename T>
 cudaError_t start(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
   auto* kernel = block_linear_kernel<KIND, P, T>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  // once per GPU (a repeated setting by racing first calls does no harm): the attribute costs a call a microsecond of the host's time
+  static std::atomic<bool> ready[kMaxDevices];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (dev >= kMaxDevices || !ready[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices) ready[dev].store(true, std::memory_order_release);
+  }
   return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, s, w, x, p);
 }
 template <int KIND, int P>

@@ -48,12 +48,11 @@ bool aligned(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % 
 size_t round256(size_t n) { return (n + 255) & ~static_cast<size_t>(255); }
 
 b2vx_status device(PerDevice** out, char* err, size_t err_len) {
-  int dev = 0, count = 0;
-  if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) {
     cudaGetLastError();
     return fail(err, err_len, B2VX_CUDA_ERROR, "no CUDA device");
   }
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return fail(err, err_len, B2VX_CUDA_ERROR, "no current CUDA device");
   std::call_once(g_registered, [] { g_register_error = cudaHostRegister(g_status, sizeof(g_status), cudaHostRegisterPortable | cudaHostRegisterMapped); });
   PerDevice& d = g_devices[dev];
   std::call_once(d.once, [&] {
