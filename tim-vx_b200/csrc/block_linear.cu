@@ -12,7 +12,7 @@
 //                          the packed scales
 //   warp 1      issuer     copies a stage's scales into tensor memory (tcgen05.cp, two slots in turn) and issues the stage's
 //                          four K steps of 32 bytes for each of the P accumulators
-//   warps 4-11  epilogue   a thread owns one feature (TMEM lane) and every second block of 16 rows
+//   warps 4-11  epilogue   out of tensor memory, scale and bias, activation, rounding, stores
 // Every wait is bounded as in gemm_tc.cu: on a time-out the CTA records a code and leaves through its common exit.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -46,7 +46,7 @@ struct LinearParams {
   int k_stages, stages, acc_bufs;
   int sfb_atoms;              // most scale tiles of x under one tile's rows
   int words;                  // scale words (tiles along K) of a row tile
-  uint32_t stage_bytes;
+  uint32_t stage_bytes, slab_bytes;
   uint32_t idesc;             // without N
   uint32_t acc_cols;          // TMEM columns of one accumulator buffer
   uint32_t sf_cols, sf_base;  // TMEM columns of a scale slot, first column of the slots
@@ -59,6 +59,7 @@ struct LinearParams {
   void* y;
   long long y_stride;
   int y_dtype;
+  int y_vec;                  // rows of y start on 16 bytes
   int* status;
 };
 
@@ -113,23 +114,56 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
   }
 }
 // Lane t of the warp gets 16 columns of TMEM lane t.
-__device__ __forceinline__ void load_16_columns(uint32_t taddr, float (&v)[16]) {
-  uint32_t r[16];
+__device__ __forceinline__ void load_lane_columns(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
         "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr)
       : "memory");
-  // the registers are valid after the wait; naming them there keeps their uses behind it
+}
+// 16 lanes x 8 N columns, N = 2 or 4: of column group h, thread t gets columns 2 (t % 4), + 1 of lane t / 4 in r[4 h], r[4 h + 1] and of lane
+// t / 4 + 8 in r[4 h + 2], r[4 h + 3].
+__device__ __forceinline__ void load_16_lanes(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void load_16_lanes(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+// The registers of a load are valid after the wait; naming them there keeps their uses behind it.
+__device__ __forceinline__ void loads_done(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
                : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
                  "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                :
                : "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void loads_done(uint32_t (&r)[8]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
+               :
+               : "memory");
+}
+// Four 8 x 8 matrices of 16-bit numbers to shared memory, transposed: lane i gives the address of row i % 8 of matrix i / 8.
+__device__ __forceinline__ void store_transposed(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// A barrier of the epilogue warps that also tells every one of them whether all came with ok.
+__device__ __forceinline__ bool epilogue_all(bool ok) {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"(static_cast<uint32_t>(ok)), "n"(kEpilogueWarps * 32) : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps * 32) : "memory"); }
 
 // One tile of the schedule: group, first row inside it, rows (as the instruction's N and as they are), feature tile.
 struct Tile {
@@ -155,11 +189,16 @@ __device__ __forceinline__ Tile tile_of(const int* lo, const int* start, const L
 }
 
 template <typename T>
-__device__ __forceinline__ T to_out(float v) {
-  if constexpr (sizeof(T) == 4) return v;
-  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
-  else return __float2bfloat16_rn(v);
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
 }
+__device__ __forceinline__ float gate(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
 template <int KIND, int P, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -170,7 +209,8 @@ block_linear_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   pdl_trigger();
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t ring = (raw + 1023u) & ~1023u;
-  Header* h = reinterpret_cast<Header*>(smem_raw + (ring - raw) + p.stages * p.stage_bytes);
+  const uint32_t staging = ring + p.stages * p.stage_bytes;       // two slabs of the epilogue
+  Header* h = reinterpret_cast<Header*>(smem_raw + (staging - raw) + 2 * p.slab_bytes);
   int* lo = reinterpret_cast<int*>(h + 1);
   int* start = lo + p.experts + 1;
   volatile int* abort_flag = &h->abort_flag;
@@ -338,56 +378,148 @@ block_linear_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
   } else if (warp >= kFirstEpilogueWarp) {
     // ------------------------------------------------------------ epilogue
     const int ew = warp - kFirstEpilogueWarp, quarter = ew & 3, half = ew >> 2;
-    const int fl = quarter * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     T* y = static_cast<T*>(p.y);
-    bool ok = true;
-    int j = 0;
-    for (int t = blockIdx.x; ok && t < num_tiles; t += gridDim.x, ++j) {
+    const bool gated = P == 2 && p.gated;
+    int j = 0, slab = 0;
+    for (int t = blockIdx.x; t < num_tiles; t += gridDim.x, ++j) {
       const Tile tile = tile_of(lo, start, p, t);
       const int buf = p.acc_bufs == 2 ? (j & 1) : 0;
       const uint32_t buf_ph = p.acc_bufs == 2 ? (j >> 1) & 1 : j & 1;
       float alpha = 1.0f;
       if (p.x_scale) alpha = __ldg(p.x_scale);
       if (p.w_scale) alpha *= __ldg(p.w_scale + tile.e);
-      int f[P];
-      float bias[P];
-#pragma unroll
-      for (int q = 0; q < P; ++q) {
-        f[q] = p.gated ? tile.f * 128 + fl : (tile.f * P + q) * 128 + fl;
-        bias[q] = p.bias && f[q] < p.n ? __ldg(p.bias + (p.gated ? (2ll * tile.e + q) * p.n : static_cast<long long>(tile.e) * p.n) + f[q]) : 0.0f;
-      }
-      ok = mbar_wait(smem_u32(&h->acc_full[buf]), buf_ph, abort_flag, p.status, 104);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      fence_after();
-      const uint32_t taddr = tmem + buf * p.acc_cols + (static_cast<uint32_t>(quarter * 32) << 16);
+      const uint32_t taddr = tmem + buf * p.acc_cols + lanes;
       const long long row0 = static_cast<long long>(tile.lo) + tile.r0;
-      for (int c = half * 16; c < tile.rows; c += 32) {
-        float v[P][16];
+      const int f0 = gated ? tile.f * 128 : tile.f * P * 128;             // first feature of the tile
+      const float* bias = p.bias ? p.bias + static_cast<long long>(tile.e) * (p.gated ? 2 : 1) * p.n : nullptr;
+      if constexpr (sizeof(T) == 4) {
+        // A thread owns a feature; a warp stores 128 bytes of a row at a time.
+        float b[P];
+        int f[P];
 #pragma unroll
-        for (int q = 0; q < P; ++q) load_16_columns(taddr + q * p.bn + c, v[q]);
-        if (P == 2 && p.gated) {
-          if (f[0] < p.n) {
+        for (int q = 0; q < P; ++q) {
+          f[q] = f0 + (gated ? 0 : q * 128) + quarter * 32 + lane;
+          b[q] = bias && f[q] < p.n ? __ldg(bias + (gated && q ? p.n : 0) + f[q]) : 0.0f;
+        }
+        const bool ok = epilogue_all(mbar_wait(smem_u32(&h->acc_full[buf]), buf_ph, abort_flag, p.status, 104));
+        if (!ok) break;
+        fence_after();
+        for (int c = half * 16; c < tile.rows; c += 32) {
+          uint32_t v[P][16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float g = fmaf(v[0][i], alpha, bias[0]), u = fmaf(v[P - 1][i], alpha, bias[P - 1]);
-              if (c + i < tile.rows) y[(row0 + c + i) * p.y_stride + f[0]] = to_out<T>(__fdividef(g, 1.0f + __expf(-g)) * u);
+          for (int q = 0; q < P; ++q) load_lane_columns(taddr + q * p.bn + c, v[q]);
+#pragma unroll
+          for (int q = 0; q < P; ++q) loads_done(v[q]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float* to = reinterpret_cast<float*>(y) + (row0 + c + i) * p.y_stride;
+            if (c + i >= tile.rows) break;
+            if (gated) {
+              if (f[0] < p.n) to[f[0]] = gate(fmaf(__uint_as_float(v[0][i]), alpha, b[0]), fmaf(__uint_as_float(v[P - 1][i]), alpha, b[P - 1]));
+            } else {
+#pragma unroll
+              for (int q = 0; q < P; ++q)
+                if (f[q] < p.n) to[f[q]] = fmaf(__uint_as_float(v[q][i]), alpha, b[q]);
             }
           }
-        } else {
-#pragma unroll
-          for (int q = 0; q < P; ++q)
-            if (f[q] < p.n) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (c + i < tile.rows) y[(row0 + c + i) * p.y_stride + f[q]] = to_out<T>(fmaf(v[q][i], alpha, bias[q]));
-            }
+          __syncwarp();
         }
+        fence_before();
         __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&h->acc_empty[buf]));
+      } else {
+        // Slabs of 32 rows: each warp turns its 32 features (of one accumulator, or of both of a gated product or half of the rows)
+        // into 16-bit numbers, transposes them into the slab buffer [row][feature] (16-byte pieces exchanged by the row's number, so
+        // that neither side meets bank conflicts), and after a barrier all warps store whole rows.  Two buffers in turn.
+        float b[4], b2[4];         // of features 8 i + lane / 4 of the warp's 32; b2: of the up half
+        const bool split = P == 1 || gated;                 // the two halves of the warps share rows, not accumulators
+        const int fw = f0 + (split ? 0 : half * 128) + quarter * 32;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int f = fw + 8 * i + (lane >> 2);
+          b[i] = bias && f < p.n ? __ldg(bias + f) : 0.0f;
+          b2[i] = gated && bias && f < p.n ? __ldg(bias + p.n + f) : 0.0f;
+        }
+        const int pieces = split ? 16 : 32;                 // 16-byte pieces of a row
+        const uint32_t pitch = pieces * 16;
+        const uint32_t my_piece = (split ? 0 : half * 16) + quarter * 4 + (lane >> 3);
+        const bool ok = epilogue_all(mbar_wait(smem_u32(&h->acc_full[buf]), buf_ph, abort_flag, p.status, 104));
+        if (!ok) break;
+        fence_after();
+        for (int c0 = 0; c0 < tile.rows; c0 += 32, ++slab) {
+          const uint32_t out = staging + (slab & 1) * p.slab_bytes;
+          const uint32_t at = out + (lane & 7) * pitch + ((my_piece ^ (lane & 7)) << 4);
+          if (!split) {
+            uint32_t v[2][16];
+            load_16_lanes(taddr + half * p.bn + c0, v[0]);
+            load_16_lanes(taddr + half * p.bn + c0 + (16u << 16), v[1]);
+            loads_done(v[0]);
+            loads_done(v[1]);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              uint32_t m[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                m[i] = pack2<T>(fmaf(__uint_as_float(v[i >> 1][4 * g + 2 * (i & 1)]), alpha, b[i]),
+                                fmaf(__uint_as_float(v[i >> 1][4 * g + 2 * (i & 1) + 1]), alpha, b[i]));
+              store_transposed(at + g * 8 * pitch, m[0], m[1], m[2], m[3]);
+            }
+          } else {
+            const int c = half * 16;
+            uint32_t v[2][8], u[2][8];
+            load_16_lanes(taddr + c0 + c, v[0]);
+            load_16_lanes(taddr + c0 + c + (16u << 16), v[1]);
+            if (gated) {
+              load_16_lanes(taddr + p.bn + c0 + c, u[0]);
+              load_16_lanes(taddr + p.bn + c0 + c + (16u << 16), u[1]);
+              loads_done(u[0]);
+              loads_done(u[1]);
+            }
+            loads_done(v[0]);
+            loads_done(v[1]);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              uint32_t m[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int r = 4 * g + 2 * (i & 1);
+                float v0 = fmaf(__uint_as_float(v[i >> 1][r]), alpha, b[i]), v1 = fmaf(__uint_as_float(v[i >> 1][r + 1]), alpha, b[i]);
+                if (gated) {
+                  v0 = gate(v0, fmaf(__uint_as_float(u[i >> 1][r]), alpha, b2[i]));
+                  v1 = gate(v1, fmaf(__uint_as_float(u[i >> 1][r + 1]), alpha, b2[i]));
+                }
+                m[i] = pack2<T>(v0, v1);
+              }
+              store_transposed(at + (c + g * 8) * pitch, m[0], m[1], m[2], m[3]);
+            }
+          }
+          if (c0 + 32 >= tile.rows) {
+            // everything of this accumulator has been read
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(smem_u32(&h->acc_empty[buf]));
+          }
+          epilogue_barrier();
+          const int rows = min(32, tile.rows - c0);
+          for (int i = threadIdx.x - kFirstEpilogueWarp * 32; i < rows * pieces; i += kEpilogueWarps * 32) {
+            const int r = split ? i >> 4 : i >> 5, q = i & (pieces - 1);
+            const int f = f0 + q * 8;
+            if (f >= p.n) continue;
+            uint32_t w0, w1, w2, w3;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3) : "r"(out + r * pitch + ((q ^ (r & 7)) << 4)));
+            T* to = y + (row0 + c0 + r) * p.y_stride + f;
+            if (p.y_vec && f + 8 <= p.n) {
+              *reinterpret_cast<uint4*>(to) = make_uint4(w0, w1, w2, w3);
+            } else {
+              const uint32_t w[4] = {w0, w1, w2, w3};
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                if (f + k < p.n) reinterpret_cast<uint16_t*>(to)[k] = static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1)));
+            }
+          }
+        }
       }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&h->acc_empty[buf]));
     }
   }
 
@@ -464,7 +596,10 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   p.sf_base = p.acc_bufs * p.acc_cols;
   p.stage_bytes = (P * 128 + p.bn) * kStageBytes + (P + p.sfb_atoms) * nw * kScaleTile;
   p.stage_bytes = (p.stage_bytes + 1023u) & ~1023u;
-  const int header = static_cast<int>(sizeof(Header)) + 8 * (a.experts + 1) + 1024;   // and the ring's alignment
+  const int elem = a.y_dtype == B2VX_DT_FLOAT32 ? 4 : 2;
+  p.y_vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride * elem % 16 == 0;
+  p.slab_bytes = elem == 4 ? 0 : 32 * 256 * (P == 2 && !a.gated ? 2 : 1);
+  const int header = 2 * p.slab_bytes + static_cast<int>(sizeof(Header)) + 8 * (a.experts + 1) + 1024;   // and the ring's alignment
   p.stages = std::min(kMaxStages, static_cast<int>((kSmemBudget - header) / p.stage_bytes));
   const size_t smem = std::max<size_t>(kMinDynSmem, p.stages * p.stage_bytes + header);
   if (fp4) {
