@@ -366,9 +366,10 @@ typedef struct b2vx_fp4_dequantize_desc {
 } b2vx_fp4_dequantize_desc;
 b2vx_status b2vx_fp4_dequantize_noalloc(const b2vx_fp4_dequantize_desc* d, const void* codes, const void* scales,
                                         const float* tensor_scale, void* y, void* cuda_stream, char* err, size_t err_len);
-/* Scales [matrices][rows][ceil(k / block)] to the packed layout, matrix after matrix. */
-b2vx_status b2vx_fp4_packed_scales_size_noalloc(int32_t format, uint64_t matrices, uint64_t rows, uint64_t k, size_t* bytes);
-b2vx_status b2vx_fp4_pack_scales_noalloc(int32_t format, uint64_t matrices, uint64_t rows, uint64_t k, const void* scales,
+/* Scales [matrices][n][ceil(k / block)] (gated: [matrices][2 n][..], gate rows first) to the packed layout of a product's
+ * weights, matrix after matrix; at most 1024 matrices. */
+b2vx_status b2vx_fp4_packed_scales_size_noalloc(int32_t format, uint64_t matrices, uint64_t n, int32_t gated, uint64_t k, size_t* bytes);
+b2vx_status b2vx_fp4_pack_scales_noalloc(int32_t format, uint64_t matrices, uint64_t n, int32_t gated, uint64_t k, const void* scales,
                                          void* packed, void* cuda_stream, char* err, size_t err_len);
 
 /* Products with one matrix (FullyConnected on device tensors) or one per group of rows (experts):
@@ -377,9 +378,9 @@ b2vx_status b2vx_fp4_pack_scales_noalloc(int32_t format, uint64_t matrices, uint
  * experts == 0: one matrix w [n][k], offsets NULL.  Otherwise w is [experts][n][k]
  * and rows offsets[e] .. offsets[e+1]-1 (int32 [experts + 1], rising, at most rows) belong to
  * expert e; other rows of y are left as they are.  Offsets that fall or lie outside 0..rows are cut to rising values in
- * there; no access leaves the buffers.  gated doubles the rows of w and bias ([2n], gate first).
+ * there; no access leaves the buffers.  gated doubles the rows of w and bias ([2n], gate first); n is a multiple of 8 then.
  *   w_format 0: w and x are 16-bit floats of x_dtype, k a multiple of 8
- *   w_format B2VX_FP4_*: w is codes [..][k/2], k a multiple of 32; w_scales packed (gated: 2 * experts matrices of n rows);
+ *   w_format B2VX_FP4_*: w is codes [..][k/2], k a multiple of 32; w_scales packed (with the same n and gated);
  *     x (float32, float16, bfloat16) is quantized to the same format on the way in.
  *     BLOCK16: alpha = x_scale * w_scale[e], the tensors' scales; required then, NULL otherwise
  * row_index (int32 [rows] or NULL): row m of the product is row row_index[m] of x (zeros where out of range).

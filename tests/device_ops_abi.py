@@ -38,8 +38,8 @@ _err = [C.c_char_p, _sz]
 _SIGNATURES = {
     "b2vx_fp4_quantize_noalloc": [C.POINTER(QuantizeDesc), _vp, _vp, _vp, _vp, _vp, _vp] + _err,
     "b2vx_fp4_dequantize_noalloc": [C.POINTER(DequantizeDesc), _vp, _vp, _vp, _vp, _vp] + _err,
-    "b2vx_fp4_packed_scales_size_noalloc": [_i32, _u64, _u64, _u64, C.POINTER(_sz)],
-    "b2vx_fp4_pack_scales_noalloc": [_i32, _u64, _u64, _u64, _vp, _vp, _vp] + _err,
+    "b2vx_fp4_packed_scales_size_noalloc": [_i32, _u64, _u64, _i32, _u64, C.POINTER(_sz)],
+    "b2vx_fp4_pack_scales_noalloc": [_i32, _u64, _u64, _i32, _u64, _vp, _vp, _vp] + _err,
     "b2vx_linear_workspace_size_noalloc": [C.POINTER(LinearDesc), C.POINTER(_sz)] + _err,
     "b2vx_linear_noalloc": [C.POINTER(LinearDesc), C.POINTER(LinearArgs), _vp] + _err,
     "b2vx_route_workspace_size_noalloc": [C.POINTER(RouteDesc), C.POINTER(_sz)] + _err,

@@ -75,7 +75,7 @@ def test_dequantize_refuses_pointers():
 
 @pytest.mark.parametrize("change,words", [
     (dict(w_format=4), "w_format"), (dict(x_dtype=1), "float32"), (dict(y_dtype=2), "float32"), (dict(w_format=0, x_dtype=9), "16-bit"),
-    (dict(gated=2), "gated"), (dict(experts=1025), "1024"), (dict(n=1 << 30), "range"), (dict(k=0, x_stride=0), "zero"), (dict(k=100, x_stride=100), "multiple"),
+    (dict(gated=2), "gated"), (dict(gated=1, n=60), "gated"), (dict(experts=1025), "1024"), (dict(n=1 << 30), "range"), (dict(k=0, x_stride=0), "zero"), (dict(k=100, x_stride=100), "multiple"),
     (dict(w_format=0, k=100, x_stride=100), "multiple"), (dict(x_stride=95), "x_stride"), (dict(y_stride=63), "y_stride"),
     (dict(rows=1 << 28, x_rows=1 << 28, n=1 << 20, y_stride=1 << 20), "tiles")])
 def test_linear_refuses(change, words):
@@ -144,9 +144,9 @@ def test_empty_calls_launch_nothing():
     assert lib.b2vx_combine_noalloc(C.byref(desc(ABI.CombineDesc, COMBINE, tokens=0)), None, None, None, None, None, None, None, 0) == 0
 
 
-def packed_size(fmt, matrices, rows, k):
+def packed_size(fmt, matrices, n, k, gated=0):
     size = C.c_size_t()
-    assert ABI.library().b2vx_fp4_packed_scales_size_noalloc(fmt, matrices, rows, k, C.byref(size)) == 0
+    assert ABI.library().b2vx_fp4_packed_scales_size_noalloc(fmt, matrices, n, gated, k, C.byref(size)) == 0
     return size.value
 
 
@@ -156,7 +156,8 @@ def test_sizes():
     assert packed_size(2, 1, 128, 256) == 4 * 512
     assert packed_size(1, 3, 129, 257) == 3 * 2 * 4 * 512
     assert packed_size(1, 0, 5, 64) == 0
-    assert ABI.library().b2vx_fp4_packed_scales_size_noalloc(0, 1, 1, 1, C.byref(C.c_size_t())) == 1
+    assert ABI.library().b2vx_fp4_packed_scales_size_noalloc(0, 1, 1, 0, 1, C.byref(C.c_size_t())) == 1
+    assert packed_size(1, 2, 72, 64, 1) == 2 * 2 * 2 * 512     # gated: 64 features to a tile
     size = C.c_size_t()
     lib = ABI.library()
     # codes of 8 rows, 48 bytes each, and scales of one tile for the rows and one for the group's own start

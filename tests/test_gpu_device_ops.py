@@ -219,26 +219,26 @@ def test_packed_layout(fmt, rows, k):
     q = D.quantize_fp4(x, fmt, scale=s)
     size = C.c_size_t()
     lib, f, b = ABI.library(), D.FORMATS[fmt], D.BLOCK[fmt]
-    assert lib.b2vx_fp4_packed_scales_size_noalloc(f, 1, rows, k, C.byref(size)) == 0
+    assert lib.b2vx_fp4_packed_scales_size_noalloc(f, 1, rows, 0, k, C.byref(size)) == 0
     direct = torch.full((size.value,), 0xAB, dtype=torch.uint8, device="cuda")
     later = torch.full((size.value,), 0xCD, dtype=torch.uint8, device="cuda")
     codes = torch.empty_like(q.codes)
     d = ABI.QuantizeDesc(f, 1, 16, rows, rows, k, k, codes.shape[1], 0)
     ABI.call(lib.b2vx_fp4_quantize_noalloc, C.byref(d), x.data_ptr(), None, None if s is None else s.data_ptr(), codes.data_ptr(), direct.data_ptr(), None)
-    ABI.call(lib.b2vx_fp4_pack_scales_noalloc, f, 1, rows, k, q.scales.data_ptr(), later.data_ptr(), None)
+    ABI.call(lib.b2vx_fp4_pack_scales_noalloc, f, 1, rows, 0, k, q.scales.data_ptr(), later.data_ptr(), None)
     torch.cuda.synchronize()
     assert torch.equal(codes, q.codes)
-    words = (k + 255) // 256 * (256 // (4 * b))
-    want = np.zeros(((rows + 127) // 128, words, 32, 4, 4), np.uint8)
+    per = 256 // (4 * b)                                     # words (four blocks) of a stage of 256 columns
+    want = np.zeros(((k + 255) // 256, (rows + 127) // 128, per, 32, 4, 4), np.uint8)
     byte = q.scales.cpu().numpy()
     for r in range(rows):
         for j in range(byte.shape[1]):
-            want[r // 128, j // 4, r % 32, r % 128 // 32, j % 4] = byte[r, j]
+            want[j // 4 // per, r // 128, j // 4 % per, r % 32, r % 128 // 32, j % 4] = byte[r, j]
     assert np.array_equal(later.cpu().numpy(), want.reshape(-1))
     got = direct.cpu().numpy().reshape(want.shape)
-    there = np.zeros((want.shape[0], 1, 32, 4, 1), bool)     # rows that do not exist are left alone
+    there = np.zeros((1, want.shape[1], 1, 32, 4, 1), bool)     # rows that do not exist are left alone
     for r in range(rows):
-        there[r // 128, 0, r % 32, r % 128 // 32, 0] = True
+        there[0, r // 128, 0, r % 32, r % 128 // 32, 0] = True
     assert np.array_equal(got[np.broadcast_to(there, got.shape)], want[np.broadcast_to(there, got.shape)])
     assert (got[~np.broadcast_to(there, got.shape)] == 0xAB).all()
 

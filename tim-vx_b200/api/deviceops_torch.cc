@@ -158,18 +158,19 @@ PyObject* dequantize(PyObject* const* a) {
   return THPVariable_Wrap(std::move(y));
 }
 
-// (scales [matrices][rows][blocks], format) -> packed scales
+// (scales [matrices][rows][blocks], format, gated) -> packed scales
 PyObject* pack(PyObject* const* a) {
   const at::Tensor& scales = tensor(a[0], "scales");
   const long format = number(a[1]);
   const int64_t block = block_of(format);
   need(scales.dim() == 3 && scales.scalar_type() == at::kByte && scales.is_contiguous(), "scales must be a dense uint8 tensor");
   Call call(scales.device());
-  const uint64_t matrices = scales.size(0), rows = scales.size(1), k = scales.size(2) * block;
+  const int32_t gated = number(a[2]) != 0;
+  const uint64_t matrices = scales.size(0), n = gated ? scales.size(1) / 2 : scales.size(1), k = scales.size(2) * block;
   size_t bytes = 0;
-  call(b2vx_fp4_packed_scales_size_noalloc(static_cast<int32_t>(format), matrices, rows, k, &bytes));
+  call(b2vx_fp4_packed_scales_size_noalloc(static_cast<int32_t>(format), matrices, n, gated, k, &bytes));
   at::Tensor packed = empty({static_cast<int64_t>(bytes)}, at::kByte, scales.device());
-  call(b2vx_fp4_pack_scales_noalloc(static_cast<int32_t>(format), matrices, rows, k, scales.data_ptr(), packed.data_ptr(), call.stream, call.err, sizeof(call.err)));
+  call(b2vx_fp4_pack_scales_noalloc(static_cast<int32_t>(format), matrices, n, gated, k, scales.data_ptr(), packed.data_ptr(), call.stream, call.err, sizeof(call.err)));
   return THPVariable_Wrap(std::move(packed));
 }
 
@@ -197,7 +198,7 @@ PyObject* product(PyObject* const* a) {
   p.x_scale = static_cast<const float*>(tensor_scale(a[9], format, 1, device, "x_scale"));
   need((a[6] != Py_None) == (experts > 0), "offsets belong to weights of experts and only to them");
   if (x.size(1) != k) wrong("x has " + std::to_string(x.size(1)) + " columns, the weight " + std::to_string(k));
-  need(!gated || w_rows % 2 == 0, "a gated weight has an even number of rows");
+  need(!gated || w_rows % 16 == 0, "the rows of a gated weight must be a multiple of 16");
   const int64_t rows = index_rows(a[7], x), n = gated ? w_rows / 2 : w_rows;
   p.offsets = static_cast<const int32_t*>(dense(a[6], "offsets", at::kInt, {experts + 1}, device));
   p.row_index = static_cast<const int32_t*>(dense(a[7], "row_index", at::kInt, {rows}, device));
@@ -318,7 +319,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
 }
 
 #define B2VX_ENTRY(fn, args) {#fn, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<fn, args>)), METH_FASTCALL, nullptr}
-PyMethodDef kMethods[] = {B2VX_ENTRY(quantize, 4), B2VX_ENTRY(dequantize, 7), B2VX_ENTRY(pack, 2), B2VX_ENTRY(product, 12),
+PyMethodDef kMethods[] = {B2VX_ENTRY(quantize, 4), B2VX_ENTRY(dequantize, 7), B2VX_ENTRY(pack, 3), B2VX_ENTRY(product, 12),
                           B2VX_ENTRY(route, 3),    B2VX_ENTRY(combine, 5),    B2VX_ENTRY(check, 1), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "deviceops_native", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,18 +1,26 @@
 // Products y = x W^T on Blackwell tensor cores for operands in 4-bit block floating point or in 16 bits, for one matrix or for
 // groups of rows that each have their own (experts).
 //
-//   y[m][f] = act( alpha_e * sum_k x[m][k] * W_e[f][k] + bias_e[f] ),   rows m in [offsets[e], offsets[e + 1])
+//   y[m][f] = alpha_e * sum_k x[m][k] * W_e[f][k] + bias_e[f],   rows m in [offsets[e], offsets[e + 1])
+//   gated:    silu(that with gate row f of W_e) * (that with up row f)
 //
-// Features are the instruction's M (128 rows of W per tile) and rows of x its N: a few rows then cost a narrow N instead of
-// an M tile of padding, the same kernel serves one row (where W streams from memory once) and many, and gate and up halves of a
-// gated product meet in one thread of the epilogue, in two accumulators.
+// Features are the instruction's M and rows of x its N: a few rows then cost a narrow N instead of an M tile of padding, and the same
+// kernel serves one row (where W streams from memory once) and many.  A tile is 128 rows of W for each CTA.  The rows of a
+// gated W come in alternating groups of eight gate and eight up rows (one five-dimensional TMA box fetches them so), so that a
+// thread of the epilogue finds the gate and the up sum of a feature in its own registers.
 //
-// One persistent CTA per SM, warp-specialised:
-//   warp 0      producer   per stage of 128 bytes of K: TMA boxes of W (P tiles of 128 rows) and of x (32 rows each), bulk copies of
-//                          the packed scales
-//   warp 1      issuer     copies a stage's scales into tensor memory (tcgen05.cp, two slots in turn) and issues the stage's
-//                          four K steps of 32 bytes for each of the P accumulators
-//   warps 4-11  epilogue   out of tensor memory, scale and bias, activation, rounding, stores
+// Persistent CTAs, one per SM, warp-specialised:
+//   warps 0, 2  producers  of W and of x: per stage of 128 bytes of K one TMA box each (small ones of few rows) and the packed scales.
+//                          Two warps and few, large copies because a wait, an announcement and a copy take one thread about 340 cycles.
+//   warp 1      issuer     copies a stage's scales into tensor memory (tcgen05.cp, two slots in turn) and issues the stage's four K steps
+//   warps 4-11  epilogue   two sets of four warps take slabs of 32 rows of the tile in turn: out of tensor memory, scale and bias,
+//                          activation, rounding, transposition into a buffer in shared memory, one TMA store
+//
+// CG = 2 (many rows): two CTAs of a cluster share a tile of 256 rows of W; each holds its 128 rows of W and half of the rows of x, and
+// the first one's issuer issues for both.  An instruction then is twice the work for the same issue, and rows of x are fetched
+// once for 256 features.  No load is multicast: every CTA fetches its own operands; the loads of both announce themselves on
+// the first one's barrier.
+//
 // Every wait is bounded as in gemm_tc.cu: on a time-out the CTA records a code and leaves through its common exit.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -33,7 +41,11 @@ constexpr int kFirstEpilogueWarp = 4;
 constexpr int kEpilogueWarps = 8;
 constexpr int kMaxStages = 10;
 constexpr int kBoxRows = 32;
-constexpr int kSmemBudget = 224 * 1024;
+constexpr int kSlabRows = 32;
+constexpr int kSlabBytes = kSlabRows * 256;                // 128 features of 16 bits, two boxes of 64
+constexpr int kStagingBytes = 4 * kSlabBytes;              // two for each set
+constexpr uint32_t kWTile = 128 * kStageBytes;
+constexpr int kSmemBudget = 226 * 1024;
 constexpr int kMaxDynSmem = 227 * 1024;
 constexpr int kMaxDevices = 64;
 constexpr int kMinDynSmem = 120 * 1024;   // keeps two CTAs from sharing an SM and its tensor memory
@@ -42,16 +54,15 @@ struct LinearParams {
   int n, rows, experts, gated;
   int bn;                     // most rows of x in a tile, a multiple of 64
   int feature_tiles;          // tiles along the features of one group
-  int scale_tiles;            // packed scale tiles along the rows of one matrix of W
+  int scale_tiles;            // 128-row tiles of one matrix of W (and of its packed scales)
   int k_stages, stages, acc_bufs;
+  int x_box;                  // rows of x in the large box, bn / CG
   int sfb_atoms;              // most scale tiles of x under one tile's rows
-  int words;                  // scale words (tiles along K) of a row tile
-  uint32_t stage_bytes, slab_bytes;
+  int x_scale_tiles;          // packed scale tiles along the rows of x
+  int after_operand;
+  uint32_t stage_bytes;
   uint32_t idesc;             // without N
-  uint32_t acc_cols;          // TMEM columns of one accumulator buffer
   uint32_t sf_cols, sf_base;  // TMEM columns of a scale slot, first column of the slots
-  const uint8_t* w_scales;
-  const uint8_t* x_scales;
   const float* x_scale;
   const float* w_scale;
   const float* bias;
@@ -59,8 +70,12 @@ struct LinearParams {
   void* y;
   long long y_stride;
   int y_dtype;
-  int y_vec;                  // rows of y start on 16 bytes
+  int y_vec;                  // rows of y start on 16 bytes: whole slabs leave by TMA
   int* status;
+};
+
+struct Maps {
+  CUtensorMap w, x, x32, w_scales, x_scales, y;
 };
 
 struct Header {
@@ -72,16 +87,87 @@ struct Header {
 };
 // Behind the header: the groups' first rows lo[experts + 1] (group e ends where e + 1 begins) and first tiles start[experts + 1].
 
+// ---- PTX wrappers (the rest: tma.cuh) ----------------------------------------
+
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
 }
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar)
-      : "memory");
+// The address of the first CTA's copy of a shared variable.
+__device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// A wait for arrivals that may come from the other CTA.
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+  const long long began = clock64();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(bar), "r"(parity), "r"(100u) : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    if (clock64() - began > kWaitLimitCycles) {
+      *abort_flag = 1;
+      atomicCAS(status, 0, code);
+      return false;
+    }
+  }
+}
+// Arrives on the barrier (CG = 2: of both CTAs) when the instructions issued so far are done.
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+}
+// TMA loads into this CTA's memory; CG = 2: bar may be the first CTA's.
+template <int CG>
+__device__ __forceinline__ void load_2d(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  if constexpr (CG == 1) {
+    tma_load_2d(dst, map, c0, c1, bar);
+  } else {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar) : "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void load_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+  if constexpr (CG == 1) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+  } else {
+    asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+  }
+}
+template <int CG>
+__device__ __forceinline__ void load_5d(uint32_t dst, const CUtensorMap* map, int c0, int c3, int c4, uint32_t bar) {
+  if constexpr (CG == 1) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %6, %6, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c3), "r"(c4), "r"(bar), "r"(0) : "memory");
+  } else {
+    asm volatile("cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %6, %6, %3, %4}], [%5];"
+                 ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c3), "r"(c4), "r"(bar), "r"(0) : "memory");
+  }
+}
+__device__ __forceinline__ void store_2d(const CUtensorMap* map, int c0, int c1, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(src) : "memory");
 }
 // K-major operand rows of one 128-byte swizzle span: groups of eight rows 1024 bytes apart.
 __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
@@ -91,28 +177,25 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
 __device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
   return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (1ull << 16) | (8ull << 32) | (1ull << 46);
 }
+template <int CG>
 __device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  if constexpr (CG == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
-template <int KIND>
+#define B2VX_MMA(group, kind, scales)                                                                 \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                     \
+               "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3" scales ", p;\n\t}"   \
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory")
+template <int KIND, int CG>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
-  if constexpr (KIND == 0) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-  } else if constexpr (KIND == B2VX_FP4_BLOCK32) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-  } else {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
-  }
+  if constexpr (KIND == 0 && CG == 1) B2VX_MMA("1", "f16", "");
+  else if constexpr (KIND == 0) B2VX_MMA("2", "f16", "");
+  else if constexpr (KIND == B2VX_FP4_BLOCK32 && CG == 1) B2VX_MMA("1", "mxf4.block_scale.scale_vec::2X", ", [%4], [%5]");
+  else if constexpr (KIND == B2VX_FP4_BLOCK32) B2VX_MMA("2", "mxf4.block_scale.scale_vec::2X", ", [%4], [%5]");
+  else if constexpr (CG == 1) B2VX_MMA("1", "mxf4nvf4.block_scale.scale_vec::4X", ", [%4], [%5]");
+  else B2VX_MMA("2", "mxf4nvf4.block_scale.scale_vec::4X", ", [%4], [%5]");
 }
+#undef B2VX_MMA
 // Lane t of the warp gets 16 columns of TMEM lane t.
 __device__ __forceinline__ void load_lane_columns(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -122,7 +205,7 @@ __device__ __forceinline__ void load_lane_columns(uint32_t taddr, uint32_t (&r)[
       : "r"(taddr)
       : "memory");
 }
-// 16 lanes x 8 N columns, N = 2 or 4: of column group h, thread t gets columns 2 (t % 4), + 1 of lane t / 4 in r[4 h], r[4 h + 1] and of lane
+// 16 lanes x 32 columns: of column group h (eight columns), thread t gets columns 2 (t % 4), + 1 of lane t / 4 in r[4 h], r[4 h + 1] and of lane
 // t / 4 + 8 in r[4 h + 2], r[4 h + 3].
 __device__ __forceinline__ void load_16_lanes(uint32_t taddr, uint32_t (&r)[16]) {
   asm volatile(
@@ -132,12 +215,6 @@ __device__ __forceinline__ void load_16_lanes(uint32_t taddr, uint32_t (&r)[16])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void load_16_lanes(uint32_t taddr, uint32_t (&r)[8]) {
-  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-               : "r"(taddr)
-               : "memory");
-}
 // The registers of a load are valid after the wait; naming them there keeps their uses behind it.
 __device__ __forceinline__ void loads_done(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -146,29 +223,24 @@ __device__ __forceinline__ void loads_done(uint32_t (&r)[16]) {
                :
                : "memory");
 }
-__device__ __forceinline__ void loads_done(uint32_t (&r)[8]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7])
-               :
-               : "memory");
-}
 // Four 8 x 8 matrices of 16-bit numbers to shared memory, transposed: lane i gives the address of row i % 8 of matrix i / 8.
 __device__ __forceinline__ void store_transposed(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// A barrier of the epilogue warps that also tells every one of them whether all came with ok.
-__device__ __forceinline__ bool epilogue_all(bool ok) {
+// Barriers of a set of epilogue warps; the second also tells every one whether all came with ok.
+__device__ __forceinline__ void set_barrier(int set) { asm volatile("bar.sync %0, 128;" ::"r"(1 + set) : "memory"); }
+__device__ __forceinline__ bool set_all(int set, bool ok) {
   uint32_t r;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-               : "=r"(r) : "r"(static_cast<uint32_t>(ok)), "n"(kEpilogueWarps * 32) : "memory");
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"(static_cast<uint32_t>(ok)), "r"(1 + set) : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void epilogue_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueWarps * 32) : "memory"); }
 
-// One tile of the schedule: group, first row inside it, rows (as the instruction's N and as they are), feature tile.
+// One tile of the schedule: group, its first row, first row inside it, rows (as they are and as the instruction's N), feature tile.
 struct Tile {
-  int e, r0, rows, n_mma, f, lo;
+  int e, lo, r0, rows, n_mma, f;
 };
+template <int CG>
 __device__ __forceinline__ Tile tile_of(const int* lo, const int* start, const LinearParams& p, int t) {
   int a = 0, b = p.experts;           // the last group whose first tile is not behind t
   while (b - a > 1) {
@@ -178,12 +250,13 @@ __device__ __forceinline__ Tile tile_of(const int* lo, const int* start, const L
   const int count = lo[a + 1] - lo[a], row_tiles = (count + p.bn - 1) / p.bn;
   const int i = t - start[a];
   const int per = ((count + row_tiles - 1) / row_tiles + 63) & ~63;   // even shares, whole halves of a scale tile
+  constexpr int step = 16 * CG;
   Tile r;
   r.e = a;
   r.f = i / row_tiles;
-  r.r0 = (i % row_tiles) * per;
+  r.r0 = (i - r.f * row_tiles) * per;
   r.rows = max(0, min(per, count - r.r0));
-  r.n_mma = max(16, (r.rows + 15) & ~15);
+  r.n_mma = max(step, (r.rows + step - 1) / step * step);
   r.lo = lo[a];
   return r;
 }
@@ -200,46 +273,55 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 __device__ __forceinline__ float gate(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
-template <int KIND, int P, typename T>
-__global__ void __launch_bounds__(kThreads, 1)
-block_linear_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const LinearParams p) {
+template <int KIND, int CG, typename T>
+__global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_constant__ Maps maps, const LinearParams p) {
   constexpr int NW = KIND == 0 ? 0 : (KIND == B2VX_FP4_BLOCK32 ? 2 : 4);   // scale words per stage
-  constexpr uint32_t kATile = 128 * kStageBytes;
   extern __shared__ uint8_t smem_raw[];
   pdl_trigger();
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t ring = (raw + 1023u) & ~1023u;
-  const uint32_t staging = ring + p.stages * p.stage_bytes;       // two slabs of the epilogue
-  Header* h = reinterpret_cast<Header*>(smem_raw + (staging - raw) + 2 * p.slab_bytes);
+  const uint32_t staging = ring + p.stages * p.stage_bytes;
+  Header* h = reinterpret_cast<Header*>(smem_raw + (staging - raw) + kStagingBytes);
   int* lo = reinterpret_cast<int*>(h + 1);
   int* start = lo + p.experts + 1;
   volatile int* abort_flag = &h->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // a stage: [P tiles of W | rows of x | scales of W | scales of x]
-  const uint32_t x_off = P * kATile, sfa_off = x_off + static_cast<uint32_t>(p.bn) * kStageBytes;
-  const uint32_t sfb_off = sfa_off + P * NW * kScaleTile;
+  const uint32_t rank = CG == 1 ? 0u : cluster_rank();
+  const int first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
+  // a stage: [128 rows of W | rows of x | scales of W | scales of x]
+  const uint32_t x_off = kWTile, sfa_off = x_off + static_cast<uint32_t>(p.x_box) * kStageBytes, sfb_off = sfa_off + NW * kScaleTile;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
-      mbar_init(smem_u32(&h->full[i]), 1);
+      mbar_init(smem_u32(&h->full[i]), 2);
       mbar_init(smem_u32(&h->empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&h->acc_full[i]), 1);
-      mbar_init(smem_u32(&h->acc_empty[i]), kEpilogueWarps);
+      mbar_init(smem_u32(&h->acc_empty[i]), CG * kEpilogueWarps);
     }
     h->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&h->tmem_base)), "r"(512u) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&h->tmem_base)), "r"(512u) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&h->tmem_base)), "r"(512u) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
   }
   if (threadIdx.x == 64) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_w)) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_x)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.w)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.x)) : "memory");
+    if (NW) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.w_scales)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.x_scales)) : "memory");
+    }
   }
-  pdl_wait();   // offsets, rows and scales are other kernels' outputs
+  // Behind the kernel that made the operand x, which began its work after everything before it had ended, only the loads of x wait.
+  if (!p.after_operand) pdl_wait();
   // The groups.  Offsets are device data that nobody has checked: they are cut to rising values among the rows that exist.
   if (warp == 0) {
     int high = 0, total = 0;
@@ -272,87 +354,108 @@ block_linear_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
     if (lane == 0) h->num_tiles = total;
   }
   fence_before();
-  __syncthreads();
+  if constexpr (CG == 1) __syncthreads();
+  else cluster_barrier();       // the other CTA's barriers are ready, too
   fence_after();
   const uint32_t tmem = h->tmem_base;
   const int num_tiles = h->num_tiles;
 
   if (warp == 0) {
-    // ------------------------------------------------------------ producer
+    // ------------------------------------------------------------ producer of W
     uint32_t s = 0, ph = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < num_tiles; t += gridDim.x) {
-      const Tile tile = tile_of(lo, start, p, t);
-      const int boxes = (tile.n_mma + kBoxRows - 1) / kBoxRows;
-      const int atoms = NW ? ((tile.r0 & 127) + tile.n_mma + 127) >> 7 : 0;
-      const uint32_t tx = P * kATile + boxes * kBoxRows * kStageBytes + (P + atoms) * NW * kScaleTile;
-      // scale tiles of W: rows that do not exist use the last tile that does (their outputs are not stored)
-      const uint8_t* sfa[P];
-#pragma unroll
-      for (int q = 0; q < P; ++q) {
-        const long long mat = p.gated ? 2ll * tile.e + q : tile.e;
-        const int st = min(p.gated ? tile.f : tile.f * P + q, p.scale_tiles - 1);
-        sfa[q] = p.w_scales + (mat * p.scale_tiles + st) * p.words * kScaleTile;
-      }
-      const uint8_t* sfb = p.x_scales + (expert_scale_row(tile.lo, tile.e) + tile.r0) / 128 * p.words * kScaleTile;
+    for (int t = first_tile; ok && t < num_tiles; t += tile_step) {
+      const Tile tile = tile_of<CG>(lo, start, p, t);
+      const int ft = tile.f * CG + static_cast<int>(rank);
+      // scales: of a tile whose rows do not exist those of the last that do (its outputs are not stored)
+      int sf = (tile.e * p.k_stages * p.scale_tiles + min(ft, p.scale_tiles - 1)) * NW;
       for (int ks = 0; ks < p.k_stages; ++ks) {
         ok = mbar_wait(smem_u32(&h->empty[s]), ph ^ 1, abort_flag, p.status, 101);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         if (elect_one()) {
-          const uint32_t full = smem_u32(&h->full[s]);
           const uint32_t dst = ring + s * p.stage_bytes;
-          mbar_arrive_expect_tx(full, tx);
-#pragma unroll
-          for (int q = 0; q < P; ++q) {
-            if (p.gated) tma_load_3d(dst + q * kATile, &map_w, ks * kStageBytes, tile.f * 128, 2 * tile.e + q, full);
-            else tma_load_3d(dst + q * kATile, &map_w, ks * kStageBytes, (tile.f * P + q) * 128, tile.e, full);
-          }
-          for (int b = 0; b < boxes; ++b)
-            tma_load_2d(dst + x_off + b * kBoxRows * kStageBytes, &map_x, ks * kStageBytes, tile.lo + tile.r0 + b * kBoxRows, full);
-          if constexpr (NW > 0) {
-#pragma unroll
-            for (int q = 0; q < P; ++q) bulk_load(dst + sfa_off + q * NW * kScaleTile, sfa[q] + ks * NW * kScaleTile, NW * kScaleTile, full);
-            for (int a = 0; a < atoms; ++a)
-              bulk_load(dst + sfb_off + a * NW * kScaleTile, sfb + (static_cast<long long>(a) * p.words + ks * NW) * kScaleTile, NW * kScaleTile, full);
-          }
+          uint32_t full = smem_u32(&h->full[s]);
+          if (CG == 2) full = in_first_cta(full);
+          if (rank == 0) mbar_arrive_expect_tx(smem_u32(&h->full[s]), CG * (kWTile + NW * kScaleTile));
+          if (p.gated) load_5d<CG>(dst, &maps.w, ks * kStageBytes, ft * 8, tile.e, full);
+          else load_3d<CG>(dst, &maps.w, ks * kStageBytes, ft * 128, tile.e, full);
+          if constexpr (NW > 0) load_2d<CG>(dst + sfa_off, &maps.w_scales, 0, sf, full);
         }
         __syncwarp();
+        sf += p.scale_tiles * NW;
         if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ producer of x
+    pdl_wait();
+    uint32_t s = 0, ph = 0;
+    bool ok = true;
+    for (int t = first_tile; ok && t < num_tiles; t += tile_step) {
+      const Tile tile = tile_of<CG>(lo, start, p, t);
+      const int need = tile.n_mma / CG, row = tile.lo + tile.r0 + static_cast<int>(rank) * need;
+      // one large box where most of it is needed, else boxes of 32 rows
+      const bool large = 2 * need > p.x_box;
+      const int boxes = large ? 1 : (need + kBoxRows - 1) / kBoxRows;
+      const int atoms = NW ? ((tile.r0 & 127) + tile.n_mma + 127) >> 7 : 0;
+      const uint32_t tx = CG * ((large ? p.x_box : boxes * kBoxRows) * kStageBytes + atoms * NW * kScaleTile);
+      int sf = static_cast<int>((expert_scale_row(tile.lo, tile.e) + tile.r0) / 128) * NW;
+      for (int ks = 0; ks < p.k_stages; ++ks) {
+        ok = mbar_wait(smem_u32(&h->empty[s]), ph ^ 1, abort_flag, p.status, 105);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t dst = ring + s * p.stage_bytes;
+          uint32_t full = smem_u32(&h->full[s]);
+          if (CG == 2) full = in_first_cta(full);
+          if (rank == 0) mbar_arrive_expect_tx(smem_u32(&h->full[s]), tx);
+          if (large) {
+            load_2d<CG>(dst + x_off, &maps.x, ks * kStageBytes, row, full);
+          } else {
+            for (int b = 0; b < boxes; ++b) load_2d<CG>(dst + x_off + b * kBoxRows * kStageBytes, &maps.x32, ks * kStageBytes, row + b * kBoxRows, full);
+          }
+          if constexpr (NW > 0)
+            for (int a = 0; a < atoms; ++a) load_2d<CG>(dst + sfb_off + a * NW * kScaleTile, &maps.x_scales, 0, sf + a * NW, full);
+        }
+        __syncwarp();
+        sf += p.x_scale_tiles * NW;
+        if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------ issuer
     uint32_t s = 0, ph = 0, slot = 0;
     bool ok = true;
     int j = 0;
-    for (int t = blockIdx.x; ok && t < num_tiles; t += gridDim.x, ++j) {
-      const Tile tile = tile_of(lo, start, p, t);
+    for (int t = first_tile; ok && t < num_tiles; t += tile_step, ++j) {
+      const Tile tile = tile_of<CG>(lo, start, p, t);
       const uint32_t idesc = p.idesc | (static_cast<uint32_t>(tile.n_mma) >> 3) << 17;
       const int atoms = NW ? ((tile.r0 & 127) + tile.n_mma + 127) >> 7 : 0;
       const uint32_t sfb_col = (tile.r0 & 127) >> 5;
       const int buf = p.acc_bufs == 2 ? (j & 1) : 0;
       const uint32_t buf_ph = p.acc_bufs == 2 ? (j >> 1) & 1 : j & 1;
-      ok = mbar_wait(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102);
+      ok = CG == 1 ? mbar_wait(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102)
+                   : wait_cluster(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       fence_after();
-      const uint32_t d = tmem + buf * p.acc_cols;
+      const uint32_t d = tmem + buf * p.bn;
       for (int ks = 0; ks < p.k_stages; ++ks) {
-        ok = mbar_wait(smem_u32(&h->full[s]), ph, abort_flag, p.status, 103);
+        ok = CG == 1 ? mbar_wait(smem_u32(&h->full[s]), ph, abort_flag, p.status, 103) : wait_cluster(smem_u32(&h->full[s]), ph, abort_flag, p.status, 103);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         fence_after();
         if (elect_one()) {
           const uint32_t base = ring + s * p.stage_bytes;
-          const uint32_t sfa_t = tmem + p.sf_base + slot * p.sf_cols, sfb_t = sfa_t + P * NW * 4;
+          const uint32_t sfa_t = tmem + p.sf_base + slot * p.sf_cols, sfb_t = sfa_t + NW * 4;
           if constexpr (NW > 0) {
             // The slot was last read by instructions two stages ago.  Copies and products of one thread execute in the order issued.
 #pragma unroll
-            for (int q = 0; q < P * NW; ++q) copy_scales(sfa_t + q * 4, scale_desc(base + sfa_off + q * kScaleTile));
+            for (int w = 0; w < NW; ++w) copy_scales<CG>(sfa_t + w * 4, scale_desc(base + sfa_off + w * kScaleTile));
             for (int a = 0; a < atoms; ++a)
 #pragma unroll
-              for (int w = 0; w < NW; ++w) copy_scales(sfb_t + (w * p.sfb_atoms + a) * 4, scale_desc(base + sfb_off + (a * NW + w) * kScaleTile));
+              for (int w = 0; w < NW; ++w) copy_scales<CG>(sfb_t + (w * p.sfb_atoms + a) * 4, scale_desc(base + sfb_off + (a * NW + w) * kScaleTile));
           }
           const uint64_t da = operand_desc(base), db = operand_desc(base + x_off);
 #pragma unroll
@@ -360,192 +463,197 @@ block_linear_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_cons
             const int w = KIND == B2VX_FP4_BLOCK32 ? k >> 1 : k;
             // the first of the word's bytes that this K step uses
             const uint32_t id = KIND == B2VX_FP4_BLOCK32 ? (k & 1) * 2u : 0u;
-            const uint32_t desc = idesc | (id << 4) | (id << 29);
-#pragma unroll
-            for (int q = 0; q < P; ++q)
-              mma<KIND>(d + q * p.bn, da + q * (kATile >> 4) + 2 * k, db + 2 * k, desc, sfa_t + (q * NW + w) * 4,
-                        sfb_t + w * p.sfb_atoms * 4 + sfb_col, (ks | k) != 0);
+            mma<KIND, CG>(d, da + 2 * k, db + 2 * k, idesc | (id << 4) | (id << 29), sfa_t + w * 4, sfb_t + w * p.sfb_atoms * 4 + sfb_col, (ks | k) != 0);
           }
-          commit(smem_u32(&h->empty[s]));
+          commit<CG>(smem_u32(&h->empty[s]));
         }
         __syncwarp();
         slot ^= 1;
         if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
       }
-      if (ok && elect_one()) commit(smem_u32(&h->acc_full[buf]));
+      if (ok && elect_one()) commit<CG>(smem_u32(&h->acc_full[buf]));
       __syncwarp();
     }
   } else if (warp >= kFirstEpilogueWarp) {
     // ------------------------------------------------------------ epilogue
-    const int ew = warp - kFirstEpilogueWarp, quarter = ew & 3, half = ew >> 2;
+    const int ew = warp - kFirstEpilogueWarp, quarter = ew & 3, set = ew >> 2;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     T* y = static_cast<T*>(p.y);
-    const bool gated = P == 2 && p.gated;
+    const int width = p.gated ? 64 : 128;                 // features of a CTA's tile
+    const int warp_width = p.gated ? 16 : 32;             // of a warp
+    const uint32_t buffers = staging + set * 2 * kSlabBytes;
     int j = 0, slab = 0;
-    for (int t = blockIdx.x; t < num_tiles; t += gridDim.x, ++j) {
-      const Tile tile = tile_of(lo, start, p, t);
+    for (int t = first_tile; t < num_tiles; t += tile_step, ++j) {
+      const Tile tile = tile_of<CG>(lo, start, p, t);
       const int buf = p.acc_bufs == 2 ? (j & 1) : 0;
       const uint32_t buf_ph = p.acc_bufs == 2 ? (j >> 1) & 1 : j & 1;
       float alpha = 1.0f;
       if (p.x_scale) alpha = __ldg(p.x_scale);
       if (p.w_scale) alpha *= __ldg(p.w_scale + tile.e);
-      const uint32_t taddr = tmem + buf * p.acc_cols + lanes;
-      const long long row0 = static_cast<long long>(tile.lo) + tile.r0;
-      const int f0 = gated ? tile.f * 128 : tile.f * P * 128;             // first feature of the tile
+      const uint32_t taddr = tmem + buf * p.bn + lanes;
+      const int row0 = tile.lo + tile.r0;
+      const int f0 = (tile.f * CG + static_cast<int>(rank)) * width;       // first feature of the CTA's tile
+      // Bias of the TMEM lanes 8 i + lane / 4 of the warp: features, or alternating eight gate and eight up features.
       const float* bias = p.bias ? p.bias + static_cast<long long>(tile.e) * (p.gated ? 2 : 1) * p.n : nullptr;
-      if constexpr (sizeof(T) == 4) {
-        // A thread owns a feature; a warp stores 128 bytes of a row at a time.
-        float b[P];
-        int f[P];
+      float b[4];
 #pragma unroll
-        for (int q = 0; q < P; ++q) {
-          f[q] = f0 + (gated ? 0 : q * 128) + quarter * 32 + lane;
-          b[q] = bias && f[q] < p.n ? __ldg(bias + (gated && q ? p.n : 0) + f[q]) : 0.0f;
-        }
-        const bool ok = epilogue_all(mbar_wait(smem_u32(&h->acc_full[buf]), buf_ph, abort_flag, p.status, 104));
-        if (!ok) break;
-        fence_after();
-        for (int c = half * 16; c < tile.rows; c += 32) {
-          uint32_t v[P][16];
+      for (int i = 0; i < 4; ++i) {
+        const int f = f0 + quarter * warp_width + (p.gated ? 8 * (i >> 1) : 8 * i) + (lane >> 2);
+        b[i] = bias && f < p.n ? __ldg(bias + (p.gated && (i & 1) ? p.n : 0) + f) : 0.0f;
+      }
+      const bool ok = set_all(set, mbar_wait(smem_u32(&h->acc_full[buf]), buf_ph, abort_flag, p.status, 104));
+      if (!ok) break;
+      fence_after();
+      // Slabs of 32 rows, the sets in turn.
+      for (int c0 = set * kSlabRows; c0 < tile.rows; c0 += 2 * kSlabRows) {
+        uint32_t v[2][16];
+        load_16_lanes(taddr + c0, v[0]);
+        load_16_lanes(taddr + c0 + (16u << 16), v[1]);
+        loads_done(v[0]);
+        loads_done(v[1]);
+        const int rows = min(kSlabRows, tile.rows - c0);
+        // value of lane group i (eight TMEM lanes), column group g, column 2 (lane % 4) + k
+        auto value = [&](int i, int g, int k) { return fmaf(__uint_as_float(v[i >> 1][4 * g + 2 * (i & 1) + k]), alpha, b[i]); };
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-          for (int q = 0; q < P; ++q) load_lane_columns(taddr + q * p.bn + c, v[q]);
+          for (int g = 0; g < 4; ++g)
 #pragma unroll
-          for (int q = 0; q < P; ++q) loads_done(v[q]);
+            for (int k = 0; k < 2; ++k) {
+              const int r = 8 * g + 2 * (lane & 3) + k;
+              if (r >= rows) continue;
+              float* to = reinterpret_cast<float*>(y) + (row0 + c0 + r) * p.y_stride + f0 + quarter * warp_width + (lane >> 2);
+              const int f = f0 + quarter * warp_width + (lane >> 2);
+              if (p.gated) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float* to = reinterpret_cast<float*>(y) + (row0 + c + i) * p.y_stride;
-            if (c + i >= tile.rows) break;
-            if (gated) {
-              if (f[0] < p.n) to[f[0]] = gate(fmaf(__uint_as_float(v[0][i]), alpha, b[0]), fmaf(__uint_as_float(v[P - 1][i]), alpha, b[P - 1]));
-            } else {
+                for (int i = 0; i < 2; ++i)
+                  if (f + 8 * i < p.n) to[8 * i] = gate(value(2 * i, g, k), value(2 * i + 1, g, k));
+              } else {
 #pragma unroll
-              for (int q = 0; q < P; ++q)
-                if (f[q] < p.n) to[f[q]] = fmaf(__uint_as_float(v[q][i]), alpha, b[q]);
+                for (int i = 0; i < 4; ++i)
+                  if (f + 8 * i < p.n) to[8 * i] = value(i, g, k);
+              }
             }
-          }
           __syncwarp();
-        }
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&h->acc_empty[buf]));
-      } else {
-        // Slabs of 32 rows: each warp turns its 32 features (of one accumulator, or of both of a gated product or half of the rows)
-        // into 16-bit numbers, transposes them into the slab buffer [row][feature] (16-byte pieces exchanged by the row's number, so
-        // that neither side meets bank conflicts), and after a barrier all warps store whole rows.  Two buffers in turn.
-        float b[4], b2[4];         // of features 8 i + lane / 4 of the warp's 32; b2: of the up half
-        const bool split = P == 1 || gated;                 // the two halves of the warps share rows, not accumulators
-        const int fw = f0 + (split ? 0 : half * 128) + quarter * 32;
+        } else {
+          // 16-bit numbers, transposed into the slab buffer: boxes of 64 features, [row][128 bytes], 16-byte pieces exchanged by the
+          // row's number as the store's 128-byte swizzle has them (neither side then meets bank conflicts).
+          const uint32_t out = buffers + (slab & 1) * kSlabBytes;
+          ++slab;
+          const uint32_t row_at = out + (lane & 7) * 128;
+          if (p.gated) {
+            // two matrices (features 8 i) of two column groups
+            const uint32_t piece = quarter * 2 + ((lane >> 3) & 1);
+            const uint32_t at = row_at + ((piece ^ (lane & 7)) << 4) + (lane >> 4) * 1024;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int f = fw + 8 * i + (lane >> 2);
-          b[i] = bias && f < p.n ? __ldg(bias + f) : 0.0f;
-          b2[i] = gated && bias && f < p.n ? __ldg(bias + p.n + f) : 0.0f;
-        }
-        const int pieces = split ? 16 : 32;                 // 16-byte pieces of a row
-        const uint32_t pitch = pieces * 16;
-        const uint32_t my_piece = (split ? 0 : half * 16) + quarter * 4 + (lane >> 3);
-        const bool ok = epilogue_all(mbar_wait(smem_u32(&h->acc_full[buf]), buf_ph, abort_flag, p.status, 104));
-        if (!ok) break;
-        fence_after();
-        for (int c0 = 0; c0 < tile.rows; c0 += 32, ++slab) {
-          const uint32_t out = staging + (slab & 1) * p.slab_bytes;
-          const uint32_t at = out + (lane & 7) * pitch + ((my_piece ^ (lane & 7)) << 4);
-          if (!split) {
-            uint32_t v[2][16];
-            load_16_lanes(taddr + half * p.bn + c0, v[0]);
-            load_16_lanes(taddr + half * p.bn + c0 + (16u << 16), v[1]);
-            loads_done(v[0]);
-            loads_done(v[1]);
+            for (int g = 0; g < 4; g += 2) {
+              uint32_t m[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                const int i = q & 1, c = g + (q >> 1);
+                m[q] = pack2<T>(gate(value(2 * i, c, 0), value(2 * i + 1, c, 0)), gate(value(2 * i, c, 1), value(2 * i + 1, c, 1)));
+              }
+              store_transposed(at + g * 1024, m[0], m[1], m[2], m[3]);
+            }
+          } else {
+            const uint32_t piece = (quarter & 1) * 4 + (lane >> 3);
+            const uint32_t at = row_at + (quarter >> 1) * 4096 + ((piece ^ (lane & 7)) << 4);
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
               uint32_t m[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                m[i] = pack2<T>(fmaf(__uint_as_float(v[i >> 1][4 * g + 2 * (i & 1)]), alpha, b[i]),
-                                fmaf(__uint_as_float(v[i >> 1][4 * g + 2 * (i & 1) + 1]), alpha, b[i]));
-              store_transposed(at + g * 8 * pitch, m[0], m[1], m[2], m[3]);
+              for (int i = 0; i < 4; ++i) m[i] = pack2<T>(value(i, g, 0), value(i, g, 1));
+              store_transposed(at + g * 1024, m[0], m[1], m[2], m[3]);
+            }
+          }
+          const bool whole = p.y_vec && rows == kSlabRows;
+          if (whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          // the store from the other buffer has been read out: after the barrier that buffer may be written
+          if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          set_barrier(set);
+          if (whole) {
+            if (quarter == 0 && lane == 0) {
+              if (f0 < p.n) store_2d(&maps.y, f0, row0 + c0, out);
+              if (!p.gated && f0 + 64 < p.n) store_2d(&maps.y, f0 + 64, row0 + c0, out + 4096);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
             }
           } else {
-            const int c = half * 16;
-            uint32_t v[2][8], u[2][8];
-            load_16_lanes(taddr + c0 + c, v[0]);
-            load_16_lanes(taddr + c0 + c + (16u << 16), v[1]);
-            if (gated) {
-              load_16_lanes(taddr + p.bn + c0 + c, u[0]);
-              load_16_lanes(taddr + p.bn + c0 + c + (16u << 16), u[1]);
-              loads_done(u[0]);
-              loads_done(u[1]);
-            }
-            loads_done(v[0]);
-            loads_done(v[1]);
+            const int pieces = p.gated ? 8 : 16;
+            for (int i = quarter * 32 + lane; i < rows * pieces; i += 128) {
+              const int r = p.gated ? i >> 3 : i >> 4, q = i & (pieces - 1), f = f0 + q * 8;
+              if (f >= p.n) continue;
+              uint32_t w[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                           : "r"(out + (q >> 3) * 4096 + r * 128 + (((q & 7) ^ (r & 7)) << 4)));
+              T* to = y + (row0 + c0 + r) * p.y_stride + f;
+              if (p.y_vec && f + 8 <= p.n) {
+                *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+              } else {
 #pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              uint32_t m[4];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int r = 4 * g + 2 * (i & 1);
-                float v0 = fmaf(__uint_as_float(v[i >> 1][r]), alpha, b[i]), v1 = fmaf(__uint_as_float(v[i >> 1][r + 1]), alpha, b[i]);
-                if (gated) {
-                  v0 = gate(v0, fmaf(__uint_as_float(u[i >> 1][r]), alpha, b2[i]));
-                  v1 = gate(v1, fmaf(__uint_as_float(u[i >> 1][r + 1]), alpha, b2[i]));
-                }
-                m[i] = pack2<T>(v0, v1);
+                for (int k = 0; k < 8; ++k)
+                  if (f + k < p.n) reinterpret_cast<uint16_t*>(to)[k] = static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1)));
               }
-              store_transposed(at + (c + g * 8) * pitch, m[0], m[1], m[2], m[3]);
-            }
-          }
-          if (c0 + 32 >= tile.rows) {
-            // everything of this accumulator has been read
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(smem_u32(&h->acc_empty[buf]));
-          }
-          epilogue_barrier();
-          const int rows = min(32, tile.rows - c0);
-          for (int i = threadIdx.x - kFirstEpilogueWarp * 32; i < rows * pieces; i += kEpilogueWarps * 32) {
-            const int r = split ? i >> 4 : i >> 5, q = i & (pieces - 1);
-            const int f = f0 + q * 8;
-            if (f >= p.n) continue;
-            uint32_t w0, w1, w2, w3;
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w0), "=r"(w1), "=r"(w2), "=r"(w3) : "r"(out + r * pitch + ((q ^ (r & 7)) << 4)));
-            T* to = y + (row0 + c0 + r) * p.y_stride + f;
-            if (p.y_vec && f + 8 <= p.n) {
-              *reinterpret_cast<uint4*>(to) = make_uint4(w0, w1, w2, w3);
-            } else {
-              const uint32_t w[4] = {w0, w1, w2, w3};
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (f + k < p.n) reinterpret_cast<uint16_t*>(to)[k] = static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1)));
             }
           }
         }
       }
+      fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (CG == 1) mbar_arrive(smem_u32(&h->acc_empty[buf]));
+        else arrive_remote(in_first_cta(smem_u32(&h->acc_empty[buf])));
+      }
     }
+    if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   // ---------------------------------------------------------------- common exit
+  __syncwarp();
   fence_before();
-  __syncthreads();
+  if constexpr (CG == 1) __syncthreads();
+  else cluster_barrier();     // the other CTA's instructions and arrivals reach into this one's memory
   if (warp == 1) {
-    __syncwarp();
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
 }
 
-bool encode_rows(CUtensorMap* map, const void* base, int rank, uint64_t kbytes, uint64_t pitch, uint64_t rows, uint64_t mats, uint32_t box_rows) {
+// ---- host side ---------------------------------------------------------------
+
+bool encode(CUtensorMap* map, CUtensorMapDataType type, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+            CUtensorMapSwizzle swizzle) {
   EncodeTiledFn fn = get_encode_fn();
-  if (!fn) return false;
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  return fn && fn(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Rows of kbytes bytes, in boxes of one stage's bytes.
+bool encode_rows(CUtensorMap* map, const void* base, uint64_t kbytes, uint64_t pitch, uint64_t rows, uint64_t mats, int rank, uint32_t box_rows) {
   const cuuint64_t dims[3] = {kbytes, rows, mats}, strides[2] = {pitch, pitch * rows};
-  const cuuint32_t box[3] = {kStageBytes, box_rows, 1}, estr[3] = {1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, static_cast<cuuint32_t>(rank), const_cast<void*>(base), dims, strides, box, estr,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  const cuuint32_t box[3] = {kStageBytes, box_rows, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, rank, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// A gated W [experts][gate, up][n][kbytes]: eight rows of gate and eight of up in turn, 64 of each to a box.
+bool encode_gated(CUtensorMap* map, const void* base, uint64_t kbytes, uint64_t n, uint64_t experts) {
+  const cuuint64_t dims[5] = {kbytes, 8, 2, n / 8, experts}, strides[4] = {kbytes, kbytes * n, kbytes * 8, kbytes * n * 2};
+  const cuuint32_t box[5] = {kStageBytes, 8, 2, 8, 1};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, 5, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// Packed scales: tiles of 512 bytes.
+bool encode_scales(CUtensorMap* map, const void* base, uint64_t tiles, uint32_t box_tiles) {
+  const cuuint64_t dims[2] = {kScaleTile / 4, tiles}, strides[1] = {kScaleTile};
+  const cuuint32_t box[2] = {kScaleTile / 4, box_tiles};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+bool encode_y(CUtensorMap* map, void* base, uint64_t n, uint64_t rows, uint64_t stride) {
+  const cuuint64_t dims[2] = {n, rows}, strides[1] = {stride * 2};
+  const cuuint32_t box[2] = {64, kSlabRows};
+  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-template <int KIND, int P, typename T>
-cudaError_t start(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
-  auto* kernel = block_linear_kernel<KIND, P, T>;
+template <int KIND, int CG, typename T>
+cudaError_t start(const Maps& maps, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
+  auto* kernel = block_linear_kernel<KIND, CG, T>;
   // once per GPU (a repeated setting by racing first calls does no harm): the attribute costs a call a microsecond of the host's time
   static std::atomic<bool> ready[kMaxDevices];
   int dev = 0;
@@ -556,13 +664,33 @@ cudaError_t start(const CUtensorMap& w, const CUtensorMap& x, const LinearParams
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) ready[dev].store(true, std::memory_order_release);
   }
-  return launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, s, w, x, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (CG > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = CG;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cudaLaunchKernelEx(&cfg, kernel, maps, p);
 }
-template <int KIND, int P>
-cudaError_t start_typed(const CUtensorMap& w, const CUtensorMap& x, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
-  if (p.y_dtype == B2VX_DT_FLOAT32) return start<KIND, P, float>(w, x, p, grid, smem, s);
-  if (p.y_dtype == B2VX_DT_FLOAT16) return start<KIND, P, __half>(w, x, p, grid, smem, s);
-  return start<KIND, P, __nv_bfloat16>(w, x, p, grid, smem, s);
+template <int KIND, int CG>
+cudaError_t start_typed(const Maps& m, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
+  if (p.y_dtype == B2VX_DT_FLOAT32) return start<KIND, CG, float>(m, p, grid, smem, s);
+  if (p.y_dtype == B2VX_DT_FLOAT16) return start<KIND, CG, __half>(m, p, grid, smem, s);
+  return start<KIND, CG, __nv_bfloat16>(m, p, grid, smem, s);
 }
 
 }  // namespace
@@ -578,39 +706,34 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   p.gated = a.gated;
   const uint64_t kbytes = fp4 ? static_cast<uint64_t>(a.k) / 2 : static_cast<uint64_t>(a.k) * 2;
   p.k_stages = static_cast<int>((kbytes + kStageBytes - 1) / kStageBytes);
-  p.words = p.k_stages * nw;
-  p.scale_tiles = static_cast<int>((a.n + 127) / 128);
+  p.scale_tiles = static_cast<int>(weight_tiles(a.n, a.gated));
 
-  const long long mean = (a.rows + a.experts - 1) / a.experts;
-  p.bn = mean <= 64 ? 64 : (mean <= 128 ? 128 : 192);
-  // Two tiles of W per CTA halve what x costs per product; one tile makes twice as many tiles.
+  // Two CTAs to a tile where groups have more rows than a tile of one has; 192 rows leave room for two accumulators and two slots of scales.
   const int groups = static_cast<int>(std::min<long long>(a.experts, a.rows));
-  const long long tiles2 = ((a.n + 255) / 256) * ((mean + p.bn - 1) / p.bn) * groups;
-  const int P = a.gated || tiles2 >= 2 * a.sm_count ? 2 : 1;
-  p.feature_tiles = a.gated ? p.scale_tiles : (p.scale_tiles + P - 1) / P;
+  const long long mean = (a.rows + groups - 1) / groups;
+  const int cg = mean <= 64 ? 1 : 2;
+  p.bn = mean <= 64 ? 64 : (mean <= 128 ? 128 : 192);
+  p.x_box = p.bn / cg;
+  p.feature_tiles = (p.scale_tiles + cg - 1) / cg;
   p.sfb_atoms = fp4 ? (p.bn + 127) / 128 + (p.bn % 128 ? 0 : 1) : 0;   // tiles start on multiples of 64 rows
-  if (p.bn == 64) p.sfb_atoms = fp4 ? 1 : 0;
-  p.acc_cols = P * p.bn;
-  p.sf_cols = (P + p.sfb_atoms) * nw * 4;
-  p.acc_bufs = 2 * p.acc_cols + 2 * p.sf_cols <= 512 ? 2 : 1;
-  p.sf_base = p.acc_bufs * p.acc_cols;
-  p.stage_bytes = (P * 128 + p.bn) * kStageBytes + (P + p.sfb_atoms) * nw * kScaleTile;
+  p.sf_cols = (1 + p.sfb_atoms) * nw * 4;
+  p.acc_bufs = 2;
+  p.sf_base = 2 * p.bn;
+  p.stage_bytes = (128 + p.x_box) * kStageBytes + (1 + p.sfb_atoms) * nw * kScaleTile;
   p.stage_bytes = (p.stage_bytes + 1023u) & ~1023u;
   const int elem = a.y_dtype == B2VX_DT_FLOAT32 ? 4 : 2;
   p.y_vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride * elem % 16 == 0;
-  p.slab_bytes = elem == 4 ? 0 : 32 * 256 * (P == 2 && !a.gated ? 2 : 1);
-  const int header = 2 * p.slab_bytes + static_cast<int>(sizeof(Header)) + 8 * (a.experts + 1) + 1024;   // and the ring's alignment
-  p.stages = std::min(kMaxStages, static_cast<int>((kSmemBudget - header) / p.stage_bytes));
-  const size_t smem = std::max<size_t>(kMinDynSmem, p.stages * p.stage_bytes + header);
+  const int behind = kStagingBytes + static_cast<int>(sizeof(Header)) + 8 * (a.experts + 1) + 1024;   // and the ring's alignment
+  p.stages = std::min(kMaxStages, static_cast<int>((kSmemBudget - behind) / p.stage_bytes));
+  const size_t smem = std::max<size_t>(kMinDynSmem, p.stages * p.stage_bytes + behind);
+  const uint32_t m = 8u * cg << 24;
   if (fp4) {
     // a and b e2m1; scales e8m0 (block32) or e4m3
-    p.idesc = (1u << 7) | (1u << 10) | (a.format == B2VX_FP4_BLOCK32 ? 1u << 23 : 0u) | (8u << 24);
+    p.idesc = (1u << 7) | (1u << 10) | (a.format == B2VX_FP4_BLOCK32 ? 1u << 23 : 0u) | m;
   } else {
     const uint32_t t = a.x_dtype == B2VX_DT_FLOAT16 ? 0u : 1u;
-    p.idesc = (1u << 4) | (t << 7) | (t << 10) | (8u << 24);
+    p.idesc = (1u << 4) | (t << 7) | (t << 10) | m;
   }
-  p.w_scales = a.w_scales;
-  p.x_scales = a.x_scales;
   p.x_scale = a.x_scale;
   p.w_scale = a.w_scale;
   p.bias = a.bias;
@@ -619,20 +742,30 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   p.y_stride = a.y_stride;
   p.y_dtype = a.y_dtype;
   p.status = a.status;
+  p.x_scale_tiles = fp4 ? static_cast<int>(expert_scale_rows(a.rows, a.experts) / 128) : 0;
+  p.after_operand = a.after_operand;
 
-  CUtensorMap map_w, map_x;
-  const uint64_t mats = static_cast<uint64_t>(a.experts) * (a.gated ? 2 : 1);
-  if (!encode_rows(&map_w, a.w, 3, kbytes, kbytes, a.n, mats, 128) ||
-      !encode_rows(&map_x, a.x, 2, kbytes, static_cast<uint64_t>(a.x_pitch), a.rows, 1, kBoxRows)) {
+  Maps maps = {};
+  const uint64_t rows = static_cast<uint64_t>(a.rows), x_pitch = static_cast<uint64_t>(a.x_pitch);
+  const uint64_t w_tiles = static_cast<uint64_t>(a.experts) * p.k_stages * p.scale_tiles * nw, x_tiles = static_cast<uint64_t>(p.k_stages) * p.x_scale_tiles * nw;
+  if (w_tiles >= 1ull << 31 || x_tiles >= 1ull << 31) {
+    *why = "the product has too many scale tiles";
+    return cudaErrorInvalidValue;
+  }
+  bool ok = a.gated ? encode_gated(&maps.w, a.w, kbytes, a.n, a.experts) : encode_rows(&maps.w, a.w, kbytes, kbytes, a.n, a.experts, 3, 128);
+  ok = ok && encode_rows(&maps.x, a.x, kbytes, x_pitch, rows, 1, 2, p.x_box) && encode_rows(&maps.x32, a.x, kbytes, x_pitch, rows, 1, 2, kBoxRows);
+  if (fp4) ok = ok && encode_scales(&maps.w_scales, a.w_scales, w_tiles, nw) && encode_scales(&maps.x_scales, a.x_scales, x_tiles, nw);
+  if (p.y_vec && elem == 2) ok = ok && encode_y(&maps.y, a.y, a.n, rows, a.y_stride);
+  if (!ok) {
     *why = "tensor map refused";
     return cudaErrorInvalidValue;
   }
   const long long most = (a.rows / p.bn + groups) * p.feature_tiles;
-  const int grid = static_cast<int>(std::max<long long>(1, std::min<long long>(a.sm_count, most)));
-  if (a.format == 0) return P == 2 ? start_typed<0, 2>(map_w, map_x, p, grid, smem, s) : start_typed<0, 1>(map_w, map_x, p, grid, smem, s);
+  const int grid = static_cast<int>(std::max<long long>(1, std::min<long long>(a.sm_count / cg, most))) * cg;
+  if (a.format == 0) return cg == 2 ? start_typed<0, 2>(maps, p, grid, smem, s) : start_typed<0, 1>(maps, p, grid, smem, s);
   if (a.format == B2VX_FP4_BLOCK32)
-    return P == 2 ? start_typed<B2VX_FP4_BLOCK32, 2>(map_w, map_x, p, grid, smem, s) : start_typed<B2VX_FP4_BLOCK32, 1>(map_w, map_x, p, grid, smem, s);
-  return P == 2 ? start_typed<B2VX_FP4_BLOCK16, 2>(map_w, map_x, p, grid, smem, s) : start_typed<B2VX_FP4_BLOCK16, 1>(map_w, map_x, p, grid, smem, s);
+    return cg == 2 ? start_typed<B2VX_FP4_BLOCK32, 2>(maps, p, grid, smem, s) : start_typed<B2VX_FP4_BLOCK32, 1>(maps, p, grid, smem, s);
+  return cg == 2 ? start_typed<B2VX_FP4_BLOCK16, 2>(maps, p, grid, smem, s) : start_typed<B2VX_FP4_BLOCK16, 1>(maps, p, grid, smem, s);
 }
 
 }  // namespace b2vx

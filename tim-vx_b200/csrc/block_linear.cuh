@@ -16,7 +16,8 @@ __host__ __device__ constexpr int fp4_block(int format) { return format == B2VX_
 
 // Scales of a product's operand ("packed"): tiles of 128 rows x 4 blocks, 512 bytes each, which is the form the tensor pipe takes
 // its scales in.  Row r's four bytes of a tile lie at (r % 32) * 16 + (r / 32) * 4: a copy of the tile into tensor memory puts rows
-// 32 c .. 32 c + 31 into its column c.  Tiles run along K first, padded to whole pipeline stages of 256 columns.
+// 32 c .. 32 c + 31 into its column c.  Order: [pipeline stage of 256 columns][128-row tile][tile of the stage], so that what a stage
+// needs of neighbouring row tiles is one piece of memory.
 constexpr int kScaleTile = 512;
 constexpr int kStageBytes = 128;                       // bytes of K per row and pipeline stage
 constexpr int kMaxExperts = 1024;
@@ -24,8 +25,10 @@ __host__ __device__ constexpr int scale_words_per_stage(int format) { return 256
 __host__ __device__ inline long long scale_words(long long k, int format) {
   return (k + 255) / 256 * scale_words_per_stage(format);
 }
-__host__ __device__ inline size_t packed_scale_bytes(long long matrices, long long rows, long long k, int format) {
-  return static_cast<size_t>(matrices) * ((rows + 127) / 128) * scale_words(k, format) * kScaleTile;
+// 128-row tiles of a matrix with n features; those of a gated one hold 64 gate and 64 up rows, in turn eight of each.
+__host__ __device__ inline long long weight_tiles(long long n, int gated) { return gated ? (n + 63) / 64 : (n + 127) / 128; }
+__host__ __device__ inline size_t packed_scale_bytes(long long matrices, long long n, int gated, long long k, int format) {
+  return static_cast<size_t>(matrices) * weight_tiles(n, gated) * scale_words(k, format) * kScaleTile;
 }
 // Rows of the packed scales of an operand whose rows belong to `experts` groups: each group starts on a tile of its own.  Group e,
 // whose first row is lo, starts at scale row expert_scale_row(lo, e); since roundup(a) + roundup(b) <= roundup(a + b) + 128, groups do
@@ -48,12 +51,13 @@ struct QuantizeArgs {
   long long scales_pitch;      // bytes; 0: packed
   const int32_t* offsets;      // packed: the groups, or null for one group of all rows
   int experts;
+  long long scale_tiles;       // packed: 128-row tiles of the scale rows
 };
 cudaError_t launch_fp4_quantize(const QuantizeArgs& a, cudaStream_t s);
 cudaError_t launch_fp4_dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
                                   const float* tensor_scale, int format, long long rows, long long k, void* y, int y_dtype,
                                   long long y_stride, cudaStream_t s);
-cudaError_t launch_fp4_pack_scales(const uint8_t* scales, int format, long long matrices, long long n, long long k, uint8_t* packed, cudaStream_t s);
+cudaError_t launch_fp4_pack_scales(const uint8_t* scales, int format, long long matrices, long long n, int gated, long long k, uint8_t* packed, cudaStream_t s);
 // rows of 16-bit numbers, gathered: y[i] = x[row_index[i]] (zeros where the index is out of range), K contiguous in y
 cudaError_t launch_gather_rows(const void* x, long long x_stride, long long x_rows, const int32_t* row_index, long long rows, long long k,
                                void* y, cudaStream_t s);
@@ -76,6 +80,7 @@ struct LinearArgs {
   const int32_t* offsets;
   void* y;
   long long y_stride;          // elements
+  bool after_operand;          // the kernel before this one in the stream made x and x_scales, and waited for all before it
   int* status;
   int sm_count;
 };

@@ -86,7 +86,7 @@ Workspace workspace_of(const b2vx_linear_desc& d) {
   if (d.w_format) {
     w.codes_pitch = d.k / 2;
     w.codes = round256(d.rows * w.codes_pitch);
-    w.scales = round256(packed_scale_bytes(1, expert_scale_rows(d.rows, d.experts ? d.experts : 1), d.k, d.w_format));
+    w.scales = round256(packed_scale_bytes(1, expert_scale_rows(d.rows, d.experts ? d.experts : 1), 0, d.k, d.w_format));
   } else {
     w.codes_pitch = d.k * 2;
     w.codes = round256(d.rows * w.codes_pitch);
@@ -101,6 +101,7 @@ b2vx_status check_linear(const b2vx_linear_desc* d, char* err, size_t err_len) {
   B2VX_NEED(is_float(d->x_dtype) && is_float(d->y_dtype), "x and y must be float32, float16 or bfloat16");
   B2VX_NEED(d->w_format || d->x_dtype != B2VX_DT_FLOAT32, "a product with 16-bit weights needs x of the weights' type, float16 or bfloat16");
   B2VX_NEED(d->gated == 0 || d->gated == 1, "gated must be 0 or 1");
+  B2VX_NEED(!d->gated || d->n % 8 == 0, "n of a gated product must be a multiple of 8");
   B2VX_NEED(d->experts <= static_cast<uint32_t>(kMaxExperts), "at most 1024 experts");
   B2VX_NEED(d->n <= kMaxExtent && d->k <= kMaxExtent && d->rows <= kMaxExtent && d->x_rows <= kMaxExtent, "an extent is out of range");
   B2VX_NEED(d->k > 0, "k must not be zero");
@@ -142,6 +143,7 @@ extern "C" b2vx_status b2vx_fp4_quantize_noalloc(const b2vx_fp4_quantize_desc* d
   a.row_index = row_index; a.tensor_scale = tensor_scale; a.format = d->format;
   a.codes = static_cast<uint8_t*>(codes); a.codes_pitch = static_cast<long long>(d->codes_pitch);
   a.scales = static_cast<uint8_t*>(scales); a.scales_pitch = rows_layout ? static_cast<long long>(d->scales_pitch) : 0;
+  a.scale_tiles = (a.rows + 127) / 128;
   return launched(launch_fp4_quantize(a, static_cast<cudaStream_t>(cuda_stream)), err, err_len);
 }
 
@@ -168,23 +170,23 @@ extern "C" b2vx_status b2vx_fp4_dequantize_noalloc(const b2vx_fp4_dequantize_des
                   err, err_len);
 }
 
-extern "C" b2vx_status b2vx_fp4_packed_scales_size_noalloc(int32_t format, uint64_t matrices, uint64_t rows, uint64_t k, size_t* bytes) {
-  if (!bytes || !is_fp4(format) || matrices > 2 * static_cast<uint64_t>(kMaxExperts) || rows > kMaxExtent || k > kMaxExtent) return B2VX_INVALID_ARG;
-  *bytes = packed_scale_bytes(static_cast<long long>(matrices), static_cast<long long>(rows), static_cast<long long>(k), format);
+extern "C" b2vx_status b2vx_fp4_packed_scales_size_noalloc(int32_t format, uint64_t matrices, uint64_t n, int32_t gated, uint64_t k, size_t* bytes) {
+  if (!bytes || !is_fp4(format) || matrices > static_cast<uint64_t>(kMaxExperts) || n > kMaxExtent || k > kMaxExtent || (gated != 0 && gated != 1)) return B2VX_INVALID_ARG;
+  *bytes = packed_scale_bytes(static_cast<long long>(matrices), static_cast<long long>(n), gated, static_cast<long long>(k), format);
   return B2VX_OK;
 }
 
-extern "C" b2vx_status b2vx_fp4_pack_scales_noalloc(int32_t format, uint64_t matrices, uint64_t rows, uint64_t k, const void* scales, void* packed,
+extern "C" b2vx_status b2vx_fp4_pack_scales_noalloc(int32_t format, uint64_t matrices, uint64_t n, int32_t gated, uint64_t k, const void* scales, void* packed,
                                                     void* cuda_stream, char* err, size_t err_len) {
   size_t bytes = 0;
-  B2VX_NEED(b2vx_fp4_packed_scales_size_noalloc(format, matrices, rows, k, &bytes) == B2VX_OK, "unknown format or an extent out of range");
+  B2VX_NEED(b2vx_fp4_packed_scales_size_noalloc(format, matrices, n, gated, k, &bytes) == B2VX_OK, "unknown format or an extent out of range");
   if (bytes == 0) return B2VX_OK;
   B2VX_NEED(scales && packed, "null argument");
   B2VX_NEED(aligned(packed, 16), "packed must be 16-byte aligned");
   PerDevice* pd;
   b2vx_status st = device(&pd, err, err_len);
   if (st != B2VX_OK) return st;
-  return launched(launch_fp4_pack_scales(static_cast<const uint8_t*>(scales), format, static_cast<long long>(matrices), static_cast<long long>(rows),
+  return launched(launch_fp4_pack_scales(static_cast<const uint8_t*>(scales), format, static_cast<long long>(matrices), static_cast<long long>(n), gated,
                                          static_cast<long long>(k), static_cast<uint8_t*>(packed), static_cast<cudaStream_t>(cuda_stream)),
                   err, err_len);
 }
@@ -229,6 +231,7 @@ extern "C" b2vx_status b2vx_linear_noalloc(const b2vx_linear_desc* d, const b2vx
   l.w = a->w; l.w_scales = static_cast<const uint8_t*>(a->w_scales);
   l.x_scale = a->x_scale; l.w_scale = a->w_scale; l.bias = a->bias; l.offsets = a->offsets;
   l.y = a->y; l.y_stride = static_cast<long long>(d->y_stride);
+  l.after_operand = !direct;
   l.status = pd->status; l.sm_count = pd->sm_count;
   cudaError_t e = cudaSuccess;
   if (fp4) {
@@ -239,6 +242,7 @@ extern "C" b2vx_status b2vx_linear_noalloc(const b2vx_linear_desc* d, const b2vx
     q.codes = codes; q.codes_pitch = static_cast<long long>(ws.codes_pitch);
     q.scales = codes + ws.codes; q.scales_pitch = 0;
     q.offsets = a->offsets; q.experts = l.experts;
+    q.scale_tiles = expert_scale_rows(l.rows, l.experts) / 128;
     e = launch_fp4_quantize(q, s);
     l.x = codes; l.x_pitch = static_cast<long long>(ws.codes_pitch); l.x_scales = q.scales;
   } else if (direct) {

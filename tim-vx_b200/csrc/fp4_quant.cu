@@ -55,8 +55,8 @@ __device__ __forceinline__ int group_of(const int32_t* offsets, int experts, lon
 template <typename T, int FORMAT, bool VEC, bool PACKED>
 __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArgs a, int chunks, int split) {
   constexpr int B = fp4_block(FORMAT), LANES = B / 8;
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();   // after the wait: a product behind this kernel may read its weights before its own wait
   const int lane = threadIdx.x & 31;
   const long long warps = static_cast<long long>(gridDim.x) * kWarps;
   const float g = FORMAT == B2VX_FP4_BLOCK16 ? __ldg(a.tensor_scale) : 1.0f;
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArg
         const long long lo = e < a.experts ? a.offsets[e] : -1;
         at = lo >= 0 && lo <= row ? expert_scale_row(lo, e) + row - lo : -1;
       }
-      if (at >= 0) tile = a.scales + (at / 128) * scale_words(a.k, FORMAT) * kScaleTile + (at % 32) * 16 + (at % 128 / 32) * 4;
+      if (at >= 0) tile = a.scales + at / 128 * (scale_words_per_stage(FORMAT) * kScaleTile) + (at % 32) * 16 + (at % 128 / 32) * 4;
     }
     for (int chunk = part; chunk < chunks; chunk += split) {
       const long long c = static_cast<long long>(chunk) * kChunk + lane * 8;
@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArg
         uint32_t word = byte | __shfl_down_sync(0xffffffffu, byte, LANES) << 8;
         word |= __shfl_down_sync(0xffffffffu, word, 2 * LANES) << 16;
         if (lane % (4 * LANES) == 0 && tile)
-          *reinterpret_cast<uint32_t*>(tile + (static_cast<long long>(chunk) * scale_words_per_stage(FORMAT) + lane / (4 * LANES)) * kScaleTile) = word;
+          *reinterpret_cast<uint32_t*>(tile + (chunk * a.scale_tiles * scale_words_per_stage(FORMAT) + lane / (4 * LANES)) * kScaleTile) = word;
       } else if (lane % LANES == 0 && c / B < blocks) {
         a.scales[row * a.scales_pitch + c / B] = static_cast<uint8_t>(byte);
       }
@@ -129,29 +129,32 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* codes, l
   }
 }
 
-// One thread per word (four blocks of a row) of the packed layout.
-__global__ void __launch_bounds__(256) pack_scales_kernel(const uint8_t* scales, long long matrices, long long n, long long blocks, long long words,
-                                                          uint32_t* packed) {
+// One thread per word (four blocks of a row) of the packed layout; per: words of a row and stage.
+__global__ void __launch_bounds__(256) pack_scales_kernel(const uint8_t* scales, long long matrices, long long n, int gated, long long blocks,
+                                                          long long words, int per, uint32_t* packed) {
   pdl_trigger();
   pdl_wait();
-  const long long tiles = (n + 127) / 128, total = matrices * tiles * words * 128, step = static_cast<long long>(gridDim.x) * blockDim.x;
+  const long long tiles = weight_tiles(n, gated), total = matrices * tiles * words * 128, step = static_cast<long long>(gridDim.x) * blockDim.x;
   for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
-    const int in = static_cast<int>(i & 127);
-    const long long w = (i >> 7) % words, t = (i >> 7) / words % tiles, m = (i >> 7) / words / tiles;
-    const long long row = t * 128 + (in & 3) * 32 + (in >> 2);
+    const int in = static_cast<int>(i & 127), r = (in & 3) * 32 + (in >> 2);
+    const long long m = (i >> 7) / (words * tiles), in_matrix = (i >> 7) % (words * tiles);
+    const long long t = in_matrix / per % tiles, w = in_matrix / (per * tiles) * per + in_matrix % per;
+    const long long f = gated ? t * 64 + (r >> 4) * 8 + (r & 7) : t * 128 + r;
     uint32_t word = 0;
-    if (row < n)
+    if (f < n) {
+      const long long row = gated ? (2 * m + ((r >> 3) & 1)) * n + f : m * n + f;
 #pragma unroll
       for (int b = 0; b < 4; ++b)
-        if (w * 4 + b < blocks) word |= static_cast<uint32_t>(scales[(m * n + row) * blocks + w * 4 + b]) << (8 * b);
+        if (w * 4 + b < blocks) word |= static_cast<uint32_t>(scales[row * blocks + w * 4 + b]) << (8 * b);
+    }
     packed[i] = word;
   }
 }
 
 __global__ void __launch_bounds__(256) gather_rows_kernel(const uint16_t* x, long long x_stride, long long x_rows, const int32_t* row_index,
                                                           long long rows, long long k, int pieces, uint4* y, int vec) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();   // as above
   const long long total = rows * pieces, step = static_cast<long long>(gridDim.x) * blockDim.x;
   for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
     const long long row = i / pieces, c = (i - row * pieces) * 8;
@@ -220,11 +223,12 @@ cudaError_t launch_fp4_dequantize(const uint8_t* codes, long long codes_pitch, c
   if (y_dtype == B2VX_DT_FLOAT16) return dequantize<__half>(codes, codes_pitch, scales, scales_pitch, tensor_scale, format, rows, k, y, y_stride, s);
   return dequantize<__nv_bfloat16>(codes, codes_pitch, scales, scales_pitch, tensor_scale, format, rows, k, y, y_stride, s);
 }
-cudaError_t launch_fp4_pack_scales(const uint8_t* scales, int format, long long matrices, long long n, long long k, uint8_t* packed, cudaStream_t s) {
+cudaError_t launch_fp4_pack_scales(const uint8_t* scales, int format, long long matrices, long long n, int gated, long long k, uint8_t* packed,
+                                   cudaStream_t s) {
   const long long blocks = (k + fp4_block(format) - 1) / fp4_block(format), words = scale_words(k, format);
-  const long long total = static_cast<long long>(packed_scale_bytes(matrices, n, k, format) / 4);
-  return launch_pdl(pack_scales_kernel, dim3(blocks_for(total, 256)), dim3(256), 0, s, scales, matrices, n, blocks, words,
-                    reinterpret_cast<uint32_t*>(packed));
+  const long long total = static_cast<long long>(packed_scale_bytes(matrices, n, gated, k, format) / 4);
+  return launch_pdl(pack_scales_kernel, dim3(blocks_for(total, 256)), dim3(256), 0, s, scales, matrices, n, gated, blocks, words,
+                    scale_words_per_stage(format), reinterpret_cast<uint32_t*>(packed));
 }
 cudaError_t launch_gather_rows(const void* x, long long x_stride, long long x_rows, const int32_t* row_index, long long rows, long long k, void* y,
                                cudaStream_t s) {

@@ -51,7 +51,7 @@ class Fp4Weight:
     """4-bit weights [n][k] or, of experts, [experts][n][k] as codes [..][n][k / 2] and scale bytes [..][n][k / block], whose scales are laid
     out for the products here, once.  The codes are used where they lie.
 
-    scale (block16): float32, one for each matrix.  gated: the matrices are [2 n][k], gate rows first."""
+    scale (block16): float32, one for each matrix.  gated: the matrices are [2 n][k], gate rows first, n a multiple of 8."""
 
     def __init__(self, codes, scales, format="block32", scale=None, gated=False):
         self.code, self.gated = _format(format), bool(gated)
@@ -60,16 +60,14 @@ class Fp4Weight:
         rows, k = codes.shape[-2], codes.shape[-1] * 2
         if k % 32:
             raise ValueError("k must be a multiple of 32")
-        if gated and rows % 2:
-            raise ValueError("a gated weight has an even number of rows")
+        if gated and rows % 16:
+            raise ValueError("the rows of a gated weight must be a multiple of 16")
         if tuple(scales.shape) != tuple(codes.shape[:-1]) + (k // BLOCK[format],) or scales.device != codes.device:
             raise ValueError("scales must have the shape %s on the codes' device" % (tuple(codes.shape[:-1]) + (k // BLOCK[format],),))
         if (scale is not None) != (format == "block16"):
             raise ValueError("scale belongs to block16 and only to it")
         self.codes, self.scale, self.format = codes, scale, format
-        matrices = (codes.shape[0] if codes.dim() == 3 else 1) * (2 if gated else 1)
-        parts = 2 if gated else 1
-        self.packed = _native.pack(scales.reshape(matrices, rows // parts, k // BLOCK[format]), self.code)
+        self.packed = _native.pack(scales.reshape(-1, rows, k // BLOCK[format]), self.code, self.gated)
 
 
 def _product(x, weight, offsets, row_index, bias, gated, x_scale, out_dtype, out):
