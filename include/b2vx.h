@@ -334,22 +334,20 @@ b2vx_status b2vx_conv2d_first_layer_noalloc(const b2vx_conv2d_noalloc_desc* d, c
  *                     tensor scale, rounded to nearest even, at most 448
  * Numbers are divided by their scale exactly, rounded to nearest even and cut to
  * +-6.  A block that holds a NaN or an infinity gets the scale NaN and codes 0.
- * Scales come in two layouts: B2VX_SCALES_ROWS, [rows][blocks of a row], and
- * B2VX_SCALES_PACKED, the operand layout of the products (tiles of 128 rows x 4
- * blocks), whose size b2vx_fp4_packed_scales_size_noalloc tells. */
+ * Scales lie as [rows][blocks of a row]; those of a product's weights are packed
+ * once for the tensor pipe (b2vx_fp4_pack_scales_noalloc). */
 #define B2VX_DT_BFLOAT16 16
 enum { B2VX_FP4_BLOCK32 = 1, B2VX_FP4_BLOCK16 = 2 };
-enum { B2VX_SCALES_ROWS = 0, B2VX_SCALES_PACKED = 1 };
 
 /* x [x_rows][x_stride] (float32, float16 or bfloat16) to codes [rows][codes_pitch]
  * and scales.  codes_pitch (bytes): a multiple of 4, at least k rounded up to 32,
- * over 2; columns from k to there get code 0.  scales_pitch (bytes, layout ROWS): at
+ * over 2; columns from k to there get code 0.  scales_pitch (bytes): at
  * least ceil(k / block).  row_index (int32 [rows], may be NULL): output row i is
  * row row_index[i] of x, a row of zeros where that is outside 0..x_rows-1.
  * tensor_scale: one float, BLOCK16 only; a scale that is not positive and finite
  * makes every block NaN. */
 typedef struct b2vx_fp4_quantize_desc {
-  int32_t format, scales_layout, x_dtype;
+  int32_t format, x_dtype;
   uint64_t x_rows, rows, k;
   uint64_t x_stride;        /* elements between rows of x */
   uint64_t codes_pitch, scales_pitch;
@@ -357,7 +355,7 @@ typedef struct b2vx_fp4_quantize_desc {
 b2vx_status b2vx_fp4_quantize_noalloc(const b2vx_fp4_quantize_desc* d, const void* x, const int32_t* row_index,
                                       const float* tensor_scale, void* codes, void* scales,
                                       void* cuda_stream, char* err, size_t err_len);
-/* The values that codes and scales (layout ROWS) stand for, times the tensor scale, rounded once to y_dtype. */
+/* The values that codes and scales stand for, times the tensor scale, rounded once to y_dtype. */
 typedef struct b2vx_fp4_dequantize_desc {
   int32_t format, y_dtype;
   uint64_t rows, k;

@@ -7,7 +7,7 @@ _vp, _u64, _u32, _i32, _sz = C.c_void_p, C.c_uint64, C.c_uint32, C.c_int32, C.c_
 
 
 class QuantizeDesc(C.Structure):
-    _fields_ = [("format", _i32), ("scales_layout", _i32), ("x_dtype", _i32), ("x_rows", _u64), ("rows", _u64), ("k", _u64), ("x_stride", _u64),
+    _fields_ = [("format", _i32), ("x_dtype", _i32), ("x_rows", _u64), ("rows", _u64), ("k", _u64), ("x_stride", _u64),
                 ("codes_pitch", _u64), ("scales_pitch", _u64)]
 
 

@@ -18,7 +18,7 @@ def desc(cls, base, **change):
     return d
 
 
-QUANTIZE = dict(format=1, scales_layout=0, x_dtype=16, x_rows=8, rows=8, k=96, x_stride=96, codes_pitch=48, scales_pitch=3)
+QUANTIZE = dict(format=1, x_dtype=16, x_rows=8, rows=8, k=96, x_stride=96, codes_pitch=48, scales_pitch=3)
 DEQUANTIZE = dict(format=1, y_dtype=16, rows=8, k=96, codes_pitch=48, scales_pitch=3, y_stride=96)
 LINEAR = dict(w_format=1, x_dtype=16, y_dtype=16, gated=0, experts=0, x_rows=8, rows=8, n=64, k=96, x_stride=96, y_stride=64)
 ROUTE = dict(logits_dtype=9, normalize=1, experts=16, top_k=4, tokens=8, logits_stride=16)
@@ -35,7 +35,7 @@ def refused(fn, *args):
 
 
 @pytest.mark.parametrize("change,scale,words", [
-    (dict(format=0), None, "format"), (dict(format=3), None, "format"), (dict(scales_layout=2), None, "layout"), (dict(x_dtype=2), None, "float32"),
+    (dict(format=0), None, "format"), (dict(format=3), None, "format"), (dict(x_dtype=2), None, "float32"),
     (dict(k=1 << 30), None, "range"), (dict(rows=1 << 30), None, "range"), (dict(x_stride=95), None, "x_stride"), (dict(x_stride=1 << 41), None, "x_stride"),
     (dict(codes_pitch=44), None, "codes_pitch"), (dict(codes_pitch=49), None, "codes_pitch"), (dict(scales_pitch=2), None, "scales_pitch"),
     (dict(format=2, scales_pitch=6), None, "tensor scale"), (dict(), PTR, "tensor scale"), (dict(rows=9), None, "row_index")])
@@ -52,8 +52,6 @@ def test_quantize_refuses_pointers():
         assert "null" in refused(fn, d, *args)
     assert "aligned" in refused(fn, d, PTR + 1, None, None, PTR, PTR, None)
     assert "aligned" in refused(fn, d, PTR, None, None, PTR + 2, PTR, None)
-    packed = C.byref(desc(ABI.QuantizeDesc, QUANTIZE, scales_layout=1))
-    assert "aligned" in refused(fn, packed, PTR, None, None, PTR, PTR + 4, None)
 
 
 @pytest.mark.parametrize("change,scale,words", [
@@ -160,27 +158,27 @@ def test_sizes():
     assert packed_size(1, 2, 72, 64, 1) == 2 * 2 * 2 * 512     # gated: 64 features to a tile
     size = C.c_size_t()
     lib = ABI.library()
-    # codes of 8 rows, 48 bytes each, and scales of one tile for the rows and one for the group's own start
+    # codes of 8 rows, 48 bytes each, and two words of scales for a tile of each expert's
     assert lib.b2vx_linear_workspace_size_noalloc(C.byref(desc(ABI.LinearDesc, LINEAR)), C.byref(size), None, 0) == 0
-    assert size.value == 512 + 2 * 2 * 512
+    assert size.value == 512 + 2 * 512
     assert lib.b2vx_linear_workspace_size_noalloc(C.byref(desc(ABI.LinearDesc, LINEAR, experts=5)), C.byref(size), None, 0) == 0
-    assert size.value == 512 + 6 * 2 * 512
+    assert size.value == 512 + 5 * 2 * 512
 
 
-def test_group_scale_rows_do_not_overlap():
-    """The rule that gives every group of rows its own scale tiles: group e starts at roundup128(lo) + 128 e."""
+@pytest.mark.parametrize("bn", [64, 128, 192, 224])
+def test_group_scale_tiles_do_not_overlap(bn):
+    """The rule that gives every tile of a group's rows its own scale tiles: group e starts at (lo / bn + e) tiles of bn rows."""
     import random
-    rng = random.Random(5)
-    up = lambda v: (v + 127) // 128 * 128
+    rng = random.Random(bn)
     for _ in range(300):
-        counts = [rng.choice([0, 0, 1, 63, 127, 128, 129, rng.randrange(2000)]) for _ in range(rng.randrange(1, 40))]
+        counts = [rng.choice([0, 0, 1, bn - 1, bn, bn + 1, rng.randrange(2000)]) for _ in range(rng.randrange(1, 40))]
         lo, end = 0, 0
         for e, n in enumerate(counts):
-            first = up(lo) + 128 * e
+            first = lo // bn + e
             assert first >= end
-            end = first + up(n)
+            end = first + -(-n // bn)
             lo += n
-        assert end <= up(lo) + 128 * len(counts)
+        assert end <= lo // bn + len(counts)
 
 
 def test_tensors_must_be_on_a_gpu():

@@ -211,36 +211,26 @@ def test_quantize_views_and_row_index(fmt, dtype, offset, stride):
 
 
 @pytest.mark.parametrize("fmt", ["block32", "block16"])
-@pytest.mark.parametrize("rows,k", [(1, 32), (130, 288), (40, 1000)])
-def test_packed_layout(fmt, rows, k):
-    """Scales written packed equal scales written by rows and packed afterwards, and both the layout's rule."""
-    x = gaussian(rows, k, torch.bfloat16, 11)
-    s = scale_for(f64(x), fmt)
-    q = D.quantize_fp4(x, fmt, scale=s)
+@pytest.mark.parametrize("matrices,n,k,gated", [(1, 1, 32, False), (2, 130, 288, False), (1, 40, 1024, True), (3, 72, 96, True)])
+def test_pack_scales(fmt, matrices, n, k, gated):
+    """The layout's rule: [stage of 256 columns][128-row tile][tile of four blocks][row % 32][row / 32][block], gated rows eight by eight."""
+    f, b = D.FORMATS[fmt], D.BLOCK[fmt]
+    scales = torch.randint(0, 255, (matrices, 2 * n if gated else n, k // b), dtype=torch.uint8, device="cuda")
     size = C.c_size_t()
-    lib, f, b = ABI.library(), D.FORMATS[fmt], D.BLOCK[fmt]
-    assert lib.b2vx_fp4_packed_scales_size_noalloc(f, 1, rows, 0, k, C.byref(size)) == 0
-    direct = torch.full((size.value,), 0xAB, dtype=torch.uint8, device="cuda")
-    later = torch.full((size.value,), 0xCD, dtype=torch.uint8, device="cuda")
-    codes = torch.empty_like(q.codes)
-    d = ABI.QuantizeDesc(f, 1, 16, rows, rows, k, k, codes.shape[1], 0)
-    ABI.call(lib.b2vx_fp4_quantize_noalloc, C.byref(d), x.data_ptr(), None, None if s is None else s.data_ptr(), codes.data_ptr(), direct.data_ptr(), None)
-    ABI.call(lib.b2vx_fp4_pack_scales_noalloc, f, 1, rows, 0, k, q.scales.data_ptr(), later.data_ptr(), None)
+    assert ABI.library().b2vx_fp4_packed_scales_size_noalloc(f, matrices, n, int(gated), k, C.byref(size)) == 0
+    packed = torch.full((size.value,), 0xCD, dtype=torch.uint8, device="cuda")
+    ABI.call(ABI.library().b2vx_fp4_pack_scales_noalloc, f, matrices, n, int(gated), k, scales.data_ptr(), packed.data_ptr(), None)
     torch.cuda.synchronize()
-    assert torch.equal(codes, q.codes)
-    per = 256 // (4 * b)                                     # words (four blocks) of a stage of 256 columns
-    want = np.zeros(((k + 255) // 256, (rows + 127) // 128, per, 32, 4, 4), np.uint8)
-    byte = q.scales.cpu().numpy()
-    for r in range(rows):
-        for j in range(byte.shape[1]):
-            want[j // 4 // per, r // 128, j // 4 % per, r % 32, r % 128 // 32, j % 4] = byte[r, j]
-    assert np.array_equal(later.cpu().numpy(), want.reshape(-1))
-    got = direct.cpu().numpy().reshape(want.shape)
-    there = np.zeros((1, want.shape[1], 1, 32, 4, 1), bool)     # rows that do not exist are left alone
-    for r in range(rows):
-        there[0, r // 128, 0, r % 32, r % 128 // 32, 0] = True
-    assert np.array_equal(got[np.broadcast_to(there, got.shape)], want[np.broadcast_to(there, got.shape)])
-    assert (got[~np.broadcast_to(there, got.shape)] == 0xAB).all()
+    per = 256 // (4 * b)                                     # words (four blocks) of a stage
+    want = np.zeros((matrices, (k + 255) // 256, -(-n // 64) if gated else -(-n // 128), per, 32, 4, 4), np.uint8)
+    byte = scales.cpu().numpy()
+    for m in range(matrices):
+        for row in range(byte.shape[1]):
+            f, up = (row % n, row // n) if gated else (row, 0)
+            t, r = (f // 64, f % 64 // 8 * 16 + up * 8 + f % 8) if gated else (f // 128, f % 128)
+            for j in range(byte.shape[2]):
+                want[m, j // 4 // per, t, j // 4 % per, r % 32, r // 32, j % 4] = byte[m, row, j]
+    assert np.array_equal(packed.cpu().numpy(), want.reshape(-1))
 
 
 def test_quantize_beyond_two_gigaelements():

@@ -128,7 +128,7 @@ PyObject* quantize(PyObject* const* a) {
   void* index = dense(a[3], "row_index", at::kInt, {rows}, device);
   Call call(device);
   at::Tensor codes = empty({rows, (k + 31) / 32 * 16}, at::kByte, device), scales = empty({rows, (k + block - 1) / block}, at::kByte, device);
-  const b2vx_fp4_quantize_desc d = {static_cast<int32_t>(format), B2VX_SCALES_ROWS, dtype_code(x.scalar_type()), static_cast<uint64_t>(x.size(0)), static_cast<uint64_t>(rows),
+  const b2vx_fp4_quantize_desc d = {static_cast<int32_t>(format), dtype_code(x.scalar_type()), static_cast<uint64_t>(x.size(0)), static_cast<uint64_t>(rows),
                                     static_cast<uint64_t>(k), stride, static_cast<uint64_t>(codes.size(1)), static_cast<uint64_t>(scales.size(1))};
   call(b2vx_fp4_quantize_noalloc(&d, x.data_ptr(), static_cast<const int32_t*>(index), static_cast<const float*>(scale), codes.data_ptr(), scales.data_ptr(),
                                  call.stream, call.err, sizeof(call.err)));

@@ -10,9 +10,9 @@
 // thread of the epilogue finds the gate and the up sum of a feature in its own registers.
 //
 // Persistent CTAs, one per SM, warp-specialised:
-//   warps 0, 2  producers  of W and of x: per stage of 128 bytes of K one TMA box each (small ones of few rows) and the packed scales.
+//   warps 0, 2  producers  of W and of x: per k-block of 128 bytes one TMA box each (small ones of few rows) and the packed scales.
 //                          Two warps and few, large copies because a wait, an announcement and a copy take one thread about 340 cycles.
-//   warp 1      issuer     copies a stage's scales into tensor memory (tcgen05.cp, two slots in turn) and issues the stage's four K steps
+//   warp 1      issuer     copies a k-block's scales into tensor memory (tcgen05.cp, two slots in turn) and issues its four K steps
 //   warps 4-11  epilogue   two sets of four warps take slabs of 32 rows of the tile in turn: out of tensor memory, scale and bias,
 //                          activation, rounding, transposition into a buffer in shared memory, one TMA store
 //
@@ -40,10 +40,12 @@ constexpr int kThreads = 12 * 32;
 constexpr int kFirstEpilogueWarp = 4;
 constexpr int kEpilogueWarps = 8;
 constexpr int kMaxStages = 10;
+constexpr uint32_t kBufferColumns = 256;                   // of tensor memory: an accumulator of up to 224 columns (256 without scales) and a slot of scales behind it
+constexpr int kGroup = 2;                                  // k-blocks of a stage, and slots of scales in tensor memory
 constexpr int kBoxRows = 32;
 constexpr int kSlabRows = 32;
 constexpr int kSlabBytes = kSlabRows * 256;                // 128 features of 16 bits, two boxes of 64
-constexpr int kStagingBytes = 4 * kSlabBytes;              // two for each set
+constexpr int kStagingBytes = 2 * kSlabBytes;              // one for each set
 constexpr uint32_t kWTile = 128 * kStageBytes;
 constexpr int kSmemBudget = 226 * 1024;
 constexpr int kMaxDynSmem = 227 * 1024;
@@ -52,17 +54,16 @@ constexpr int kMinDynSmem = 120 * 1024;   // keeps two CTAs from sharing an SM a
 
 struct LinearParams {
   int n, rows, experts, gated;
-  int bn;                     // most rows of x in a tile, a multiple of 64
+  int bn;                     // most rows of x in a tile
   int feature_tiles;          // tiles along the features of one group
   int scale_tiles;            // 128-row tiles of one matrix of W (and of its packed scales)
-  int k_stages, stages, acc_bufs;
+  int k_blocks, stages;       // blocks of 128 bytes of K
   int x_box;                  // rows of x in the large box, bn / CG
-  int sfb_atoms;              // most scale tiles of x under one tile's rows
+  int sfb_atoms;              // scale tiles of x to a tile of bn rows
   int x_scale_tiles;          // packed scale tiles along the rows of x
   int after_operand;
-  uint32_t stage_bytes;
+  uint32_t block_bytes, stage_bytes;
   uint32_t idesc;             // without N
-  uint32_t sf_cols, sf_base;  // TMEM columns of a scale slot, first column of the slots
   const float* x_scale;
   const float* w_scale;
   const float* bias;
@@ -169,25 +170,25 @@ __device__ __forceinline__ void store_2d(const CUtensorMap* map, int c0, int c1,
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(src) : "memory");
 }
-// K-major operand rows of one 128-byte swizzle span: groups of eight rows 1024 bytes apart.
-__device__ __forceinline__ uint64_t operand_desc(uint32_t addr) {
-  return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-// A scale tile: 32 rows of 16 bytes, not swizzled, groups of eight rows 128 bytes apart.
-__device__ __forceinline__ uint64_t scale_desc(uint32_t addr) {
-  return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (1ull << 16) | (8ull << 32) | (1ull << 46);
-}
+// Descriptors of shared-memory operands as their low halves, start address in 16-byte units (addresses stay below 256 KB, so
+// additions do not leave that field), and constant high halves.
+//   operand: K-major rows of one 128-byte swizzle span, groups of eight rows 1024 bytes apart
+//   scales:  a tile of 32 rows of 16 bytes, not swizzled, groups of eight rows 128 bytes apart
+constexpr uint32_t kDescLow = 1u << 16;
+constexpr uint32_t kOperandHigh = 64u | (1u << 14) | (2u << 29), kScaleHigh = 8u | (1u << 14);
 template <int CG>
-__device__ __forceinline__ void copy_scales(uint32_t taddr, uint64_t desc) {
-  if constexpr (CG == 1) asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-  else asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+__device__ __forceinline__ void copy_scales(uint32_t taddr, uint32_t desc_low) {
+  if constexpr (CG == 1)
+    asm volatile("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\ttcgen05.cp.cta_group::1.32x128b.warpx4 [%0], d;\n\t}" ::"r"(taddr), "r"(desc_low), "n"(kScaleHigh) : "memory");
+  else
+    asm volatile("{\n\t.reg .b64 d;\n\tmov.b64 d, {%1, %2};\n\ttcgen05.cp.cta_group::2.32x128b.warpx4 [%0], d;\n\t}" ::"r"(taddr), "r"(desc_low), "n"(kScaleHigh) : "memory");
 }
-#define B2VX_MMA(group, kind, scales)                                                                 \
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                     \
-               "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3" scales ", p;\n\t}"   \
-               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory")
+#define B2VX_MMA(group, kind, scales)                                                                                      \
+  asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %7};\n\tmov.b64 db, {%2, %7};\n\tsetp.ne.b32 p, %6, 0;\n\t" \
+               "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], da, db, %3" scales ", p;\n\t}"                         \
+               ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate), "n"(kOperandHigh) : "memory")
 template <int KIND, int CG>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+__device__ __forceinline__ void mma(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
   if constexpr (KIND == 0 && CG == 1) B2VX_MMA("1", "f16", "");
   else if constexpr (KIND == 0) B2VX_MMA("2", "f16", "");
   else if constexpr (KIND == B2VX_FP4_BLOCK32 && CG == 1) B2VX_MMA("1", "mxf4.block_scale.scale_vec::2X", ", [%4], [%5]");
@@ -236,9 +237,10 @@ __device__ __forceinline__ bool set_all(int set, bool ok) {
   return r != 0;
 }
 
-// One tile of the schedule: group, its first row, first row inside it, rows (as they are and as the instruction's N), feature tile.
+// One tile of the schedule: group, its first row, the tile's number and first row inside it, rows (as they are and as the instruction's N),
+// feature tile.
 struct Tile {
-  int e, lo, r0, rows, n_mma, f;
+  int e, lo, i, r0, rows, n_mma, f;
 };
 template <int CG>
 __device__ __forceinline__ Tile tile_of(const int* lo, const int* start, const LinearParams& p, int t) {
@@ -249,12 +251,13 @@ __device__ __forceinline__ Tile tile_of(const int* lo, const int* start, const L
   }
   const int count = lo[a + 1] - lo[a], row_tiles = (count + p.bn - 1) / p.bn;
   const int i = t - start[a];
-  const int per = ((count + row_tiles - 1) / row_tiles + 63) & ~63;   // even shares, whole halves of a scale tile
+  const int per = rows_of_tile(count, p.bn);
   constexpr int step = 16 * CG;
   Tile r;
   r.e = a;
   r.f = i / row_tiles;
-  r.r0 = (i - r.f * row_tiles) * per;
+  r.i = i - r.f * row_tiles;
+  r.r0 = r.i * per;
   r.rows = max(0, min(per, count - r.r0));
   r.n_mma = max(step, (r.rows + step - 1) / step * step);
   r.lo = lo[a];
@@ -288,7 +291,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 1 ? 0u : cluster_rank();
   const int first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
-  // a stage: [128 rows of W | rows of x | scales of W | scales of x]
+  // a k-block: [128 rows of W | rows of x | scales of W | scales of x]
   const uint32_t x_off = kWTile, sfa_off = x_off + static_cast<uint32_t>(p.x_box) * kStageBytes, sfb_off = sfa_off + NW * kScaleTile;
 
   if (threadIdx.x == 0) {
@@ -303,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     h->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 1) {
+  if (warp == 1) {   // all of the SM's tensor memory, so column addresses start at 0
     if constexpr (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&h->tmem_base)), "r"(512u) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -357,121 +360,138 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   if constexpr (CG == 1) __syncthreads();
   else cluster_barrier();       // the other CTA's barriers are ready, too
   fence_after();
-  const uint32_t tmem = h->tmem_base;
   const int num_tiles = h->num_tiles;
 
+  // The control warps run their loops with all lanes, so that what feeds a copy or an instruction is the same in all of them and can live
+  // in uniform registers, and elect one (always the same) for the issue.  What a stage costs the issuing thread besides
+  // its instructions, some 300 cycles of waiting and bookkeeping, is why a stage holds two k-blocks, and why nothing votes on a wait
+  // that gave up: a producer's lane then loads nothing more, the issuer runs out on whatever lies there, and the exit waits for
+  // copies in flight.
+  const uint32_t full0 = smem_u32(h->full), empty0 = smem_u32(h->empty);
   if (warp == 0) {
     // ------------------------------------------------------------ producer of W
+    const uint32_t announce = CG == 1 ? full0 : in_first_cta(full0);
     uint32_t s = 0, ph = 0;
     bool ok = true;
-    for (int t = first_tile; ok && t < num_tiles; t += tile_step) {
+    for (int t = first_tile; t < num_tiles; t += tile_step) {
       const Tile tile = tile_of<CG>(lo, start, p, t);
       const int ft = tile.f * CG + static_cast<int>(rank);
       // scales: of a tile whose rows do not exist those of the last that do (its outputs are not stored)
-      int sf = (tile.e * p.k_stages * p.scale_tiles + min(ft, p.scale_tiles - 1)) * NW;
-      for (int ks = 0; ks < p.k_stages; ++ks) {
-        ok = mbar_wait(smem_u32(&h->empty[s]), ph ^ 1, abort_flag, p.status, 101);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+      int sf = (tile.e * p.k_blocks * p.scale_tiles + min(ft, p.scale_tiles - 1)) * NW;
+      for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
         if (elect_one()) {
-          const uint32_t dst = ring + s * p.stage_bytes;
-          uint32_t full = smem_u32(&h->full[s]);
-          if (CG == 2) full = in_first_cta(full);
-          if (rank == 0) mbar_arrive_expect_tx(smem_u32(&h->full[s]), CG * (kWTile + NW * kScaleTile));
-          if (p.gated) load_5d<CG>(dst, &maps.w, ks * kStageBytes, ft * 8, tile.e, full);
-          else load_3d<CG>(dst, &maps.w, ks * kStageBytes, ft * 128, tile.e, full);
-          if constexpr (NW > 0) load_2d<CG>(dst + sfa_off, &maps.w_scales, 0, sf, full);
+          ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 101);
+          if (ok) {
+            uint32_t dst = ring + s * p.stage_bytes;
+            const uint32_t full = announce + 8 * s;
+            const int end = min(kb + kGroup, p.k_blocks);
+            if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (end - kb) * CG * (kWTile + NW * kScaleTile));
+            int scales = sf;
+            for (int k = kb; k < end; ++k, dst += p.block_bytes, scales += p.scale_tiles * NW) {
+              if (p.gated) load_5d<CG>(dst, &maps.w, k * kStageBytes, ft * 8, tile.e, full);
+              else load_3d<CG>(dst, &maps.w, k * kStageBytes, ft * 128, tile.e, full);
+              if constexpr (NW > 0) load_2d<CG>(dst + sfa_off, &maps.w_scales, 0, scales, full);
+            }
+          }
         }
         __syncwarp();
-        sf += p.scale_tiles * NW;
+        sf += kGroup * p.scale_tiles * NW;
         if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
       }
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------ producer of x
     pdl_wait();
+    const uint32_t announce = CG == 1 ? full0 : in_first_cta(full0);
     uint32_t s = 0, ph = 0;
     bool ok = true;
-    for (int t = first_tile; ok && t < num_tiles; t += tile_step) {
+    for (int t = first_tile; t < num_tiles; t += tile_step) {
       const Tile tile = tile_of<CG>(lo, start, p, t);
       const int need = tile.n_mma / CG, row = tile.lo + tile.r0 + static_cast<int>(rank) * need;
       // one large box where most of it is needed, else boxes of 32 rows
       const bool large = 2 * need > p.x_box;
       const int boxes = large ? 1 : (need + kBoxRows - 1) / kBoxRows;
-      const int atoms = NW ? ((tile.r0 & 127) + tile.n_mma + 127) >> 7 : 0;
+      const int atoms = NW ? (tile.n_mma + 127) >> 7 : 0;
       const uint32_t tx = CG * ((large ? p.x_box : boxes * kBoxRows) * kStageBytes + atoms * NW * kScaleTile);
-      int sf = static_cast<int>((expert_scale_row(tile.lo, tile.e) + tile.r0) / 128) * NW;
-      for (int ks = 0; ks < p.k_stages; ++ks) {
-        ok = mbar_wait(smem_u32(&h->empty[s]), ph ^ 1, abort_flag, p.status, 105);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
+      int sf = (expert_scale_tile(tile.lo, tile.e, p.bn) + tile.i * p.sfb_atoms) * NW;
+      for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
         if (elect_one()) {
-          const uint32_t dst = ring + s * p.stage_bytes;
-          uint32_t full = smem_u32(&h->full[s]);
-          if (CG == 2) full = in_first_cta(full);
-          if (rank == 0) mbar_arrive_expect_tx(smem_u32(&h->full[s]), tx);
-          if (large) {
-            load_2d<CG>(dst + x_off, &maps.x, ks * kStageBytes, row, full);
-          } else {
-            for (int b = 0; b < boxes; ++b) load_2d<CG>(dst + x_off + b * kBoxRows * kStageBytes, &maps.x32, ks * kStageBytes, row + b * kBoxRows, full);
+          ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 105);
+          if (ok) {
+            uint32_t dst = ring + s * p.stage_bytes;
+            const uint32_t full = announce + 8 * s;
+            const int end = min(kb + kGroup, p.k_blocks);
+            if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (end - kb) * tx);
+            int scales = sf;
+            for (int k = kb; k < end; ++k, dst += p.block_bytes, scales += p.x_scale_tiles * NW) {
+              if (large) {
+                load_2d<CG>(dst + x_off, &maps.x, k * kStageBytes, row, full);
+              } else {
+                for (int b = 0; b < boxes; ++b) load_2d<CG>(dst + x_off + b * kBoxRows * kStageBytes, &maps.x32, k * kStageBytes, row + b * kBoxRows, full);
+              }
+              if constexpr (NW > 0)
+                for (int a = 0; a < atoms; ++a) load_2d<CG>(dst + sfb_off + a * NW * kScaleTile, &maps.x_scales, 0, scales + a * NW, full);
+            }
           }
-          if constexpr (NW > 0)
-            for (int a = 0; a < atoms; ++a) load_2d<CG>(dst + sfb_off + a * NW * kScaleTile, &maps.x_scales, 0, sf + a * NW, full);
         }
         __syncwarp();
-        sf += p.x_scale_tiles * NW;
+        sf += kGroup * p.x_scale_tiles * NW;
         if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1 && rank == 0) {
     // ------------------------------------------------------------ issuer
-    uint32_t s = 0, ph = 0, slot = 0;
-    bool ok = true;
+    uint32_t s = 0, ph = 0;
     int j = 0;
-    for (int t = first_tile; ok && t < num_tiles; t += tile_step, ++j) {
+    const uint32_t ring_low = (ring >> 4) | kDescLow, stage_low = p.stage_bytes >> 4, block_low = p.block_bytes >> 4;
+    uint32_t low = ring_low;                               // of the stage's first operand
+    for (int t = first_tile; t < num_tiles; t += tile_step, ++j) {
       const Tile tile = tile_of<CG>(lo, start, p, t);
       const uint32_t idesc = p.idesc | (static_cast<uint32_t>(tile.n_mma) >> 3) << 17;
-      const int atoms = NW ? ((tile.r0 & 127) + tile.n_mma + 127) >> 7 : 0;
-      const uint32_t sfb_col = (tile.r0 & 127) >> 5;
-      const int buf = p.acc_bufs == 2 ? (j & 1) : 0;
-      const uint32_t buf_ph = p.acc_bufs == 2 ? (j >> 1) & 1 : j & 1;
-      ok = CG == 1 ? mbar_wait(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102)
-                   : wait_cluster(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
+      const int atoms = NW ? (tile.n_mma + 127) >> 7 : 0;
+      const int buf = j & 1;
+      const uint32_t buf_ph = (j >> 1) & 1;
+      if (CG == 1) mbar_wait(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102);
+      else wait_cluster(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102);
+      __syncwarp();
       fence_after();
-      const uint32_t d = tmem + buf * p.bn;
-      for (int ks = 0; ks < p.k_stages; ++ks) {
-        ok = CG == 1 ? mbar_wait(smem_u32(&h->full[s]), ph, abort_flag, p.status, 103) : wait_cluster(smem_u32(&h->full[s]), ph, abort_flag, p.status, 103);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        fence_after();
+      const uint32_t d = buf * kBufferColumns;
+      // One k-block: its scales into slot `slot` of tensor memory, then four K steps.  The slot was last read by the instructions of
+      // the stage before; copies and products of one thread execute in the order issued.
+      auto k_block = [&](uint32_t at, int slot, bool first) {
+        const uint32_t sfa = p.bn + slot * kBufferColumns, sfb = sfa + NW * 4;
+        if constexpr (NW > 0) {
+          const uint32_t sfa_low = at + (sfa_off >> 4), sfb_low = at + (sfb_off >> 4);
+#pragma unroll
+          for (int w = 0; w < NW; ++w) copy_scales<CG>(sfa + w * 4, sfa_low + w * (kScaleTile >> 4));
+#pragma unroll
+          for (int w = 0; w < NW; ++w) copy_scales<CG>(sfb + w * 8, sfb_low + w * (kScaleTile >> 4));
+          if (atoms > 1) {
+#pragma unroll
+            for (int w = 0; w < NW; ++w) copy_scales<CG>(sfb + w * 8 + 4, sfb_low + (NW + w) * (kScaleTile >> 4));
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int w = KIND == B2VX_FP4_BLOCK32 ? k >> 1 : k;
+          // the first of the word's bytes that this K step uses
+          const uint32_t id = KIND == B2VX_FP4_BLOCK32 ? (k & 1) * 2u : 0u;
+          mma<KIND, CG>(d, at + 2 * k, at + (x_off >> 4) + 2 * k, idesc | (id << 4) | (id << 29), sfa + w * 4, sfb + w * 8, !(first && k == 0));
+        }
+      };
+      for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
+        mbar_wait(full0 + 8 * s, ph, abort_flag, p.status, 103);
         if (elect_one()) {
-          const uint32_t base = ring + s * p.stage_bytes;
-          const uint32_t sfa_t = tmem + p.sf_base + slot * p.sf_cols, sfb_t = sfa_t + NW * 4;
-          if constexpr (NW > 0) {
-            // The slot was last read by instructions two stages ago.  Copies and products of one thread execute in the order issued.
-#pragma unroll
-            for (int w = 0; w < NW; ++w) copy_scales<CG>(sfa_t + w * 4, scale_desc(base + sfa_off + w * kScaleTile));
-            for (int a = 0; a < atoms; ++a)
-#pragma unroll
-              for (int w = 0; w < NW; ++w) copy_scales<CG>(sfb_t + (w * p.sfb_atoms + a) * 4, scale_desc(base + sfb_off + (a * NW + w) * kScaleTile));
-          }
-          const uint64_t da = operand_desc(base), db = operand_desc(base + x_off);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int w = KIND == B2VX_FP4_BLOCK32 ? k >> 1 : k;
-            // the first of the word's bytes that this K step uses
-            const uint32_t id = KIND == B2VX_FP4_BLOCK32 ? (k & 1) * 2u : 0u;
-            mma<KIND, CG>(d, da + 2 * k, db + 2 * k, idesc | (id << 4) | (id << 29), sfa_t + w * 4, sfb_t + w * p.sfb_atoms * 4 + sfb_col, (ks | k) != 0);
-          }
-          commit<CG>(smem_u32(&h->empty[s]));
+          fence_after();
+          k_block(low, 0, kb == 0);
+          if (kb + 1 < p.k_blocks) k_block(low + block_low, 1, false);
+          commit<CG>(empty0 + 8 * s);
         }
         __syncwarp();
-        slot ^= 1;
-        if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
+        low += stage_low;
+        if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; low = ring_low; }
       }
-      if (ok && elect_one()) commit<CG>(smem_u32(&h->acc_full[buf]));
+      if (elect_one()) commit<CG>(smem_u32(&h->acc_full[buf]));
       __syncwarp();
     }
   } else if (warp >= kFirstEpilogueWarp) {
@@ -481,16 +501,16 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     T* y = static_cast<T*>(p.y);
     const int width = p.gated ? 64 : 128;                 // features of a CTA's tile
     const int warp_width = p.gated ? 16 : 32;             // of a warp
-    const uint32_t buffers = staging + set * 2 * kSlabBytes;
-    int j = 0, slab = 0;
+    const uint32_t out = staging + set * kSlabBytes;
+    int j = 0;
     for (int t = first_tile; t < num_tiles; t += tile_step, ++j) {
       const Tile tile = tile_of<CG>(lo, start, p, t);
-      const int buf = p.acc_bufs == 2 ? (j & 1) : 0;
-      const uint32_t buf_ph = p.acc_bufs == 2 ? (j >> 1) & 1 : j & 1;
+      const int buf = j & 1;
+      const uint32_t buf_ph = (j >> 1) & 1;
       float alpha = 1.0f;
       if (p.x_scale) alpha = __ldg(p.x_scale);
       if (p.w_scale) alpha *= __ldg(p.w_scale + tile.e);
-      const uint32_t taddr = tmem + buf * p.bn + lanes;
+      const uint32_t taddr = buf * kBufferColumns + lanes;
       const int row0 = tile.lo + tile.r0;
       const int f0 = (tile.f * CG + static_cast<int>(rank)) * width;       // first feature of the CTA's tile
       // Bias of the TMEM lanes 8 i + lane / 4 of the warp: features, or alternating eight gate and eight up features.
@@ -535,40 +555,42 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
             }
           __syncwarp();
         } else {
-          // 16-bit numbers, transposed into the slab buffer: boxes of 64 features, [row][128 bytes], 16-byte pieces exchanged by the
+          // 16-bit numbers, transposed into the set's slab buffer: boxes of 64 features, [row][128 bytes], 16-byte pieces exchanged by the
           // row's number as the store's 128-byte swizzle has them (neither side then meets bank conflicts).
-          const uint32_t out = buffers + (slab & 1) * kSlabBytes;
-          ++slab;
-          const uint32_t row_at = out + (lane & 7) * 128;
+          uint32_t m[4][4];
+          uint32_t at, step;                               // where matrices m[0] go, and from one m to the next
           if (p.gated) {
-            // two matrices (features 8 i) of two column groups
+            // two matrices (features 8 i) of two column groups at a time
             const uint32_t piece = quarter * 2 + ((lane >> 3) & 1);
-            const uint32_t at = row_at + ((piece ^ (lane & 7)) << 4) + (lane >> 4) * 1024;
+            at = out + (lane & 7) * 128 + ((piece ^ (lane & 7)) << 4) + (lane >> 4) * 1024;
+            step = 2048;
 #pragma unroll
-            for (int g = 0; g < 4; g += 2) {
-              uint32_t m[4];
+            for (int g = 0; g < 2; ++g)
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                const int i = q & 1, c = g + (q >> 1);
-                m[q] = pack2<T>(gate(value(2 * i, c, 0), value(2 * i + 1, c, 0)), gate(value(2 * i, c, 1), value(2 * i + 1, c, 1)));
+                const int i = q & 1, c = 2 * g + (q >> 1);
+                m[g][q] = pack2<T>(gate(value(2 * i, c, 0), value(2 * i + 1, c, 0)), gate(value(2 * i, c, 1), value(2 * i + 1, c, 1)));
               }
-              store_transposed(at + g * 1024, m[0], m[1], m[2], m[3]);
-            }
           } else {
             const uint32_t piece = (quarter & 1) * 4 + (lane >> 3);
-            const uint32_t at = row_at + (quarter >> 1) * 4096 + ((piece ^ (lane & 7)) << 4);
+            at = out + (quarter >> 1) * 4096 + (lane & 7) * 128 + ((piece ^ (lane & 7)) << 4);
+            step = 1024;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              uint32_t m[4];
+            for (int g = 0; g < 4; ++g)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) m[i] = pack2<T>(value(i, g, 0), value(i, g, 1));
-              store_transposed(at + g * 1024, m[0], m[1], m[2], m[3]);
-            }
+              for (int i = 0; i < 4; ++i) m[g][i] = pack2<T>(value(i, g, 0), value(i, g, 1));
+          }
+          // the buffer is free once the store of the last slab has read it (or every thread has, before it came here)
+          if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          set_barrier(set);
+          store_transposed(at, m[0][0], m[0][1], m[0][2], m[0][3]);
+          store_transposed(at + step, m[1][0], m[1][1], m[1][2], m[1][3]);
+          if (!p.gated) {
+            store_transposed(at + 2 * step, m[2][0], m[2][1], m[2][2], m[2][3]);
+            store_transposed(at + 3 * step, m[3][0], m[3][1], m[3][2], m[3][3]);
           }
           const bool whole = p.y_vec && rows == kSlabRows;
           if (whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          // the store from the other buffer has been read out: after the barrier that buffer may be written
-          if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           set_barrier(set);
           if (whole) {
             if (quarter == 0 && lane == 0) {
@@ -611,10 +633,15 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   fence_before();
   if constexpr (CG == 1) __syncthreads();
   else cluster_barrier();     // the other CTA's instructions and arrivals reach into this one's memory
+  if (*abort_flag) {          // copies in flight land within microseconds
+    const long long began = clock64();
+    while (clock64() - began < 200000) {}
+    __syncwarp();
+  }
   if (warp == 1) {
     fence_after();
-    if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
-    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(h->tmem_base), "r"(512u) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(h->tmem_base), "r"(512u) : "memory");
   }
 }
 
@@ -705,26 +732,23 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   p.experts = a.experts;
   p.gated = a.gated;
   const uint64_t kbytes = fp4 ? static_cast<uint64_t>(a.k) / 2 : static_cast<uint64_t>(a.k) * 2;
-  p.k_stages = static_cast<int>((kbytes + kStageBytes - 1) / kStageBytes);
+  p.k_blocks = static_cast<int>((kbytes + kStageBytes - 1) / kStageBytes);
   p.scale_tiles = static_cast<int>(weight_tiles(a.n, a.gated));
 
-  // Two CTAs to a tile where groups have more rows than a tile of one has; 192 rows leave room for two accumulators and two slots of scales.
   const int groups = static_cast<int>(std::min<long long>(a.experts, a.rows));
-  const long long mean = (a.rows + groups - 1) / groups;
-  const int cg = mean <= 64 ? 1 : 2;
-  p.bn = mean <= 64 ? 64 : (mean <= 128 ? 128 : 192);
+  p.bn = tile_rows(a.rows, a.experts, a.format);
+  const int cg = p.bn <= 64 ? 1 : 2;
   p.x_box = p.bn / cg;
   p.feature_tiles = (p.scale_tiles + cg - 1) / cg;
-  p.sfb_atoms = fp4 ? (p.bn + 127) / 128 + (p.bn % 128 ? 0 : 1) : 0;   // tiles start on multiples of 64 rows
-  p.sf_cols = (1 + p.sfb_atoms) * nw * 4;
-  p.acc_bufs = 2;
-  p.sf_base = 2 * p.bn;
-  p.stage_bytes = (128 + p.x_box) * kStageBytes + (1 + p.sfb_atoms) * nw * kScaleTile;
-  p.stage_bytes = (p.stage_bytes + 1023u) & ~1023u;
+  p.sfb_atoms = fp4 ? (p.bn + 127) / 128 : 0;
+  p.block_bytes = (128 + p.x_box) * kStageBytes + (1 + p.sfb_atoms) * nw * kScaleTile;
+  p.block_bytes = (p.block_bytes + 1023u) & ~1023u;
   const int elem = a.y_dtype == B2VX_DT_FLOAT32 ? 4 : 2;
   p.y_vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride * elem % 16 == 0;
   const int behind = kStagingBytes + static_cast<int>(sizeof(Header)) + 8 * (a.experts + 1) + 1024;   // and the ring's alignment
-  p.stages = std::min(kMaxStages, static_cast<int>((kSmemBudget - behind) / p.stage_bytes));
+  const int room = static_cast<int>((kSmemBudget - behind) / p.block_bytes);      // k-blocks that fit
+  p.stages = std::min(kMaxStages, room / kGroup);
+  p.stage_bytes = kGroup * p.block_bytes;
   const size_t smem = std::max<size_t>(kMinDynSmem, p.stages * p.stage_bytes + behind);
   const uint32_t m = 8u * cg << 24;
   if (fp4) {
@@ -742,12 +766,12 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   p.y_stride = a.y_stride;
   p.y_dtype = a.y_dtype;
   p.status = a.status;
-  p.x_scale_tiles = fp4 ? static_cast<int>(expert_scale_rows(a.rows, a.experts) / 128) : 0;
+  p.x_scale_tiles = fp4 ? static_cast<int>(expert_scale_tiles(a.rows, a.experts, p.bn)) : 0;
   p.after_operand = a.after_operand;
 
   Maps maps = {};
   const uint64_t rows = static_cast<uint64_t>(a.rows), x_pitch = static_cast<uint64_t>(a.x_pitch);
-  const uint64_t w_tiles = static_cast<uint64_t>(a.experts) * p.k_stages * p.scale_tiles * nw, x_tiles = static_cast<uint64_t>(p.k_stages) * p.x_scale_tiles * nw;
+  const uint64_t w_tiles = static_cast<uint64_t>(a.experts) * p.k_blocks * p.scale_tiles * nw, x_tiles = static_cast<uint64_t>(p.k_blocks) * p.x_scale_tiles * nw;
   if (w_tiles >= 1ull << 31 || x_tiles >= 1ull << 31) {
     *why = "the product has too many scale tiles";
     return cudaErrorInvalidValue;

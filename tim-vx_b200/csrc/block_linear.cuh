@@ -30,11 +30,22 @@ __host__ __device__ inline long long weight_tiles(long long n, int gated) { retu
 __host__ __device__ inline size_t packed_scale_bytes(long long matrices, long long n, int gated, long long k, int format) {
   return static_cast<size_t>(matrices) * weight_tiles(n, gated) * scale_words(k, format) * kScaleTile;
 }
-// Rows of the packed scales of an operand whose rows belong to `experts` groups: each group starts on a tile of its own.  Group e,
-// whose first row is lo, starts at scale row expert_scale_row(lo, e); since roundup(a) + roundup(b) <= roundup(a + b) + 128, groups do
-// not overlap and the space ends at expert_scale_rows.
-__host__ __device__ inline long long expert_scale_row(long long lo, long long e) { return (lo + 127) / 128 * 128 + 128 * e; }
-__host__ __device__ inline long long expert_scale_rows(long long rows, long long experts) { return (rows + 127) / 128 * 128 + 128 * experts; }
+// Rows of x in a tile of a product.  Up to 64 rows to a group: narrow tiles of one CTA.  More: tiles of two CTAs, as wide as leaves
+// tensor memory for two accumulators and two slots of scales (twice as many of block16).
+inline int tile_rows(long long rows, int experts, int format) {
+  const long long groups = rows < experts ? rows : experts, mean = groups ? (rows + groups - 1) / groups : 0;
+  return mean <= 64 ? 64 : (mean <= 128 ? 128 : (format == B2VX_FP4_BLOCK16 ? 192 : 224));
+}
+// Rows of each tile of a group: its rows in even shares.
+__host__ __device__ inline int rows_of_tile(int count, int bn) {
+  const int tiles = (count + bn - 1) / bn;
+  return tiles ? ((count + tiles - 1) / tiles + 31) / 32 * 32 : 32;
+}
+// Packed scales of x: every tile's rows start on a scale tile of their own (an instruction takes its scales from an even column of tensor
+// memory on, so 32-row steps inside a scale tile would not do).  Group e, whose first row is lo, starts at scale tile
+// expert_scale_tile(lo, e); since floor(a + b) >= floor(a) + floor(b), the tiles of group e end where group e + 1 may start.
+__host__ __device__ inline int expert_scale_tile(int lo, int e, int bn) { return (lo / bn + e) * ((bn + 127) / 128); }
+__host__ __device__ inline long long expert_scale_tiles(long long rows, long long experts, int bn) { return (rows / bn + experts) * ((bn + 127) / 128); }
 
 struct QuantizeArgs {
   const void* x;
@@ -48,10 +59,11 @@ struct QuantizeArgs {
   uint8_t* codes;
   long long codes_pitch;       // bytes
   uint8_t* scales;
-  long long scales_pitch;      // bytes; 0: packed
+  long long scales_pitch;      // bytes; 0: packed, for a product
   const int32_t* offsets;      // packed: the groups, or null for one group of all rows
   int experts;
-  long long scale_tiles;       // packed: 128-row tiles of the scale rows
+  int bn;                      // packed: rows of the product's tiles
+  int scale_tiles;             // packed: expert_scale_tiles
 };
 cudaError_t launch_fp4_quantize(const QuantizeArgs& a, cudaStream_t s);
 cudaError_t launch_fp4_dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,

@@ -86,7 +86,8 @@ Workspace workspace_of(const b2vx_linear_desc& d) {
   if (d.w_format) {
     w.codes_pitch = d.k / 2;
     w.codes = round256(d.rows * w.codes_pitch);
-    w.scales = round256(packed_scale_bytes(1, expert_scale_rows(d.rows, d.experts ? d.experts : 1), 0, d.k, d.w_format));
+    const int experts = d.experts ? static_cast<int>(d.experts) : 1;
+    w.scales = round256(static_cast<size_t>(expert_scale_tiles(d.rows, experts, tile_rows(d.rows, experts, d.w_format))) * scale_words(d.k, d.w_format) * kScaleTile);
   } else {
     w.codes_pitch = d.k * 2;
     w.codes = round256(d.rows * w.codes_pitch);
@@ -120,19 +121,17 @@ extern "C" b2vx_status b2vx_fp4_quantize_noalloc(const b2vx_fp4_quantize_desc* d
                                                  void* codes, void* scales, void* cuda_stream, char* err, size_t err_len) {
   B2VX_NEED(d, "null descriptor");
   B2VX_NEED(is_fp4(d->format), "format must be B2VX_FP4_BLOCK32 or B2VX_FP4_BLOCK16");
-  B2VX_NEED(d->scales_layout == B2VX_SCALES_ROWS || d->scales_layout == B2VX_SCALES_PACKED, "unknown layout of scales");
   B2VX_NEED(is_float(d->x_dtype), "x must be float32, float16 or bfloat16");
   B2VX_NEED(d->rows <= kMaxExtent && d->k <= kMaxExtent && d->x_rows <= kMaxExtent, "an extent is out of range");
   B2VX_NEED(d->x_stride >= d->k && d->x_stride <= kMaxStride, "x_stride is smaller than a row or out of range");
   const uint64_t block = fp4_block(d->format), k32 = (d->k + 31) / 32 * 32;
   B2VX_NEED(d->codes_pitch % 4 == 0 && d->codes_pitch >= k32 / 2 && d->codes_pitch <= kMaxStride, "codes_pitch must be a multiple of 4 that holds k rounded up to 32");
-  const bool rows_layout = d->scales_layout == B2VX_SCALES_ROWS;
-  B2VX_NEED(!rows_layout || (d->scales_pitch >= (d->k + block - 1) / block && d->scales_pitch <= kMaxStride), "scales_pitch is smaller than a row of scales");
+  B2VX_NEED(d->scales_pitch >= (d->k + block - 1) / block && d->scales_pitch <= kMaxStride, "scales_pitch is smaller than a row of scales");
   B2VX_NEED((tensor_scale != nullptr) == (d->format == B2VX_FP4_BLOCK16), "a tensor scale belongs to B2VX_FP4_BLOCK16 and only to it");
   B2VX_NEED(row_index || d->rows <= d->x_rows, "more rows than x has, and no row_index");
   if (d->rows == 0 || d->k == 0) return B2VX_OK;
   B2VX_NEED(codes && scales && (x || d->x_rows == 0), "null argument");
-  B2VX_NEED(aligned(x, size_of(d->x_dtype)) && aligned(codes, 4) && (rows_layout || aligned(scales, 16)), "a pointer is not aligned");
+  B2VX_NEED(aligned(x, size_of(d->x_dtype)) && aligned(codes, 4), "a pointer is not aligned");
   PerDevice* pd;
   b2vx_status st = device(&pd, err, err_len);
   if (st != B2VX_OK) return st;
@@ -142,8 +141,7 @@ extern "C" b2vx_status b2vx_fp4_quantize_noalloc(const b2vx_fp4_quantize_desc* d
   a.rows = static_cast<long long>(d->rows); a.k = static_cast<long long>(d->k);
   a.row_index = row_index; a.tensor_scale = tensor_scale; a.format = d->format;
   a.codes = static_cast<uint8_t*>(codes); a.codes_pitch = static_cast<long long>(d->codes_pitch);
-  a.scales = static_cast<uint8_t*>(scales); a.scales_pitch = rows_layout ? static_cast<long long>(d->scales_pitch) : 0;
-  a.scale_tiles = (a.rows + 127) / 128;
+  a.scales = static_cast<uint8_t*>(scales); a.scales_pitch = static_cast<long long>(d->scales_pitch);
   return launched(launch_fp4_quantize(a, static_cast<cudaStream_t>(cuda_stream)), err, err_len);
 }
 
@@ -242,7 +240,8 @@ extern "C" b2vx_status b2vx_linear_noalloc(const b2vx_linear_desc* d, const b2vx
     q.codes = codes; q.codes_pitch = static_cast<long long>(ws.codes_pitch);
     q.scales = codes + ws.codes; q.scales_pitch = 0;
     q.offsets = a->offsets; q.experts = l.experts;
-    q.scale_tiles = expert_scale_rows(l.rows, l.experts) / 128;
+    q.bn = tile_rows(l.rows, l.experts, l.format);
+    q.scale_tiles = static_cast<int>(expert_scale_tiles(l.rows, l.experts, q.bn));
     e = launch_fp4_quantize(q, s);
     l.x = codes; l.x_pitch = static_cast<long long>(ws.codes_pitch); l.x_scales = q.scales;
   } else if (direct) {

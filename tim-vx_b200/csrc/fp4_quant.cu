@@ -71,13 +71,18 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArg
     const long long k_here = there ? a.k : 0;
     uint8_t* tile = nullptr;      // PACKED: where the row's words of the first scale tile lie; null: the row belongs to no group
     if (PACKED) {
-      long long at = row;
+      int e = 0, lo = 0, count = static_cast<int>(a.rows);
       if (a.offsets) {
-        const int e = group_of(a.offsets, a.experts, row, lane);
-        const long long lo = e < a.experts ? a.offsets[e] : -1;
-        at = lo >= 0 && lo <= row ? expert_scale_row(lo, e) + row - lo : -1;
+        e = group_of(a.offsets, a.experts, row, lane);
+        lo = e < a.experts ? a.offsets[e] : -1;
+        count = e < a.experts ? min(a.offsets[e + 1], static_cast<int>(a.rows)) - lo : 0;
       }
-      if (at >= 0) tile = a.scales + at / 128 * (scale_words_per_stage(FORMAT) * kScaleTile) + (at % 32) * 16 + (at % 128 / 32) * 4;
+      const int in = static_cast<int>(row) - lo;            // row inside its group
+      if (lo >= 0 && in >= 0 && in < count) {
+        const int per = rows_of_tile(count, a.bn), i = in / per, r = in - i * per;
+        const int at = expert_scale_tile(lo, e, a.bn) + i * ((a.bn + 127) / 128) + r / 128;
+        tile = a.scales + static_cast<long long>(at) * (scale_words_per_stage(FORMAT) * kScaleTile) + (r % 32) * 16 + (r % 128 / 32) * 4;
+      }
     }
     for (int chunk = part; chunk < chunks; chunk += split) {
       const long long c = static_cast<long long>(chunk) * kChunk + lane * 8;
@@ -91,7 +96,7 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArg
         uint32_t word = byte | __shfl_down_sync(0xffffffffu, byte, LANES) << 8;
         word |= __shfl_down_sync(0xffffffffu, word, 2 * LANES) << 16;
         if (lane % (4 * LANES) == 0 && tile)
-          *reinterpret_cast<uint32_t*>(tile + (chunk * a.scale_tiles * scale_words_per_stage(FORMAT) + lane / (4 * LANES)) * kScaleTile) = word;
+          *reinterpret_cast<uint32_t*>(tile + (static_cast<long long>(chunk) * a.scale_tiles * scale_words_per_stage(FORMAT) + lane / (4 * LANES)) * kScaleTile) = word;
       } else if (lane % LANES == 0 && c / B < blocks) {
         a.scales[row * a.scales_pitch + c / B] = static_cast<uint8_t>(byte);
       }
