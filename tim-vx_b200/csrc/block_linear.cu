@@ -14,7 +14,7 @@
 //                          Two warps and few, large copies because a wait, an announcement and a copy take one thread about 340 cycles.
 //   warp 1      issuer     copies a k-block's scales into tensor memory (tcgen05.cp, two slots in turn) and issues its four K steps
 //   warps 4-11  epilogue   two sets of four warps take slabs of 32 rows of the tile in turn: out of tensor memory, scale and bias,
-//                          activation, rounding, transposition into a buffer in shared memory, one TMA store
+//                          activation, rounding, transposition through a buffer in shared memory, 16-byte stores
 //
 // CG = 2 (many rows): two CTAs of a cluster share a tile of 256 rows of W; each holds its 128 rows of W and half of the rows of x, and
 // the first one's issuer issues for both.  An instruction then is twice the work for the same issue, and rows of x are fetched
@@ -71,12 +71,12 @@ struct LinearParams {
   void* y;
   long long y_stride;
   int y_dtype;
-  int y_vec;                  // rows of y start on 16 bytes: whole slabs leave by TMA
+  int y_vec;                  // rows of y start on 16 bytes
   int* status;
 };
 
 struct Maps {
-  CUtensorMap w, x, x32, w_scales, x_scales, y;
+  CUtensorMap w, x, x32, w_scales, x_scales;
 };
 
 struct Header {
@@ -165,10 +165,6 @@ __device__ __forceinline__ void load_5d(uint32_t dst, const CUtensorMap* map, in
     asm volatile("cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %6, %6, %3, %4}], [%5];"
                  ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c3), "r"(c4), "r"(bar), "r"(0) : "memory");
   }
-}
-__device__ __forceinline__ void store_2d(const CUtensorMap* map, int c0, int c1, uint32_t src) {
-  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];"
-               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(src) : "memory");
 }
 // Descriptors of shared-memory operands as their low halves, start address in 16-byte units (addresses stay below 256 KB, so
 // additions do not leave that field), and constant high halves.
@@ -555,8 +551,9 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
             }
           __syncwarp();
         } else {
-          // 16-bit numbers, transposed into the set's slab buffer: boxes of 64 features, [row][128 bytes], 16-byte pieces exchanged by the
-          // row's number as the store's 128-byte swizzle has them (neither side then meets bank conflicts).
+          // 16-bit numbers, transposed into the set's slab buffer: [64 features][row][128 bytes], 16-byte pieces exchanged by the row's number
+          // (neither side then meets bank conflicts), and stored by threads.  A TMA store of the slab waits behind the loads of the next
+          // tiles that are already queued: with 1408 columns of K a slab then took 2500 cycles.
           uint32_t m[4][4];
           uint32_t at, step;                               // where matrices m[0] go, and from one m to the next
           if (p.gated) {
@@ -580,39 +577,36 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
 #pragma unroll
               for (int i = 0; i < 4; ++i) m[g][i] = pack2<T>(value(i, g, 0), value(i, g, 1));
           }
-          // the buffer is free once the store of the last slab has read it (or every thread has, before it came here)
-          if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          set_barrier(set);
+          set_barrier(set);                                // every thread has read the last slab
           store_transposed(at, m[0][0], m[0][1], m[0][2], m[0][3]);
           store_transposed(at + step, m[1][0], m[1][1], m[1][2], m[1][3]);
           if (!p.gated) {
             store_transposed(at + 2 * step, m[2][0], m[2][1], m[2][2], m[2][3]);
             store_transposed(at + 3 * step, m[3][0], m[3][1], m[3][2], m[3][3]);
           }
-          const bool whole = p.y_vec && rows == kSlabRows;
-          if (whole) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           set_barrier(set);
-          if (whole) {
-            if (quarter == 0 && lane == 0) {
-              if (f0 < p.n) store_2d(&maps.y, f0, row0 + c0, out);
-              if (!p.gated && f0 + 64 < p.n) store_2d(&maps.y, f0 + 64, row0 + c0, out + 4096);
-              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            }
-          } else {
-            const int pieces = p.gated ? 8 : 16;
-            for (int i = quarter * 32 + lane; i < rows * pieces; i += 128) {
-              const int r = p.gated ? i >> 3 : i >> 4, q = i & (pieces - 1), f = f0 + q * 8;
-              if (f >= p.n) continue;
-              uint32_t w[4];
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                           : "r"(out + (q >> 3) * 4096 + r * 128 + (((q & 7) ^ (r & 7)) << 4)));
-              T* to = y + (row0 + c0 + r) * p.y_stride + f;
-              if (p.y_vec && f + 8 <= p.n) {
-                *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+          // 16 bytes a thread and step: of 128 (gated: 64) features a row, eight (sixteen) rows at a time
+          const int thread = quarter * 32 + lane;
+          const int q = p.gated ? thread & 7 : thread & 15, r0 = p.gated ? thread >> 3 : thread >> 4, r_step = p.gated ? 16 : 8, f = f0 + 8 * q;
+          T* to = y + (row0 + c0 + r0) * p.y_stride + f;
+          const uint32_t from = out + (q >> 3) * 4096 + r0 * 128 + (((q & 7) ^ (r0 & 7)) << 4);
+          if (f < p.n) {
+            uint32_t w[4][4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              if (u < 2 || !p.gated)
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[u][0]), "=r"(w[u][1]), "=r"(w[u][2]), "=r"(w[u][3]) : "r"(from + u * r_step * 128));
+            const bool vec = p.y_vec && f + 8 <= p.n;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              if ((u >= 2 && p.gated) || r0 + u * r_step >= rows) continue;
+              T* dst = to + u * r_step * p.y_stride;
+              if (vec) {
+                *reinterpret_cast<uint4*>(dst) = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
               } else {
 #pragma unroll
                 for (int k = 0; k < 8; ++k)
-                  if (f + k < p.n) reinterpret_cast<uint16_t*>(to)[k] = static_cast<uint16_t>(w[k >> 1] >> (16 * (k & 1)));
+                  if (f + k < p.n) reinterpret_cast<uint16_t*>(dst)[k] = static_cast<uint16_t>(w[u][k >> 1] >> (16 * (k & 1)));
               }
             }
           }
@@ -625,7 +619,6 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
         else arrive_remote(in_first_cta(smem_u32(&h->acc_empty[buf])));
       }
     }
-    if (quarter == 0 && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
 
   // ---------------------------------------------------------------- common exit
@@ -672,12 +665,6 @@ bool encode_scales(CUtensorMap* map, const void* base, uint64_t tiles, uint32_t 
   const cuuint32_t box[2] = {kScaleTile / 4, box_tiles};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
-bool encode_y(CUtensorMap* map, void* base, uint64_t n, uint64_t rows, uint64_t stride) {
-  const cuuint64_t dims[2] = {n, rows}, strides[1] = {stride * 2};
-  const cuuint32_t box[2] = {64, kSlabRows};
-  return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
-}
-
 template <int KIND, int CG, typename T>
 cudaError_t start(const Maps& maps, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
   auto* kernel = block_linear_kernel<KIND, CG, T>;
@@ -779,7 +766,6 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   bool ok = a.gated ? encode_gated(&maps.w, a.w, kbytes, a.n, a.experts) : encode_rows(&maps.w, a.w, kbytes, kbytes, a.n, a.experts, 3, 128);
   ok = ok && encode_rows(&maps.x, a.x, kbytes, x_pitch, rows, 1, 2, p.x_box) && encode_rows(&maps.x32, a.x, kbytes, x_pitch, rows, 1, 2, kBoxRows);
   if (fp4) ok = ok && encode_scales(&maps.w_scales, a.w_scales, w_tiles, nw) && encode_scales(&maps.x_scales, a.x_scales, x_tiles, nw);
-  if (p.y_vec && elem == 2) ok = ok && encode_y(&maps.y, a.y, a.n, rows, a.y_stride);
   if (!ok) {
     *why = "tensor map refused";
     return cudaErrorInvalidValue;
