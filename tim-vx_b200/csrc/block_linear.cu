@@ -79,14 +79,17 @@ struct Maps {
   CUtensorMap w, x, x32, w_scales, x_scales;
 };
 
-struct Header {
+struct alignas(16) Header {
   unsigned long long full[kMaxStages], empty[kMaxStages];
   unsigned long long acc_full[2], acc_empty[2];
   uint32_t tmem_base;
   int abort_flag;
   int num_tiles;
 };
-// Behind the header: the groups' first rows lo[experts + 1] (group e ends where e + 1 begins) and first tiles start[experts + 1].
+// Behind the header, for each group and one more: first row, first tile, tiles along its rows, rows of each of them.
+struct Group {
+  int lo, start, tiles, per;
+};
 
 // ---- PTX wrappers (the rest: tma.cuh) ----------------------------------------
 
@@ -106,8 +109,10 @@ __device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// What it tells of is tensor memory that has been read (tcgen05 fences order that), so it need not order this thread's stores to global
+// memory: with release at cluster scope it waited for the rows of y to arrive, 1.5 us a tile.
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 // A wait for arrivals that may come from the other CTA.
 __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
@@ -238,25 +243,32 @@ __device__ __forceinline__ bool set_all(int set, bool ok) {
 struct Tile {
   int e, lo, i, r0, rows, n_mma, f;
 };
+// `from`: a group at or before the tile's (that of an earlier tile of this CTA).  Kept short, in particular of divisions: between two
+// tiles every role makes this computation.
 template <int CG>
-__device__ __forceinline__ Tile tile_of(const int* lo, const int* start, const LinearParams& p, int t) {
-  int a = 0, b = p.experts;           // the last group whose first tile is not behind t
+__device__ __forceinline__ Tile tile_of(const Group* groups, const LinearParams& p, int t, int from) {
+  int a = from, b = p.experts;           // the last group whose first tile is not behind t
   while (b - a > 1) {
     const int mid = (a + b) >> 1;
-    if (start[mid] <= t) a = mid; else b = mid;
+    if (groups[mid].start <= t) a = mid; else b = mid;
   }
-  const int count = lo[a + 1] - lo[a], row_tiles = (count + p.bn - 1) / p.bn;
-  const int i = t - start[a];
-  const int per = rows_of_tile(count, p.bn);
+  const Group g = groups[a];
+  const int in = t - g.start;
+  int f = in;
+  if (g.tiles > 1) {                     // in / g.tiles: the quotient of floats is off by one at most
+    f = static_cast<int>(__fdividef(static_cast<float>(in), static_cast<float>(g.tiles)));
+    const int r = in - f * g.tiles;
+    f += r < 0 ? -1 : (r >= g.tiles ? 1 : 0);
+  }
   constexpr int step = 16 * CG;
   Tile r;
   r.e = a;
-  r.f = i / row_tiles;
-  r.i = i - r.f * row_tiles;
-  r.r0 = r.i * per;
-  r.rows = max(0, min(per, count - r.r0));
+  r.f = f;
+  r.i = in - f * g.tiles;
+  r.r0 = r.i * g.per;
+  r.rows = max(0, min(g.per, groups[a + 1].lo - g.lo - r.r0));
   r.n_mma = max(step, (r.rows + step - 1) / step * step);
-  r.lo = lo[a];
+  r.lo = g.lo;
   return r;
 }
 
@@ -281,8 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   const uint32_t ring = (raw + 1023u) & ~1023u;
   const uint32_t staging = ring + p.stages * p.stage_bytes;
   Header* h = reinterpret_cast<Header*>(smem_raw + (staging - raw) + kStagingBytes);
-  int* lo = reinterpret_cast<int*>(h + 1);
-  int* start = lo + p.experts + 1;
+  Group* groups = reinterpret_cast<Group*>(h + 1);
   volatile int* abort_flag = &h->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 1 ? 0u : cluster_rank();
@@ -334,19 +345,25 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
         if (lane >= d) v = max(v, up);
       }
       v = max(v, high);
-      // this chunk's last value is the next chunk's first bound; tiles of group e - 1, which ends at v
+      // this chunk's last value is the next chunk's first bound; group e - 1 ends at v
       const int prev = __shfl_up_sync(0xffffffffu, v, 1);
       const int from = lane ? prev : high;
       high = __shfl_sync(0xffffffffu, v, 31);
-      int sum = e >= 1 && e <= p.experts ? (v - from + p.bn - 1) / p.bn * p.feature_tiles : 0;
+      const bool ends = e >= 1 && e <= p.experts;
+      const int row_tiles = ends ? (v - from + p.bn - 1) / p.bn : 0;
+      int sum = row_tiles * p.feature_tiles;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const int up = __shfl_up_sync(0xffffffffu, sum, d);
         if (lane >= d) sum += up;
       }
       if (e <= p.experts) {
-        lo[e] = v;
-        start[e] = total + sum;
+        groups[e].lo = v;
+        groups[e].start = total + sum;
+      }
+      if (ends) {
+        groups[e - 1].tiles = row_tiles;
+        groups[e - 1].per = rows_of_tile(v - from, p.bn);
       }
       total += __shfl_sync(0xffffffffu, sum, 31);
     }
@@ -369,8 +386,9 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     const uint32_t announce = CG == 1 ? full0 : in_first_cta(full0);
     uint32_t s = 0, ph = 0;
     bool ok = true;
-    for (int t = first_tile; t < num_tiles; t += tile_step) {
-      const Tile tile = tile_of<CG>(lo, start, p, t);
+    for (int t = first_tile, e = 0; t < num_tiles; t += tile_step) {
+      const Tile tile = tile_of<CG>(groups, p, t, e);
+      e = tile.e;
       const int ft = tile.f * CG + static_cast<int>(rank);
       // scales: of a tile whose rows do not exist those of the last that do (its outputs are not stored)
       int sf = (tile.e * p.k_blocks * p.scale_tiles + min(ft, p.scale_tiles - 1)) * NW;
@@ -401,8 +419,9 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     const uint32_t announce = CG == 1 ? full0 : in_first_cta(full0);
     uint32_t s = 0, ph = 0;
     bool ok = true;
-    for (int t = first_tile; t < num_tiles; t += tile_step) {
-      const Tile tile = tile_of<CG>(lo, start, p, t);
+    for (int t = first_tile, e = 0; t < num_tiles; t += tile_step) {
+      const Tile tile = tile_of<CG>(groups, p, t, e);
+      e = tile.e;
       const int need = tile.n_mma / CG, row = tile.lo + tile.r0 + static_cast<int>(rank) * need;
       // one large box where most of it is needed, else boxes of 32 rows
       const bool large = 2 * need > p.x_box;
@@ -441,8 +460,9 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     int j = 0;
     const uint32_t ring_low = (ring >> 4) | kDescLow, stage_low = p.stage_bytes >> 4, block_low = p.block_bytes >> 4;
     uint32_t low = ring_low;                               // of the stage's first operand
+    Tile tile = {};
+    if (first_tile < num_tiles) tile = tile_of<CG>(groups, p, first_tile, 0);
     for (int t = first_tile; t < num_tiles; t += tile_step, ++j) {
-      const Tile tile = tile_of<CG>(lo, start, p, t);
       const uint32_t idesc = p.idesc | (static_cast<uint32_t>(tile.n_mma) >> 3) << 17;
       const int atoms = NW ? (tile.n_mma + 127) >> 7 : 0;
       const int buf = j & 1;
@@ -476,6 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
         }
       };
       for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
+        // the next tile is worked out while the instructions of this one's last stages run
+        if (kb + kGroup >= p.k_blocks && t + tile_step < num_tiles) tile = tile_of<CG>(groups, p, t + tile_step, tile.e);
         mbar_wait(full0 + 8 * s, ph, abort_flag, p.status, 103);
         if (elect_one()) {
           fence_after();
@@ -498,28 +520,56 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     const int width = p.gated ? 64 : 128;                 // features of a CTA's tile
     const int warp_width = p.gated ? 16 : 32;             // of a warp
     const uint32_t out = staging + set * kSlabBytes;
+    const float x_scale = p.x_scale ? __ldg(p.x_scale) : 1.0f;
+    // What a tile needs of global memory is asked for while the tile before it is worked on.  Bias of the TMEM lanes 8 i + lane / 4 of
+    // the warp: features, or alternating eight gate and eight up features.
+    struct Ahead {
+      Tile tile;
+      float w_scale, bias[4];
+    };
+    auto ahead = [&](int t, int e) {
+      Ahead a = {};
+      a.w_scale = 1.0f;
+      if (t >= num_tiles) return a;
+      a.tile = tile_of<CG>(groups, p, t, e);
+      if (p.w_scale) a.w_scale = __ldg(p.w_scale + a.tile.e);
+      if (p.bias) {
+        const float* bias = p.bias + static_cast<long long>(a.tile.e) * (p.gated ? 2 : 1) * p.n;
+        const int f0 = (a.tile.f * CG + static_cast<int>(rank)) * width + quarter * warp_width + (lane >> 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int f = f0 + (p.gated ? 8 * (i >> 1) : 8 * i);
+          if (f < p.n) a.bias[i] = __ldg(bias + (p.gated && (i & 1) ? p.n : 0) + f);
+        }
+      }
+      return a;
+    };
     int j = 0;
+    Ahead next = ahead(first_tile, 0);
     for (int t = first_tile; t < num_tiles; t += tile_step, ++j) {
-      const Tile tile = tile_of<CG>(lo, start, p, t);
+      const Ahead now = next;
+      const Tile& tile = now.tile;
+      const float alpha = x_scale * now.w_scale;
+      const float (&b)[4] = now.bias;
+      next = ahead(t + tile_step, tile.e);
       const int buf = j & 1;
       const uint32_t buf_ph = (j >> 1) & 1;
-      float alpha = 1.0f;
-      if (p.x_scale) alpha = __ldg(p.x_scale);
-      if (p.w_scale) alpha *= __ldg(p.w_scale + tile.e);
       const uint32_t taddr = buf * kBufferColumns + lanes;
       const int row0 = tile.lo + tile.r0;
       const int f0 = (tile.f * CG + static_cast<int>(rank)) * width;       // first feature of the CTA's tile
-      // Bias of the TMEM lanes 8 i + lane / 4 of the warp: features, or alternating eight gate and eight up features.
-      const float* bias = p.bias ? p.bias + static_cast<long long>(tile.e) * (p.gated ? 2 : 1) * p.n : nullptr;
-      float b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int f = f0 + quarter * warp_width + (p.gated ? 8 * (i >> 1) : 8 * i) + (lane >> 2);
-        b[i] = bias && f < p.n ? __ldg(bias + (p.gated && (i & 1) ? p.n : 0) + f) : 0.0f;
-      }
       const bool ok = set_all(set, mbar_wait(smem_u32(&h->acc_full[buf]), buf_ph, abort_flag, p.status, 104));
       if (!ok) break;
       fence_after();
+      // The accumulator is free for the tile after the next one once everything of it is in registers, before any row is stored.
+      auto release = [&] {
+        fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CG == 1) mbar_arrive(smem_u32(&h->acc_empty[buf]));
+          else arrive_remote(in_first_cta(smem_u32(&h->acc_empty[buf])));
+        }
+      };
+      if (set * kSlabRows >= tile.rows) release();
       // Slabs of 32 rows, the sets in turn.
       for (int c0 = set * kSlabRows; c0 < tile.rows; c0 += 2 * kSlabRows) {
         uint32_t v[2][16];
@@ -527,6 +577,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
         load_16_lanes(taddr + c0 + (16u << 16), v[1]);
         loads_done(v[0]);
         loads_done(v[1]);
+        if (c0 + 2 * kSlabRows >= tile.rows) release();
         const int rows = min(kSlabRows, tile.rows - c0);
         // value of lane group i (eight TMEM lanes), column group g, column 2 (lane % 4) + k
         auto value = [&](int i, int g, int k) { return fmaf(__uint_as_float(v[i >> 1][4 * g + 2 * (i & 1) + k]), alpha, b[i]); };
@@ -611,12 +662,6 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
             }
           }
         }
-      }
-      fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (CG == 1) mbar_arrive(smem_u32(&h->acc_empty[buf]));
-        else arrive_remote(in_first_cta(smem_u32(&h->acc_empty[buf])));
       }
     }
   }
@@ -732,7 +777,7 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   p.block_bytes = (p.block_bytes + 1023u) & ~1023u;
   const int elem = a.y_dtype == B2VX_DT_FLOAT32 ? 4 : 2;
   p.y_vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride * elem % 16 == 0;
-  const int behind = kStagingBytes + static_cast<int>(sizeof(Header)) + 8 * (a.experts + 1) + 1024;   // and the ring's alignment
+  const int behind = kStagingBytes + static_cast<int>(sizeof(Header)) + static_cast<int>(sizeof(Group)) * (a.experts + 1) + 1024;   // and the ring's alignment
   const int room = static_cast<int>((kSmemBudget - behind) / p.block_bytes);      // k-blocks that fit
   p.stages = std::min(kMaxStages, room / kGroup);
   p.stage_bytes = kGroup * p.block_bytes;
