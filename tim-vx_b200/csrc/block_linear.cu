@@ -10,8 +10,9 @@
 // thread of the epilogue finds the gate and the up sum of a feature in its own registers.
 //
 // Persistent CTAs, one per SM, warp-specialised:
-//   warps 0, 2  producers  of W and of x: per k-block of 128 bytes one TMA box each (small ones of few rows) and the packed scales.
-//                          Two warps and few, large copies because a wait, an announcement and a copy take one thread about 340 cycles.
+//   warps 0, 2  producers  of W and of x: per k-block of 128 bytes one TMA box each (small ones of few rows)
+//   warp 3      producer   of the packed scales of both.  Three warps because a wait, an announcement and a copy take one thread about
+//                          340 cycles and each further copy 55.
 //   warp 1      issuer     copies a k-block's scales into tensor memory (tcgen05.cp, two slots in turn) and issues its four K steps
 //   warps 4-11  epilogue   two sets of four warps take slabs of 32 rows of the tile in turn: out of tensor memory, scale and bias,
 //                          activation, rounding, transposition through a buffer in shared memory, 16-byte stores
@@ -53,7 +54,7 @@ constexpr int kMaxDevices = 64;
 constexpr int kMinDynSmem = 120 * 1024;   // keeps two CTAs from sharing an SM and its tensor memory
 
 struct LinearParams {
-  int n, rows, experts, gated;
+  int n, rows, experts;
   int bn;                     // most rows of x in a tile
   int feature_tiles;          // tiles along the features of one group
   int scale_tiles;            // 128-row tiles of one matrix of W (and of its packed scales)
@@ -282,9 +283,19 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&v);
   }
 }
+// The same 16-byte pieces one number at a time, where rows of y are not aligned or a piece is cut; out of line, it would only be in the way.
+template <typename T>
+__device__ __noinline__ void store_elements(T* to, long long step, uint32_t from, int row_step, int steps, int rows, int count) {
+  for (int u = 0; u < steps && u * row_step < rows; ++u, to += step)
+    for (int k = 0; k < count; ++k) {
+      uint16_t v;
+      asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(from + u * row_step * 128 + 2 * k));
+      reinterpret_cast<uint16_t*>(to)[k] = v;
+    }
+}
 __device__ __forceinline__ float gate(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
-template <int KIND, int CG, typename T>
+template <int KIND, int CG, bool GATED, typename T>
 __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_constant__ Maps maps, const LinearParams p) {
   constexpr int NW = KIND == 0 ? 0 : (KIND == B2VX_FP4_BLOCK32 ? 2 : 4);   // scale words per stage
   extern __shared__ uint8_t smem_raw[];
@@ -303,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
-      mbar_init(smem_u32(&h->full[i]), 2);
+      mbar_init(smem_u32(&h->full[i]), NW ? 3 : 2);
       mbar_init(smem_u32(&h->empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
@@ -390,8 +401,6 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const Tile tile = tile_of<CG>(groups, p, t, e);
       e = tile.e;
       const int ft = tile.f * CG + static_cast<int>(rank);
-      // scales: of a tile whose rows do not exist those of the last that do (its outputs are not stored)
-      int sf = (tile.e * p.k_blocks * p.scale_tiles + min(ft, p.scale_tiles - 1)) * NW;
       for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
         if (elect_one()) {
           ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 101);
@@ -399,17 +408,14 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
             uint32_t dst = ring + s * p.stage_bytes;
             const uint32_t full = announce + 8 * s;
             const int end = min(kb + kGroup, p.k_blocks);
-            if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (end - kb) * CG * (kWTile + NW * kScaleTile));
-            int scales = sf;
-            for (int k = kb; k < end; ++k, dst += p.block_bytes, scales += p.scale_tiles * NW) {
-              if (p.gated) load_5d<CG>(dst, &maps.w, k * kStageBytes, ft * 8, tile.e, full);
+            if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (end - kb) * CG * kWTile);
+            for (int k = kb; k < end; ++k, dst += p.block_bytes) {
+              if (GATED) load_5d<CG>(dst, &maps.w, k * kStageBytes, ft * 8, tile.e, full);
               else load_3d<CG>(dst, &maps.w, k * kStageBytes, ft * 128, tile.e, full);
-              if constexpr (NW > 0) load_2d<CG>(dst + sfa_off, &maps.w_scales, 0, scales, full);
             }
           }
         }
         __syncwarp();
-        sf += kGroup * p.scale_tiles * NW;
         if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
       }
     }
@@ -426,9 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       // one large box where most of it is needed, else boxes of 32 rows
       const bool large = 2 * need > p.x_box;
       const int boxes = large ? 1 : (need + kBoxRows - 1) / kBoxRows;
-      const int atoms = NW ? (tile.n_mma + 127) >> 7 : 0;
-      const uint32_t tx = CG * ((large ? p.x_box : boxes * kBoxRows) * kStageBytes + atoms * NW * kScaleTile);
-      int sf = (expert_scale_tile(tile.lo, tile.e, p.bn) + tile.i * p.sfb_atoms) * NW;
+      const uint32_t tx = CG * (large ? p.x_box : boxes * kBoxRows) * kStageBytes;
       for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
         if (elect_one()) {
           ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 105);
@@ -437,20 +441,49 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
             const uint32_t full = announce + 8 * s;
             const int end = min(kb + kGroup, p.k_blocks);
             if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (end - kb) * tx);
-            int scales = sf;
-            for (int k = kb; k < end; ++k, dst += p.block_bytes, scales += p.x_scale_tiles * NW) {
+            for (int k = kb; k < end; ++k, dst += p.block_bytes) {
               if (large) {
                 load_2d<CG>(dst + x_off, &maps.x, k * kStageBytes, row, full);
               } else {
                 for (int b = 0; b < boxes; ++b) load_2d<CG>(dst + x_off + b * kBoxRows * kStageBytes, &maps.x32, k * kStageBytes, row + b * kBoxRows, full);
               }
-              if constexpr (NW > 0)
-                for (int a = 0; a < atoms; ++a) load_2d<CG>(dst + sfb_off + a * NW * kScaleTile, &maps.x_scales, 0, scales + a * NW, full);
             }
           }
         }
         __syncwarp();
-        sf += kGroup * p.x_scale_tiles * NW;
+        if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
+      }
+    }
+  } else if (NW > 0 && warp == 3) {
+    // ------------------------------------------------------------ producer of scales
+    pdl_wait();
+    const uint32_t announce = CG == 1 ? full0 : in_first_cta(full0);
+    const uint32_t tx = CG * (1 + p.sfb_atoms) * NW * kScaleTile;
+    uint32_t s = 0, ph = 0;
+    bool ok = true;
+    for (int t = first_tile, e = 0; t < num_tiles; t += tile_step) {
+      const Tile tile = tile_of<CG>(groups, p, t, e);
+      e = tile.e;
+      // of a tile of W whose rows do not exist those of the last that do (its outputs are not stored)
+      int sfa = (tile.e * p.k_blocks * p.scale_tiles + min(tile.f * CG + static_cast<int>(rank), p.scale_tiles - 1)) * NW;
+      int sfb = (expert_scale_tile(tile.lo, tile.e, p.bn) + tile.i * p.sfb_atoms) * NW;
+      for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
+        const int blocks = min(kGroup, p.k_blocks - kb);
+        if (elect_one()) {
+          ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 106);
+          if (ok) {
+            uint32_t dst = ring + s * p.stage_bytes;
+            const uint32_t full = announce + 8 * s;
+            if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, blocks * tx);
+            for (int b = 0; b < blocks; ++b, dst += p.block_bytes) {
+              load_2d<CG>(dst + sfa_off, &maps.w_scales, 0, sfa + b * p.scale_tiles * NW, full);
+              load_2d<CG>(dst + sfb_off, &maps.x_scales, 0, sfb + b * p.x_scale_tiles * NW, full);
+            }
+          }
+        }
+        __syncwarp();
+        sfa += kGroup * p.scale_tiles * NW;
+        sfb += kGroup * p.x_scale_tiles * NW;
         if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
       }
     }
@@ -517,8 +550,8 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     const int ew = warp - kFirstEpilogueWarp, quarter = ew & 3, set = ew >> 2;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     T* y = static_cast<T*>(p.y);
-    const int width = p.gated ? 64 : 128;                 // features of a CTA's tile
-    const int warp_width = p.gated ? 16 : 32;             // of a warp
+    const int width = GATED ? 64 : 128;                 // features of a CTA's tile
+    const int warp_width = GATED ? 16 : 32;             // of a warp
     const uint32_t out = staging + set * kSlabBytes;
     const float x_scale = p.x_scale ? __ldg(p.x_scale) : 1.0f;
     // What a tile needs of global memory is asked for while the tile before it is worked on.  Bias of the TMEM lanes 8 i + lane / 4 of
@@ -534,12 +567,12 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       a.tile = tile_of<CG>(groups, p, t, e);
       if (p.w_scale) a.w_scale = __ldg(p.w_scale + a.tile.e);
       if (p.bias) {
-        const float* bias = p.bias + static_cast<long long>(a.tile.e) * (p.gated ? 2 : 1) * p.n;
+        const float* bias = p.bias + static_cast<long long>(a.tile.e) * (GATED ? 2 : 1) * p.n;
         const int f0 = (a.tile.f * CG + static_cast<int>(rank)) * width + quarter * warp_width + (lane >> 2);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int f = f0 + (p.gated ? 8 * (i >> 1) : 8 * i);
-          if (f < p.n) a.bias[i] = __ldg(bias + (p.gated && (i & 1) ? p.n : 0) + f);
+          const int f = f0 + (GATED ? 8 * (i >> 1) : 8 * i);
+          if (f < p.n) a.bias[i] = __ldg(bias + (GATED && (i & 1) ? p.n : 0) + f);
         }
       }
       return a;
@@ -590,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
               if (r >= rows) continue;
               float* to = reinterpret_cast<float*>(y) + (row0 + c0 + r) * p.y_stride + f0 + quarter * warp_width + (lane >> 2);
               const int f = f0 + quarter * warp_width + (lane >> 2);
-              if (p.gated) {
+              if (GATED) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
                   if (f + 8 * i < p.n) to[8 * i] = gate(value(2 * i, g, k), value(2 * i + 1, g, k));
@@ -607,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
           // tiles that are already queued: with 1408 columns of K a slab then took 2500 cycles.
           uint32_t m[4][4];
           uint32_t at, step;                               // where matrices m[0] go, and from one m to the next
-          if (p.gated) {
+          if (GATED) {
             // two matrices (features 8 i) of two column groups at a time
             const uint32_t piece = quarter * 2 + ((lane >> 3) & 1);
             at = out + (lane & 7) * 128 + ((piece ^ (lane & 7)) << 4) + (lane >> 4) * 1024;
@@ -631,34 +664,29 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
           set_barrier(set);                                // every thread has read the last slab
           store_transposed(at, m[0][0], m[0][1], m[0][2], m[0][3]);
           store_transposed(at + step, m[1][0], m[1][1], m[1][2], m[1][3]);
-          if (!p.gated) {
+          if (!GATED) {
             store_transposed(at + 2 * step, m[2][0], m[2][1], m[2][2], m[2][3]);
             store_transposed(at + 3 * step, m[3][0], m[3][1], m[3][2], m[3][3]);
           }
           set_barrier(set);
           // 16 bytes a thread and step: of 128 (gated: 64) features a row, eight (sixteen) rows at a time
+          constexpr int kSteps = GATED ? 2 : 4, kRowStep = kSlabRows / kSteps;
           const int thread = quarter * 32 + lane;
-          const int q = p.gated ? thread & 7 : thread & 15, r0 = p.gated ? thread >> 3 : thread >> 4, r_step = p.gated ? 16 : 8, f = f0 + 8 * q;
+          const int q = GATED ? thread & 7 : thread & 15, r0 = GATED ? thread >> 3 : thread >> 4, f = f0 + 8 * q;
           T* to = y + (row0 + c0 + r0) * p.y_stride + f;
           const uint32_t from = out + (q >> 3) * 4096 + r0 * 128 + (((q & 7) ^ (r0 & 7)) << 4);
           if (f < p.n) {
-            uint32_t w[4][4];
+            uint32_t w[kSteps][4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (u < 2 || !p.gated)
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[u][0]), "=r"(w[u][1]), "=r"(w[u][2]), "=r"(w[u][3]) : "r"(from + u * r_step * 128));
-            const bool vec = p.y_vec && f + 8 <= p.n;
+            for (int u = 0; u < kSteps; ++u)
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[u][0]), "=r"(w[u][1]), "=r"(w[u][2]), "=r"(w[u][3]) : "r"(from + u * kRowStep * 128));
+            if (p.y_vec && f + 8 <= p.n) {
+              const long long step = kRowStep * p.y_stride;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              if ((u >= 2 && p.gated) || r0 + u * r_step >= rows) continue;
-              T* dst = to + u * r_step * p.y_stride;
-              if (vec) {
-                *reinterpret_cast<uint4*>(dst) = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
-              } else {
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
-                  if (f + k < p.n) reinterpret_cast<uint16_t*>(dst)[k] = static_cast<uint16_t>(w[u][k >> 1] >> (16 * (k & 1)));
-              }
+              for (int u = 0; u < kSteps; ++u, to += step)
+                if (r0 + u * kRowStep < rows) *reinterpret_cast<uint4*>(to) = make_uint4(w[u][0], w[u][1], w[u][2], w[u][3]);
+            } else {
+              store_elements<T>(to, kRowStep * p.y_stride, from, kRowStep, kSteps, rows - r0, min(8, p.n - f));
             }
           }
         }
@@ -710,9 +738,9 @@ bool encode_scales(CUtensorMap* map, const void* base, uint64_t tiles, uint32_t 
   const cuuint32_t box[2] = {kScaleTile / 4, box_tiles};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
-template <int KIND, int CG, typename T>
+template <int KIND, int CG, bool GATED, typename T>
 cudaError_t start(const Maps& maps, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
-  auto* kernel = block_linear_kernel<KIND, CG, T>;
+  auto* kernel = block_linear_kernel<KIND, CG, GATED, T>;
   // once per GPU (a repeated setting by racing first calls does no harm): the attribute costs a call a microsecond of the host's time
   static std::atomic<bool> ready[kMaxDevices];
   int dev = 0;
@@ -745,11 +773,16 @@ cudaError_t start(const Maps& maps, const LinearParams& p, int grid, size_t smem
   cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, maps, p);
 }
-template <int KIND, int CG>
+template <int KIND, int CG, bool GATED>
 cudaError_t start_typed(const Maps& m, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
-  if (p.y_dtype == B2VX_DT_FLOAT32) return start<KIND, CG, float>(m, p, grid, smem, s);
-  if (p.y_dtype == B2VX_DT_FLOAT16) return start<KIND, CG, __half>(m, p, grid, smem, s);
-  return start<KIND, CG, __nv_bfloat16>(m, p, grid, smem, s);
+  if (p.y_dtype == B2VX_DT_FLOAT32) return start<KIND, CG, GATED, float>(m, p, grid, smem, s);
+  if (p.y_dtype == B2VX_DT_FLOAT16) return start<KIND, CG, GATED, __half>(m, p, grid, smem, s);
+  return start<KIND, CG, GATED, __nv_bfloat16>(m, p, grid, smem, s);
+}
+template <int KIND>
+cudaError_t start_kind(const Maps& m, const LinearParams& p, int cg, int gated, int grid, size_t smem, cudaStream_t s) {
+  if (cg == 2) return gated ? start_typed<KIND, 2, true>(m, p, grid, smem, s) : start_typed<KIND, 2, false>(m, p, grid, smem, s);
+  return gated ? start_typed<KIND, 1, true>(m, p, grid, smem, s) : start_typed<KIND, 1, false>(m, p, grid, smem, s);
 }
 
 }  // namespace
@@ -762,7 +795,6 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   p.n = static_cast<int>(a.n);
   p.rows = static_cast<int>(a.rows);
   p.experts = a.experts;
-  p.gated = a.gated;
   const uint64_t kbytes = fp4 ? static_cast<uint64_t>(a.k) / 2 : static_cast<uint64_t>(a.k) * 2;
   p.k_blocks = static_cast<int>((kbytes + kStageBytes - 1) / kStageBytes);
   p.scale_tiles = static_cast<int>(weight_tiles(a.n, a.gated));
@@ -810,17 +842,16 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   }
   bool ok = a.gated ? encode_gated(&maps.w, a.w, kbytes, a.n, a.experts) : encode_rows(&maps.w, a.w, kbytes, kbytes, a.n, a.experts, 3, 128);
   ok = ok && encode_rows(&maps.x, a.x, kbytes, x_pitch, rows, 1, 2, p.x_box) && encode_rows(&maps.x32, a.x, kbytes, x_pitch, rows, 1, 2, kBoxRows);
-  if (fp4) ok = ok && encode_scales(&maps.w_scales, a.w_scales, w_tiles, nw) && encode_scales(&maps.x_scales, a.x_scales, x_tiles, nw);
+  if (fp4) ok = ok && encode_scales(&maps.w_scales, a.w_scales, w_tiles, nw) && encode_scales(&maps.x_scales, a.x_scales, x_tiles, nw * p.sfb_atoms);
   if (!ok) {
     *why = "tensor map refused";
     return cudaErrorInvalidValue;
   }
   const long long most = (a.rows / p.bn + groups) * p.feature_tiles;
   const int grid = static_cast<int>(std::max<long long>(1, std::min<long long>(a.sm_count / cg, most))) * cg;
-  if (a.format == 0) return cg == 2 ? start_typed<0, 2>(maps, p, grid, smem, s) : start_typed<0, 1>(maps, p, grid, smem, s);
-  if (a.format == B2VX_FP4_BLOCK32)
-    return cg == 2 ? start_typed<B2VX_FP4_BLOCK32, 2>(maps, p, grid, smem, s) : start_typed<B2VX_FP4_BLOCK32, 1>(maps, p, grid, smem, s);
-  return cg == 2 ? start_typed<B2VX_FP4_BLOCK16, 2>(maps, p, grid, smem, s) : start_typed<B2VX_FP4_BLOCK16, 1>(maps, p, grid, smem, s);
+  if (a.format == 0) return start_kind<0>(maps, p, cg, a.gated, grid, smem, s);
+  if (a.format == B2VX_FP4_BLOCK32) return start_kind<B2VX_FP4_BLOCK32>(maps, p, cg, a.gated, grid, smem, s);
+  return start_kind<B2VX_FP4_BLOCK16>(maps, p, cg, a.gated, grid, smem, s);
 }
 
 }  // namespace b2vx
