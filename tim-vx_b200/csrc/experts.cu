@@ -8,9 +8,10 @@
 //   place    a thread per pair
 #include <algorithm>
 
-#include "block_linear.cuh"
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
 #include "experts.cuh"
-#include "fp4.cuh"
 #include "pdl.cuh"
 
 namespace b2vx {

@@ -26,7 +26,7 @@ __device__ __forceinline__ uint32_t e2m1_codes(const float (&v)[8]) {
   return r;
 }
 // The values of eight codes.
-__device__ __forceinline__ void e2m1_values(uint32_t codes, float (&v)[8]) {
+__device__ __forceinline__ void e2m1_values(uint32_t codes, float* v) {
   uint32_t h[4];
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
@@ -68,76 +68,93 @@ __device__ __forceinline__ float e2m1_magnitude(uint32_t c) {
   return c < 2 ? 0.5f * c : __int_as_float((((c >> 1) + 126u) << 23) | ((c & 1u) << 22));
 }
 
-// The block's scale byte and the codes of this lane's eight numbers, which are `LANES` lanes' share of a block.
+// What quantization needs of block16's tensor scale, worked out once by a thread.
+struct TensorScale {
+  float g = 1.0f;          // times lift
+  float lift = 1.0f;       // numbers are multiplied by it: near the ends of float's range nothing then overflows or loses bits
+  float over_g = 1.0f;     // 1 / g
+  float over_6g = 1.0f;    // 1 / (6 g)
+  bool ok = true;
+};
 template <int FORMAT>
-__device__ __forceinline__ uint32_t quantize_8(float (&v)[8], float g, uint32_t& byte) {
-  constexpr int LANES = FORMAT == B2VX_FP4_BLOCK32 ? 4 : 2;
-  // magnitudes as integers: NaN is above infinity is above everything else
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-#pragma unroll
-  for (int d = 1; d < LANES; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-  float w[8];
+__device__ __forceinline__ TensorScale tensor_scale(const float* p) {
+  TensorScale t;
+  if (FORMAT == B2VX_FP4_BLOCK16) {
+    const float g = __ldg(p);
+    t.ok = g > 0.0f && g < __int_as_float(0x7f800000);
+    t.lift = g < 0x1p-60f ? 0x1p64f : (g > 0x1p60f ? 0x1p-64f : 1.0f);
+    t.g = g * t.lift;
+    t.over_g = 1.0f / t.g;
+    t.over_6g = 1.0f / (6.0f * t.g);
+  }
+  return t;
+}
+// Eight codes of numbers times a factor.
+__device__ __forceinline__ uint32_t e2m1_codes_times(const float* v, float f) {
+  const float r[8] = {v[0] * f, v[1] * f, v[2] * f, v[3] * f, v[4] * f, v[5] * f, v[6] * f, v[7] * f};
+  return e2m1_codes(r);
+}
+// Where a little less and a little more than a quotient round to different codes: the border between the two decides, by a comparison
+// that is exact, since border * s has few bits and the fused product with g is rounded only after the subtraction.  (Numbers of few
+// bits over a scale of few bits often lie on a border or next to it: with a tensor scale of 1 / 56, 16-bit numbers in one block
+// of twelve.)  diff: the nibbles that differ; number(i): the lane's i-th number.
+template <typename F>
+__device__ __forceinline__ uint32_t settle_codes(uint32_t codes, uint32_t diff, float s, float g, float lift, F number) {
+  while (diff) {
+    const int at = (__ffs(static_cast<int>(diff)) - 1) & ~3;
+    diff &= ~(15u << at);
+    const uint32_t a = (codes >> at) & 7u;                     // the other one is a + 1
+    const float border = 0.5f * (e2m1_magnitude(a) + e2m1_magnitude(a + 1u)) * s;
+    const float r = fmaf(border, g, -fabsf(number(at >> 2)) * lift);
+    if (r < 0.0f || (r == 0.0f && (a & 1u))) codes += 1u << at;
+  }
+  return codes;
+}
+
+// The block's scale byte and the codes of this lane's sixteen numbers: a block of block16, or half of one of block32, whose other half is
+// the neighbouring lane's.  top: the largest magnitude of the lane's numbers, as bits (NaN is above infinity is above everything else).
+// number(i): the lane's i-th number once more, for the few that need it.
+template <int FORMAT, typename F>
+__device__ __forceinline__ uint2 quantize_16(const float (&v)[16], uint32_t top, const TensorScale& t, uint32_t& byte, F number) {
   if (FORMAT == B2VX_FP4_BLOCK32) {
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    const int e = static_cast<int>(top >> 23) - 2;            // biased exponent of 2^(floor(log2 amax) - 2)
+    byte = static_cast<uint32_t>(max(e, 0));
+    const float f = __uint_as_float((254u - min(byte, 253u)) << 23);   // a power of two: the products are exact
+    uint2 codes = make_uint2(e2m1_codes_times(v, f), e2m1_codes_times(v + 8, f));
     if (top >= 0x7f800000u) {
       byte = 255u;
-      return 0u;
+      codes = make_uint2(0u, 0u);
     }
-    const int e = static_cast<int>(top >> 23) - 2;       // biased exponent of 2^(floor(log2 amax) - 2)
-    byte = static_cast<uint32_t>(max(e, 0));
-    const float inv = __uint_as_float((254u - byte) << 23);   // a power of two: products below are exact
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = v[i] * inv;
-    return e2m1_codes(w);
+    return codes;
   }
-  if (top >= 0x7f800000u || !(g > 0.0f) || !(g < __int_as_float(0x7f800000))) {
-    byte = 127u;
-    return 0u;
-  }
-  // Tensor scales near the ends of float's range: numbers and scale times one power of two, so that nothing below overflows or loses bits.
-  if (g < 0x1p-60f || g > 0x1p60f) {
-    const float lift = g < 1.0f ? 0x1p64f : 0x1p-64f;
-    g *= lift;
-    top = __float_as_uint(__uint_as_float(top) * lift);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= lift;
-  }
-  // amax / (6 g) in two roundings is off by less than 2^-22 of itself: where a little less and a little more round to the
-  // same byte, that is the answer; else the border between them decides, by an exact comparison: border * 6 has few bits and the
-  // fused product with g is rounded only after the subtraction.
-  const float amax = __uint_as_float(top);
-  const float q = amax / (6.0f * g);
-  const uint32_t two = e4m3_bytes(q * (1.0f - 0x1p-21f), q * (1.0f + 0x1p-21f));
+  // amax / (6 g) as a product of three roundings is off by less than 2^-22 of itself: where a little less and a little more round to
+  // the same byte, that is the answer, else the border between them, as in settle_codes.
+  constexpr float kLess = 1.0f - 0x1p-20f, kMore = 1.0f + 0x1p-20f;
+  const float amax = __uint_as_float(top) * t.lift;
+  const float q = amax * t.over_6g;
+  const uint32_t two = e4m3_bytes(q * kLess, q * kMore);
   byte = two >> 8;
   if ((two & 0xff) != byte) {
     const float border6 = 3.0f * (e4m3_value(two & 0xff) + e4m3_value(byte));
-    const float r = fmaf(border6, g, -amax);
+    const float r = fmaf(border6, t.g, -amax);
     if (r > 0.0f || (r == 0.0f && (byte & 1u))) byte = two & 0xff;
   }
   const float s = e4m3_value(byte);
-  if (byte == 0) return 0u;
-  // The numbers over s g, by the same argument.
-  const float inv = 1.0f / (s * g);
-  float hi[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float y = v[i] * inv;
-    w[i] = y * (1.0f - 0x1p-21f);
-    hi[i] = y * (1.0f + 0x1p-21f);
+  float over_s;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(over_s) : "f"(s));   // off by 2^-23; s = 0 is dealt with below
+  // The numbers over s g: the approximate reciprocal, two products and 1 / g are off by less than 2^-21 together.
+  const float inv = over_s * t.over_g * t.lift, less = inv * kLess, more = inv * kMore;
+  uint2 codes = make_uint2(e2m1_codes_times(v, less), e2m1_codes_times(v + 8, less));
+  const uint2 up = make_uint2(e2m1_codes_times(v, more), e2m1_codes_times(v + 8, more));
+  if ((codes.x != up.x || codes.y != up.y) && byte != 0) {
+    codes.x = settle_codes(codes.x, codes.x ^ up.x, s, t.g, t.lift, number);
+    codes.y = settle_codes(codes.y, codes.y ^ up.y, s, t.g, t.lift, [&](int i) { return number(8 + i); });
   }
-  uint32_t codes = e2m1_codes(w);
-  const uint32_t up = e2m1_codes(hi);
-  if (codes != up) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t a = (codes >> (4 * i)) & 7u, b = (up >> (4 * i)) & 7u;
-      if (a != b) {
-        const float border = 0.5f * (e2m1_magnitude(a) + e2m1_magnitude(b)) * s;
-        const float r = fmaf(border, g, -fabsf(v[i]));
-        if (r < 0.0f || (r == 0.0f && (a & 1u))) codes += (b - a) << (4 * i);
-      }
-    }
+  if (byte == 0) codes = make_uint2(0u, 0u);                  // every number rounds to zero
+  if (top >= 0x7f800000u || !t.ok) {
+    byte = 127u;
+    codes = make_uint2(0u, 0u);
   }
   return codes;
 }

@@ -1,8 +1,8 @@
 // Rows of numbers to 4-bit block floating point and back, packing of scales, gathering of rows.
 //
-// Quantization reads every number once and writes half a byte and a scale's share for it; it is bound by memory (a block is 16 or 32
-// neighbouring columns, 2 or 4 lanes of eight columns each, so its maximum costs one or two shuffles).  Eight numbers a lane:
-// one 16-byte load of 16-bit numbers, one 4-byte store of codes, 128 bytes a warp.
+// Quantization reads every number once and writes half a byte and a scale's share for it; memory bounds block32, the instructions of
+// the two-sided rounding block16.  Sixteen columns a lane: a block of block16, so that its scale, some forty instructions, is worked out
+// once, or half a block of block32.
 #include <algorithm>
 
 #include "block_linear.cuh"
@@ -13,7 +13,7 @@ namespace b2vx {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kChunk = 256;   // columns of a warp per step, one pipeline stage of the products
+constexpr int kChunk = 512;   // columns of a warp per step, two k-blocks of the products
 
 template <typename T>
 __device__ __forceinline__ float to_float(T v) {
@@ -28,19 +28,43 @@ __device__ __forceinline__ T from_float(float v) {
   else return __float2bfloat16_rn(v);
 }
 
-// Eight numbers from column c on, zeros from column k on.  VEC: rows start on 16 bytes, so whole pieces load in 16 bytes.
+// Sixteen numbers from column c on, zeros from column k on, as they lie.  VEC: rows start on 16 bytes, so whole pieces load in 16 bytes.
+template <typename T>
+struct alignas(16) Sixteen {
+  T v[16];
+};
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_8(const T* row, long long c, long long k, float (&v)[8]) {
-  if (VEC && c + 8 <= k) {
-    alignas(16) T t[8];
+__device__ __forceinline__ Sixteen<T> load_16(const T* row, int c, int k) {
+  Sixteen<T> t;
+  constexpr int W = sizeof(t) / 16;
+  if (VEC && c + 16 <= k) {
     const uint4* src = reinterpret_cast<const uint4*>(row + c);
-    *reinterpret_cast<uint4*>(t) = __ldg(src);
-    if (sizeof(T) == 4) *reinterpret_cast<uint4*>(t + 4) = __ldg(src + 1);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float(t[i]);
+    for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(&t)[i] = __ldg(src + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < k ? to_float(row[c + i]) : 0.0f;
+    for (int i = 0; i < 16; ++i) t.v[i] = c + i < k ? row[c + i] : from_float<T>(0.0f);
+  }
+  return t;
+}
+// The largest magnitude, as float bits.
+template <typename T>
+__device__ __forceinline__ uint32_t top_of(const Sixteen<T>& t) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(t.v[i]) & 0x7fffffffu);
+    return top;
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&t);
+    constexpr uint32_t kMagnitudes = 0x7fff7fffu;
+    uint32_t two = w[0] & kMagnitudes;
+#pragma unroll
+    for (int i = 1; i < 7; i += 2) two = __vimax3_u16x2(two, w[i] & kMagnitudes, w[i + 1] & kMagnitudes);
+    two = __vmaxu2(two, w[7] & kMagnitudes);
+    const uint32_t top = max(two & 0xffffu, two >> 16);
+    if constexpr (std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top)))) & 0x7fffffffu;
+    else return top << 16;
   }
 }
 
@@ -54,21 +78,24 @@ __device__ __forceinline__ int group_of(const int32_t* offsets, int experts, lon
 // `split` warps share a row, each taking every split-th chunk.
 template <typename T, int FORMAT, bool VEC, bool PACKED>
 __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArgs a, int chunks, int split) {
-  constexpr int B = fp4_block(FORMAT), LANES = B / 8;
+  constexpr int B = fp4_block(FORMAT), LANES = B / 16, PER = scale_words_per_stage(FORMAT);   // lanes to a block, words to a k-block
   pdl_wait();
   pdl_trigger();   // after the wait: a product behind this kernel may read its weights before its own wait
   const int lane = threadIdx.x & 31;
-  const long long warps = static_cast<long long>(gridDim.x) * kWarps;
-  const float g = FORMAT == B2VX_FP4_BLOCK16 ? __ldg(a.tensor_scale) : 1.0f;
-  const long long k32 = (a.k + 31) / 32 * 32, blocks = (a.k + B - 1) / B;
+  const uint32_t warps = gridDim.x * kWarps, units = static_cast<uint32_t>(a.rows) * split;
+  const TensorScale scale = tensor_scale<FORMAT>(a.tensor_scale);
+  const int k = static_cast<int>(a.k), k32 = (k + 31) / 32 * 32, blocks = (k + B - 1) / B;
   const T* x = static_cast<const T*>(a.x);
-  for (long long unit = static_cast<long long>(blockIdx.x) * kWarps + (threadIdx.x >> 5); unit < a.rows * split; unit += warps) {
-    const long long row = split == 1 ? unit : unit / split;
-    const int part = split == 1 ? 0 : static_cast<int>(unit - row * split);
+  for (uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5); unit < units; unit += warps) {
+    const uint32_t row = split == 1 ? unit : unit / split;
+    const int part = static_cast<int>(unit - row * split);
     const long long src = a.row_index ? a.row_index[row] : row;
     const bool there = src >= 0 && src < a.x_rows;
     const T* from = x + (there ? src : 0) * a.x_stride;
-    const long long k_here = there ? a.k : 0;
+    const int k_here = there ? k : 0;
+    uint8_t* codes_row = a.codes + row * a.codes_pitch;
+    int c = part * kChunk + lane * 16;
+    Sixteen<T> t = load_16<T, VEC>(from, c, k_here);
     uint8_t* tile = nullptr;      // PACKED: where the row's words of the first scale tile lie; null: the row belongs to no group
     if (PACKED) {
       int e = 0, lo = 0, count = static_cast<int>(a.rows);
@@ -81,55 +108,86 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArg
       if (lo >= 0 && in >= 0 && in < count) {
         const int per = rows_of_tile(count, a.bn), i = in / per, r = in - i * per;
         const int at = expert_scale_tile(lo, e, a.bn) + i * ((a.bn + 127) / 128) + r / 128;
-        tile = a.scales + static_cast<long long>(at) * (scale_words_per_stage(FORMAT) * kScaleTile) + (r % 32) * 16 + (r % 128 / 32) * 4;
+        tile = a.scales + static_cast<long long>(at) * (PER * kScaleTile) + (r % 32) * 16 + (r % 128 / 32) * 4;
       }
     }
     for (int chunk = part; chunk < chunks; chunk += split) {
-      const long long c = static_cast<long long>(chunk) * kChunk + lane * 8;
-      float v[8];
-      load_8<T, VEC>(from, c, k_here, v);
+      // the next chunk is asked for before this one is worked on
+      const int c_next = c + split * kChunk;
+      Sixteen<T> next = t;
+      if (chunk + split < chunks) next = load_16<T, VEC>(from, c_next, k_here);
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = to_float(t.v[i]);
       uint32_t byte;
-      const uint32_t codes = quantize_8<FORMAT>(v, g, byte);
-      if (c < k32) *reinterpret_cast<uint32_t*>(a.codes + row * a.codes_pitch + c / 2) = codes;
+      const uint2 codes = quantize_16<FORMAT>(v, top_of(t), scale, byte, [&](int i) { return to_float(from[c + i]); });
+      if (c < k32) {
+        // k32 is a multiple of 32, c of 16: all sixteen codes lie inside the row
+        uint32_t* to = reinterpret_cast<uint32_t*>(codes_row + c / 2);
+        if (a.codes_pitch % 8 == 0) *reinterpret_cast<uint2*>(to) = codes;
+        else { to[0] = codes.x; to[1] = codes.y; }
+      }
       if (PACKED) {
-        if (c >= a.k) byte = 0;
+        if (c >= k) byte = 0;
         uint32_t word = byte | __shfl_down_sync(0xffffffffu, byte, LANES) << 8;
         word |= __shfl_down_sync(0xffffffffu, word, 2 * LANES) << 16;
-        if (lane % (4 * LANES) == 0 && tile)
-          *reinterpret_cast<uint32_t*>(tile + (static_cast<long long>(chunk) * a.scale_tiles * scale_words_per_stage(FORMAT) + lane / (4 * LANES)) * kScaleTile) = word;
+        const int k_block = c / 256, w = lane % 16 / (4 * LANES);
+        if (lane % (4 * LANES) == 0 && tile && k_block * 256 < k)
+          *reinterpret_cast<uint32_t*>(tile + (static_cast<long long>(k_block) * a.scale_tiles * PER + w) * kScaleTile) = word;
       } else if (lane % LANES == 0 && c / B < blocks) {
         a.scales[row * a.scales_pitch + c / B] = static_cast<uint8_t>(byte);
       }
+      t = next;
+      c = c_next;
     }
   }
 }
 
+// Rows of values: `split` warps share a row as above, sixteen columns a lane and step, two steps asked for at once.
 template <typename T, int FORMAT>
-__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
-                                                         const float* tensor_scale, long long rows, long long k, T* y, long long y_stride,
-                                                         int pieces, int vec) {
-  constexpr int B = fp4_block(FORMAT);
+__global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
+                                                                 const float* tensor_scale, uint32_t rows, int k, T* y, long long y_stride,
+                                                                 int chunks, int split, int vec) {
+  constexpr int B = fp4_block(FORMAT), U = 2;
   pdl_trigger();
   pdl_wait();
+  const int lane = threadIdx.x & 31;
   const float g = FORMAT == B2VX_FP4_BLOCK16 ? __ldg(tensor_scale) : 1.0f;
-  const long long total = rows * pieces, step = static_cast<long long>(gridDim.x) * blockDim.x;
-  for (long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x; i < total; i += step) {
-    const long long row = i / pieces, c = (i - row * pieces) * 8;
-    const uint32_t word = __ldg(reinterpret_cast<const uint32_t*>(codes + row * codes_pitch + c / 2));
-    const float s = scale_value<FORMAT>(__ldg(scales + row * scales_pitch + c / B));
-    float v[8];
-    e2m1_values(word, v);
-    alignas(16) T out[8];
+  const uint32_t warps = gridDim.x * kWarps, units = rows * split;
+  for (uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5); unit < units; unit += warps) {
+    const uint32_t row = split == 1 ? unit : unit / split;
+    const uint8_t *codes_row = codes + row * codes_pitch, *scales_row = scales + row * scales_pitch;
+    T* to = y + row * y_stride;
+    for (int chunk = static_cast<int>(unit - row * split); chunk < chunks; chunk += U * split) {
+      uint32_t word[U][2], byte[U];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) out[j] = from_float<T>(FORMAT == B2VX_FP4_BLOCK16 ? v[j] * s * g : v[j] * s);
-    T* dst = y + row * y_stride + c;
-    if (vec && c + 8 <= k) {
-      *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(out);
-      if (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst + 4) = *reinterpret_cast<const uint4*>(out + 4);
-    } else {
+      for (int u = 0; u < U; ++u) {
+        const int c = (chunk + u * split) * kChunk + lane * 16;
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(codes_row + c / 2);
+        word[u][0] = c < k ? __ldg(from) : 0u;
+        word[u][1] = c < k ? __ldg(from + 1) : 0u;
+        byte[u] = c < k ? __ldg(scales_row + c / B) : 0u;
+      }
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (c + j < k) dst[j] = out[j];
+      for (int u = 0; u < U; ++u) {
+        const int c = (chunk + u * split) * kChunk + lane * 16;
+        if (c >= k) break;
+        const float s = scale_value<FORMAT>(byte[u]);
+        float v[16];
+        e2m1_values(word[u][0], v);
+        e2m1_values(word[u][1], v + 8);
+        Sixteen<T> out;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) out.v[j] = from_float<T>(FORMAT == B2VX_FP4_BLOCK16 ? v[j] * s * g : v[j] * s);
+        if (vec && c + 16 <= k) {
+#pragma unroll
+          for (int i = 0; i < static_cast<int>(sizeof(out)) / 16; ++i) reinterpret_cast<uint4*>(to + c)[i] = reinterpret_cast<const uint4*>(&out)[i];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (c + j < k) to[c + j] = out.v[j];
+        }
+      }
     }
   }
 }
@@ -181,15 +239,20 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const uint16_t* x, lon
 }
 
 int blocks_for(long long threads, int per_block) {
-  return static_cast<int>(std::max<long long>(1, std::min<long long>((threads + per_block - 1) / per_block, 148 * 8)));
+  return static_cast<int>(std::max<long long>(1, std::min<long long>((threads + per_block - 1) / per_block, 148 * 5)));
+}
+
+// Warps that share a row: up to as many as it has chunks, so that there are about four units of work for each warp that fits the GPU (40 an
+// SM) and an uneven last round costs little.
+int split_of(long long rows, int chunks) {
+  const long long fill = 4 * 148 * 40;
+  return static_cast<int>(std::max<long long>(1, std::min<long long>(chunks, fill / std::max<long long>(1, rows))));
 }
 
 template <typename T, int FORMAT, bool VEC>
 cudaError_t quantize(const QuantizeArgs& a, cudaStream_t s) {
   const int chunks = static_cast<int>((a.k + kChunk - 1) / kChunk);
-  // a row to a warp where the rows fill the GPU (8 blocks an SM), else shared by up to as many warps as it has chunks
-  const long long fill = 148 * 8 * kWarps;
-  const int split = static_cast<int>(std::max<long long>(1, std::min<long long>(chunks, fill / std::max<long long>(1, a.rows))));
+  const int split = split_of(a.rows, chunks);
   const int grid = blocks_for(a.rows * split, kWarps);
   if (a.scales_pitch == 0) return launch_pdl(quantize_kernel<T, FORMAT, VEC, true>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
   return launch_pdl(quantize_kernel<T, FORMAT, VEC, false>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
@@ -206,12 +269,12 @@ cudaError_t quantize_format(const QuantizeArgs& a, cudaStream_t s) {
 template <typename T>
 cudaError_t dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch, const float* tensor_scale, int format,
                        long long rows, long long k, void* y, long long y_stride, cudaStream_t s) {
-  const int pieces = static_cast<int>((k + 7) / 8);
+  const int chunks = static_cast<int>((k + kChunk - 1) / kChunk);
+  const int split = split_of(rows, chunks);
   const int vec = reinterpret_cast<uintptr_t>(y) % 16 == 0 && (y_stride * sizeof(T)) % 16 == 0;
-  const int grid = blocks_for(rows * pieces, 256);
   auto* kernel = format == B2VX_FP4_BLOCK32 ? dequantize_kernel<T, B2VX_FP4_BLOCK32> : dequantize_kernel<T, B2VX_FP4_BLOCK16>;
-  return launch_pdl(kernel, dim3(grid), dim3(256), 0, s, codes, codes_pitch, scales, scales_pitch, tensor_scale, rows, k, static_cast<T*>(y), y_stride,
-                    pieces, vec);
+  return launch_pdl(kernel, dim3(blocks_for(rows * split, kWarps)), dim3(kWarps * 32), 0, s, codes, codes_pitch, scales, scales_pitch, tensor_scale,
+                    static_cast<uint32_t>(rows), static_cast<int>(k), static_cast<T*>(y), y_stride, chunks, split, vec);
 }
 
 }  // namespace
