@@ -369,6 +369,27 @@ def test_linear_row_index_and_types():
     close(y, *expected(operand(rows, "block32")[0], wv[0], None, False))
 
 
+@pytest.mark.parametrize("fmt,k", [("block32", 1056), ("block16", 1120)])
+def test_expert_linear_rows_taken_several_times(fmt, k):
+    """Enough rows that each row of x is quantized once and then copied; indices outside x give rows of zeros."""
+    tokens, rows, n, experts = 300, 5000, 72, 5
+    x = gaussian(tokens, k, torch.bfloat16, 12, 1.0)
+    rng = np.random.default_rng(3)
+    index = rng.integers(-2, tokens + 2, rows).astype(np.int32)
+    starts = np.array([0, 700, 700, 2001, 4990, 4997], np.int32)
+    w, wv = weight_of(experts, n, k, fmt, 6)
+    xv, s = operand(x, fmt)
+    y = torch.full((rows, n), -77.0, dtype=torch.bfloat16, device="cuda")
+    D.expert_linear(x, w, torch.from_numpy(starts).cuda(), row_index=torch.from_numpy(index).cuda(), x_scale=s, out=y)
+    there = (index >= 0) & (index < tokens)
+    full = np.where(there[:, None], xv[np.where(there, index, 0)], 0.0)
+    for e in range(experts):
+        lo, hi = starts[e], starts[e + 1]
+        if hi > lo:
+            close(y[lo:hi], *expected(full[lo:hi], wv[e], None, False))
+    assert (y[starts[-1]:] == -77.0).all()
+
+
 def test_nan_scales_reach_only_their_outputs():
     x = gaussian(5, 128, torch.bfloat16, 1, 0.5)
     x[2, 7] = float("nan")

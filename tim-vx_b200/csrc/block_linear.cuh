@@ -66,6 +66,10 @@ struct QuantizeArgs {
   int scale_tiles;             // packed: expert_scale_tiles
 };
 cudaError_t launch_fp4_quantize(const QuantizeArgs& a, cudaStream_t s);
+// The operand x of a product (packed scales; codes_pitch is k / 2, a multiple of 16): quantized in one step, or each row of x once and then
+// copied to where row_index wants it.  `between`: fp4_twice_bytes bytes for that, aligned to 16.
+size_t fp4_twice_bytes(const QuantizeArgs& a);
+cudaError_t launch_fp4_operand(const QuantizeArgs& a, void* between, cudaStream_t s);
 cudaError_t launch_fp4_dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
                                   const float* tensor_scale, int format, long long rows, long long k, void* y, int y_dtype,
                                   long long y_stride, cudaStream_t s);

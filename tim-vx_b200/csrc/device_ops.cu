@@ -78,7 +78,7 @@ int device_status(bool clear) {
 
 // The parts of a product's workspace.
 struct Workspace {
-  size_t codes = 0, scales = 0, total = 0;
+  size_t codes = 0, scales = 0, between = 0, total = 0;
   uint64_t codes_pitch = 0;
 };
 Workspace workspace_of(const b2vx_linear_desc& d) {
@@ -92,7 +92,14 @@ Workspace workspace_of(const b2vx_linear_desc& d) {
     w.codes_pitch = d.k * 2;
     w.codes = round256(d.rows * w.codes_pitch);
   }
-  w.total = w.codes + w.scales;
+  if (d.w_format) {   // whether there will be a row_index is not known here
+    static const int32_t kSome = 0;
+    QuantizeArgs q = {};
+    q.x_rows = static_cast<long long>(d.x_rows); q.rows = static_cast<long long>(d.rows); q.k = static_cast<long long>(d.k);
+    q.format = d.w_format; q.row_index = &kSome;
+    w.between = round256(fp4_twice_bytes(q));
+  }
+  w.total = w.codes + w.scales + w.between;
   return w;
 }
 
@@ -242,7 +249,7 @@ extern "C" b2vx_status b2vx_linear_noalloc(const b2vx_linear_desc* d, const b2vx
     q.offsets = a->offsets; q.experts = l.experts;
     q.bn = tile_rows(l.rows, l.experts, l.format);
     q.scale_tiles = static_cast<int>(expert_scale_tiles(l.rows, l.experts, q.bn));
-    e = launch_fp4_quantize(q, s);
+    e = launch_fp4_operand(q, codes + ws.codes + ws.scales, s);
     l.x = codes; l.x_pitch = static_cast<long long>(ws.codes_pitch); l.x_scales = q.scales;
   } else if (direct) {
     l.x = a->x; l.x_pitch = static_cast<long long>(d->x_stride) * 2;
