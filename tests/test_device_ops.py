@@ -21,7 +21,7 @@ def desc(cls, base, **change):
 QUANTIZE = dict(format=1, x_dtype=16, x_rows=8, rows=8, k=96, x_stride=96, codes_pitch=48, scales_pitch=3)
 DEQUANTIZE = dict(format=1, y_dtype=16, rows=8, k=96, codes_pitch=48, scales_pitch=3, y_stride=96)
 LINEAR = dict(w_format=1, x_dtype=16, y_dtype=16, gated=0, experts=0, x_rows=8, rows=8, n=64, k=96, x_stride=96, y_stride=64)
-ROUTE = dict(logits_dtype=9, normalize=1, experts=16, top_k=4, tokens=8, logits_stride=16)
+ROUTE = dict(logits_dtype=9, normalize=1, experts=16, top_k=4, tokens=200, logits_stride=16)
 COMBINE = dict(dtype=16, top_k=2, tokens=8, n=64, z_rows=16, z_stride=64, residual_stride=64, y_stride=64)
 
 

@@ -291,7 +291,7 @@ extern "C" b2vx_status b2vx_route_noalloc(const b2vx_route_desc* d, const void* 
   }
   B2VX_NEED(logits && ids && weights && row_index && slots, "null argument");
   B2VX_NEED(aligned(logits, size_of(d->logits_dtype)), "a pointer is not aligned");
-  B2VX_NEED(workspace && aligned(workspace, 256) && workspace_bytes >= need, "a 256-byte aligned workspace of the told size is needed");
+  B2VX_NEED(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), "a 256-byte aligned workspace of the told size is needed");
   st = device(&pd, err, err_len);
   if (st != B2VX_OK) return st;
   return launched(launch_route(*d, logits, ids, weights, offsets, row_index, slots, workspace, s), err, err_len);

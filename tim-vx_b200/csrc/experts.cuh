@@ -11,7 +11,7 @@
 
 namespace b2vx {
 
-constexpr int kMaxTopK = 32;
+constexpr int kMaxTopK = 32;   // of a token: a lane for each
 
 size_t route_workspace_bytes(long long tokens, int experts);
 cudaError_t launch_route(const b2vx_route_desc& d, const void* logits, int32_t* ids, float* weights, int32_t* offsets, int32_t* row_index,
