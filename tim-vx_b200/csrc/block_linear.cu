@@ -22,6 +22,10 @@
 // once for 256 features.  No load is multicast: every CTA fetches its own operands; the loads of both announce themselves on
 // the first one's barrier.
 //
+// SPLIT (few tiles): the CTAs of a cluster share one tile's K.  Each leaves its partial sums in its shared memory, and after a barrier of the
+// cluster each adds up a share of the tile's features over all of them, in the order of the CTAs.  (One row through 4096 x 4096 has
+// 32 tiles: 32 SMs draw their 128 rows of W at 65 bytes a clock, a fifth of what memory gives.)
+//
 // Every wait is bounded as in gemm_tc.cu: on a time-out the CTA records a code and leaves through its common exit.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -62,6 +66,8 @@ struct LinearParams {
   int x_box;                  // rows of x in the large box, bn / CG
   int sfb_atoms;              // scale tiles of x to a tile of bn rows
   int x_scale_tiles;          // packed scale tiles along the rows of x
+  int split, split_blocks;    // CTAs that share a tile's K, k-blocks of each
+  uint32_t staging_bytes;
   int after_operand;
   uint32_t block_bytes, stage_bytes;
   uint32_t idesc;             // without N
@@ -106,6 +112,12 @@ __device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
   uint32_t r;
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
   return r;
+}
+// Four floats at the same place in CTA `cta`'s shared memory.
+__device__ __forceinline__ void load_from_cta(uint32_t addr, int cta, float (&v)[4]) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(cta));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(a) : "memory");
 }
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -295,7 +307,7 @@ __device__ __noinline__ void store_elements(T* to, long long step, uint32_t from
 }
 __device__ __forceinline__ float gate(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
-template <int KIND, int CG, bool GATED, typename T>
+template <int KIND, int CG, bool GATED, bool SPLIT, typename T>
 __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_constant__ Maps maps, const LinearParams p) {
   constexpr int NW = KIND == 0 ? 0 : (KIND == B2VX_FP4_BLOCK32 ? 2 : 4);   // scale words per stage
   extern __shared__ uint8_t smem_raw[];
@@ -303,12 +315,15 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t ring = (raw + 1023u) & ~1023u;
   const uint32_t staging = ring + p.stages * p.stage_bytes;
-  Header* h = reinterpret_cast<Header*>(smem_raw + (staging - raw) + kStagingBytes);
+  Header* h = reinterpret_cast<Header*>(smem_raw + (staging - raw) + p.staging_bytes);
   Group* groups = reinterpret_cast<Group*>(h + 1);
   volatile int* abort_flag = &h->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = CG == 1 ? 0u : cluster_rank();
-  const int first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
+  const int sharing = SPLIT ? p.split : CG;
+  const int first_tile = blockIdx.x / sharing, tile_step = gridDim.x / sharing;
+  const int part = SPLIT ? static_cast<int>(cluster_rank()) : 0;
+  const int kb_first = SPLIT ? part * p.split_blocks : 0, kb_end = SPLIT ? min(p.k_blocks, kb_first + p.split_blocks) : p.k_blocks;
   // a k-block: [128 rows of W | rows of x | scales of W | scales of x]
   const uint32_t x_off = kWTile, sfa_off = x_off + static_cast<uint32_t>(p.x_box) * kStageBytes, sfb_off = sfa_off + NW * kScaleTile;
 
@@ -401,13 +416,13 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const Tile tile = tile_of<CG>(groups, p, t, e);
       e = tile.e;
       const int ft = tile.f * CG + static_cast<int>(rank);
-      for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
+      for (int kb = kb_first; kb < kb_end; kb += kGroup) {
         if (elect_one()) {
           ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 101);
           if (ok) {
             uint32_t dst = ring + s * p.stage_bytes;
             const uint32_t full = announce + 8 * s;
-            const int end = min(kb + kGroup, p.k_blocks);
+            const int end = min(kb + kGroup, kb_end);
             if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (end - kb) * CG * kWTile);
             for (int k = kb; k < end; ++k, dst += p.block_bytes) {
               if (GATED) load_5d<CG>(dst, &maps.w, k * kStageBytes, ft * 8, tile.e, full);
@@ -433,13 +448,13 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const bool large = 2 * need > p.x_box;
       const int boxes = large ? 1 : (need + kBoxRows - 1) / kBoxRows;
       const uint32_t tx = CG * (large ? p.x_box : boxes * kBoxRows) * kStageBytes;
-      for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
+      for (int kb = kb_first; kb < kb_end; kb += kGroup) {
         if (elect_one()) {
           ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 105);
           if (ok) {
             uint32_t dst = ring + s * p.stage_bytes;
             const uint32_t full = announce + 8 * s;
-            const int end = min(kb + kGroup, p.k_blocks);
+            const int end = min(kb + kGroup, kb_end);
             if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (end - kb) * tx);
             for (int k = kb; k < end; ++k, dst += p.block_bytes) {
               if (large) {
@@ -465,10 +480,10 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const Tile tile = tile_of<CG>(groups, p, t, e);
       e = tile.e;
       // of a tile of W whose rows do not exist those of the last that do (its outputs are not stored)
-      int sfa = (tile.e * p.k_blocks * p.scale_tiles + min(tile.f * CG + static_cast<int>(rank), p.scale_tiles - 1)) * NW;
-      int sfb = (expert_scale_tile(tile.lo, tile.e, p.bn) + tile.i * p.sfb_atoms) * NW;
-      for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
-        const int blocks = min(kGroup, p.k_blocks - kb);
+      int sfa = ((tile.e * p.k_blocks + kb_first) * p.scale_tiles + min(tile.f * CG + static_cast<int>(rank), p.scale_tiles - 1)) * NW;
+      int sfb = (kb_first * p.x_scale_tiles + expert_scale_tile(tile.lo, tile.e, p.bn) + tile.i * p.sfb_atoms) * NW;
+      for (int kb = kb_first; kb < kb_end; kb += kGroup) {
+        const int blocks = min(kGroup, kb_end - kb);
         if (elect_one()) {
           ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 106);
           if (ok) {
@@ -528,14 +543,14 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
           mma<KIND, CG>(d, at + 2 * k, at + (x_off >> 4) + 2 * k, idesc | (id << 4) | (id << 29), sfa + w * 4, sfb + w * 8, !(first && k == 0));
         }
       };
-      for (int kb = 0; kb < p.k_blocks; kb += kGroup) {
+      for (int kb = kb_first; kb < kb_end; kb += kGroup) {
         // the next tile is worked out while the instructions of this one's last stages run
-        if (kb + kGroup >= p.k_blocks && t + tile_step < num_tiles) tile = tile_of<CG>(groups, p, t + tile_step, tile.e);
+        if (kb + kGroup >= kb_end && t + tile_step < num_tiles) tile = tile_of<CG>(groups, p, t + tile_step, tile.e);
         mbar_wait(full0 + 8 * s, ph, abort_flag, p.status, 103);
         if (elect_one()) {
           fence_after();
-          k_block(low, 0, kb == 0);
-          if (kb + 1 < p.k_blocks) k_block(low + block_low, 1, false);
+          k_block(low, 0, kb == kb_first);
+          if (kb + 1 < kb_end) k_block(low + block_low, 1, false);
           commit<CG>(empty0 + 8 * s);
         }
         __syncwarp();
@@ -545,7 +560,25 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       if (elect_one()) commit<CG>(smem_u32(&h->acc_full[buf]));
       __syncwarp();
     }
-  } else if (warp >= kFirstEpilogueWarp) {
+  } else if (SPLIT && warp >= kFirstEpilogueWarp) {
+    // ------------------------------------------------------------ partial sums: [row][128 lanes] floats
+    const int ew = warp - kFirstEpilogueWarp, quarter = ew & 3, set = ew >> 2;
+    if (first_tile < num_tiles) {
+      const Tile tile = tile_of<CG>(groups, p, first_tile, 0);
+      mbar_wait(smem_u32(&h->acc_full[0]), 0, abort_flag, p.status, 104);
+      __syncwarp();
+      fence_after();
+      for (int c0 = set * 16; c0 < tile.rows; c0 += 32) {
+        uint32_t v[16];
+        load_lane_columns((static_cast<uint32_t>(quarter * 32) << 16) + c0, v);
+        loads_done(v);
+        const uint32_t to = staging + c0 * 512 + (quarter * 32 + lane) * 4;
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          if (c0 + c < tile.rows) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + c * 512), "r"(v[c]) : "memory");
+      }
+    }
+  } else if (!SPLIT && warp >= kFirstEpilogueWarp) {
     // ------------------------------------------------------------ epilogue
     const int ew = warp - kFirstEpilogueWarp, quarter = ew & 3, set = ew >> 2;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
@@ -694,10 +727,51 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     }
   }
 
+  if constexpr (SPLIT) {
+    // A share of the tile's lanes (features, or gate and up features eight by eight) is this CTA's to add up.
+    __syncwarp();
+    cluster_barrier();
+    if (first_tile < num_tiles) {
+      const Tile tile = tile_of<CG>(groups, p, first_tile, 0);
+      const int lanes = 128 / p.split, quads = GATED ? lanes / 8 : lanes / 4;      // of four features
+      const float alpha = (p.x_scale ? __ldg(p.x_scale) : 1.0f) * (p.w_scale ? __ldg(p.w_scale + tile.e) : 1.0f);
+      const float* bias = p.bias ? p.bias + static_cast<long long>(tile.e) * (GATED ? 2 : 1) * p.n : nullptr;
+      const int f_first = tile.f * (GATED ? 64 : 128) + part * (GATED ? lanes / 2 : lanes);
+      for (int i = threadIdx.x; i < tile.rows * quads; i += kThreads) {
+        const int r = i / quads, q = i - r * quads;
+        const int f = f_first + 4 * q;
+        // quads of a gated tile: two of gate, two of up in turn
+        const uint32_t at = staging + r * 512 + (part * lanes + (GATED ? (q >> 1) * 16 + (q & 1) * 4 : 4 * q)) * 4;
+        float sum[GATED ? 2 : 1][4];
+#pragma unroll
+        for (int g = 0; g < (GATED ? 2 : 1); ++g)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) sum[g][k] = 0.0f;
+        for (int c = 0; c < p.split; ++c)
+#pragma unroll
+          for (int g = 0; g < (GATED ? 2 : 1); ++g) {
+            float v[4];
+            load_from_cta(at + g * 32, c, v);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) sum[g][k] += v[k];
+          }
+        T* to = static_cast<T*>(p.y) + (static_cast<long long>(tile.lo) + tile.r0 + r) * p.y_stride + f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (f + k >= p.n) break;
+          float v = fmaf(sum[0][k], alpha, bias ? __ldg(bias + f + k) : 0.0f);
+          if (GATED) v = gate(v, fmaf(sum[GATED ? 1 : 0][k], alpha, bias ? __ldg(bias + p.n + f + k) : 0.0f));
+          if constexpr (sizeof(T) == 4) to[k] = v;
+          else reinterpret_cast<uint16_t*>(to)[k] = static_cast<uint16_t>(pack2<T>(v, v));
+        }
+      }
+    }
+  }
+
   // ---------------------------------------------------------------- common exit
   __syncwarp();
   fence_before();
-  if constexpr (CG == 1) __syncthreads();
+  if constexpr (CG == 1 && !SPLIT) __syncthreads();
   else cluster_barrier();     // the other CTA's instructions and arrivals reach into this one's memory
   if (*abort_flag) {          // copies in flight land within microseconds
     const long long began = clock64();
@@ -738,9 +812,9 @@ bool encode_scales(CUtensorMap* map, const void* base, uint64_t tiles, uint32_t 
   const cuuint32_t box[2] = {kScaleTile / 4, box_tiles};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
-template <int KIND, int CG, bool GATED, typename T>
+template <int KIND, int CG, bool GATED, bool SPLIT, typename T>
 cudaError_t start(const Maps& maps, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
-  auto* kernel = block_linear_kernel<KIND, CG, GATED, T>;
+  auto* kernel = block_linear_kernel<KIND, CG, GATED, SPLIT, T>;
   // once per GPU (a repeated setting by racing first calls does no harm): the attribute costs a call a microsecond of the host's time
   static std::atomic<bool> ready[kMaxDevices];
   int dev = 0;
@@ -758,9 +832,9 @@ cudaError_t start(const Maps& maps, const LinearParams& p, int grid, size_t smem
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (CG > 1) {
+  if (CG > 1 || SPLIT) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = CG;
+    attr[n].val.clusterDim.x = SPLIT ? p.split : CG;
     attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
     ++n;
   }
@@ -773,16 +847,17 @@ cudaError_t start(const Maps& maps, const LinearParams& p, int grid, size_t smem
   cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, maps, p);
 }
-template <int KIND, int CG, bool GATED>
+template <int KIND, int CG, bool GATED, bool SPLIT>
 cudaError_t start_typed(const Maps& m, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
-  if (p.y_dtype == B2VX_DT_FLOAT32) return start<KIND, CG, GATED, float>(m, p, grid, smem, s);
-  if (p.y_dtype == B2VX_DT_FLOAT16) return start<KIND, CG, GATED, __half>(m, p, grid, smem, s);
-  return start<KIND, CG, GATED, __nv_bfloat16>(m, p, grid, smem, s);
+  if (p.y_dtype == B2VX_DT_FLOAT32) return start<KIND, CG, GATED, SPLIT, float>(m, p, grid, smem, s);
+  if (p.y_dtype == B2VX_DT_FLOAT16) return start<KIND, CG, GATED, SPLIT, __half>(m, p, grid, smem, s);
+  return start<KIND, CG, GATED, SPLIT, __nv_bfloat16>(m, p, grid, smem, s);
 }
 template <int KIND>
 cudaError_t start_kind(const Maps& m, const LinearParams& p, int cg, int gated, int grid, size_t smem, cudaStream_t s) {
-  if (cg == 2) return gated ? start_typed<KIND, 2, true>(m, p, grid, smem, s) : start_typed<KIND, 2, false>(m, p, grid, smem, s);
-  return gated ? start_typed<KIND, 1, true>(m, p, grid, smem, s) : start_typed<KIND, 1, false>(m, p, grid, smem, s);
+  if (cg == 2) return gated ? start_typed<KIND, 2, true, false>(m, p, grid, smem, s) : start_typed<KIND, 2, false, false>(m, p, grid, smem, s);
+  if (p.split > 1) return gated ? start_typed<KIND, 1, true, true>(m, p, grid, smem, s) : start_typed<KIND, 1, false, true>(m, p, grid, smem, s);
+  return gated ? start_typed<KIND, 1, true, false>(m, p, grid, smem, s) : start_typed<KIND, 1, false, false>(m, p, grid, smem, s);
 }
 
 }  // namespace
@@ -809,7 +884,18 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   p.block_bytes = (p.block_bytes + 1023u) & ~1023u;
   const int elem = a.y_dtype == B2VX_DT_FLOAT32 ? 4 : 2;
   p.y_vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride * elem % 16 == 0;
-  const int behind = kStagingBytes + static_cast<int>(sizeof(Header)) + static_cast<int>(sizeof(Group)) * (a.experts + 1) + 1024;   // and the ring's alignment
+  // CTAs to a tile's K: as many of 8, 4, 2 as leave every tile a cluster of its own in one round and every CTA a stage of K.
+  const long long most = (a.rows / p.bn + groups) * p.feature_tiles;
+  p.split = 1;
+  for (int c = 8; cg == 1 && c > 1 && p.split == 1; c /= 2) {
+    const int blocks = (p.k_blocks + c - 1) / c;
+    if (most * c <= a.sm_count && blocks >= kGroup && (c - 1) * blocks < p.k_blocks) {
+      p.split = c;
+      p.split_blocks = blocks;
+    }
+  }
+  p.staging_bytes = p.split > 1 ? p.bn * 512 : kStagingBytes;
+  const int behind = static_cast<int>(p.staging_bytes) + static_cast<int>(sizeof(Header)) + static_cast<int>(sizeof(Group)) * (a.experts + 1) + 1024;   // and the ring's alignment
   const int room = static_cast<int>((kSmemBudget - behind) / p.block_bytes);      // k-blocks that fit
   p.stages = std::min(kMaxStages, room / kGroup);
   p.stage_bytes = kGroup * p.block_bytes;
@@ -847,8 +933,7 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
     *why = "tensor map refused";
     return cudaErrorInvalidValue;
   }
-  const long long most = (a.rows / p.bn + groups) * p.feature_tiles;
-  const int grid = static_cast<int>(std::max<long long>(1, std::min<long long>(a.sm_count / cg, most))) * cg;
+  const int grid = p.split > 1 ? static_cast<int>(most) * p.split : static_cast<int>(std::max<long long>(1, std::min<long long>(a.sm_count / cg, most))) * cg;
   if (a.format == 0) return start_kind<0>(maps, p, cg, a.gated, grid, smem, s);
   if (a.format == B2VX_FP4_BLOCK32) return start_kind<B2VX_FP4_BLOCK32>(maps, p, cg, a.gated, grid, smem, s);
   return start_kind<B2VX_FP4_BLOCK16>(maps, p, cg, a.gated, grid, smem, s);
