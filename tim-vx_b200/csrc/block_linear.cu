@@ -22,8 +22,8 @@
 // once for 256 features.  No load is multicast: every CTA fetches its own operands; the loads of both announce themselves on
 // the first one's barrier.
 //
-// SPLIT (few tiles): the CTAs of a cluster share one tile's K.  Each leaves its partial sums in its shared memory, and after a barrier of the
-// cluster each adds up a share of the tile's features over all of them, in the order of the CTAs.  (One row through 4096 x 4096 has
+// SPLIT (few tiles): the CTAs of a cluster share one tile's K.  Each writes its partial sums into the shared memory of the CTA that a share of
+// the tile's features belongs to, and after a barrier of the cluster that one adds them up, in the order of the CTAs.  (One row through 4096 x 4096 has
 // 32 tiles: 32 SMs draw their 128 rows of W at 65 bytes a clock, a fifth of what memory gives.)
 //
 // Every wait is bounded as in gemm_tc.cu: on a time-out the CTA records a code and leaves through its common exit.
@@ -113,11 +113,11 @@ __device__ __forceinline__ uint32_t in_first_cta(uint32_t addr) {
   asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
   return r;
 }
-// Four floats at the same place in CTA `cta`'s shared memory.
-__device__ __forceinline__ void load_from_cta(uint32_t addr, int cta, float (&v)[4]) {
-  uint32_t a;
-  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(cta));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(a) : "memory");
+// The same address in CTA `cta`.
+__device__ __forceinline__ uint32_t in_cta(uint32_t addr, int cta) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(cta));
+  return r;
 }
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -396,8 +396,8 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     if (lane == 0) h->num_tiles = total;
   }
   fence_before();
-  if constexpr (CG == 1) __syncthreads();
-  else cluster_barrier();       // the other CTA's barriers are ready, too
+  if constexpr (CG == 1 && !SPLIT) __syncthreads();
+  else cluster_barrier();       // the other CTAs have started and their barriers are ready, too
   fence_after();
   const int num_tiles = h->num_tiles;
 
@@ -561,10 +561,12 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       __syncwarp();
     }
   } else if (SPLIT && warp >= kFirstEpilogueWarp) {
-    // ------------------------------------------------------------ partial sums: [row][128 lanes] floats
+    // ------------------------------------------------------------ partial sums, to the CTA whose lanes they are: [CTA][row][its lanes]
     const int ew = warp - kFirstEpilogueWarp, quarter = ew & 3, set = ew >> 2;
     if (first_tile < num_tiles) {
       const Tile tile = tile_of<CG>(groups, p, first_tile, 0);
+      const int width = 128 / p.split, l = quarter * 32 + lane, owner = l / width;
+      const uint32_t to = in_cta(staging + (part * tile.rows * width + l - owner * width) * 4, owner), step = width * 4;
       mbar_wait(smem_u32(&h->acc_full[0]), 0, abort_flag, p.status, 104);
       __syncwarp();
       fence_after();
@@ -572,10 +574,9 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
         uint32_t v[16];
         load_lane_columns((static_cast<uint32_t>(quarter * 32) << 16) + c0, v);
         loads_done(v);
-        const uint32_t to = staging + c0 * 512 + (quarter * 32 + lane) * 4;
 #pragma unroll
         for (int c = 0; c < 16; ++c)
-          if (c0 + c < tile.rows) asm volatile("st.shared.b32 [%0], %1;" ::"r"(to + c * 512), "r"(v[c]) : "memory");
+          if (c0 + c < tile.rows) asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(to + (c0 + c) * step), "r"(v[c]) : "memory");
       }
     }
   } else if (!SPLIT && warp >= kFirstEpilogueWarp) {
@@ -728,42 +729,53 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   }
 
   if constexpr (SPLIT) {
-    // A share of the tile's lanes (features, or gate and up features eight by eight) is this CTA's to add up.
+    // This CTA's share of the tile's lanes (features, or gate and up features eight by eight): four features a thread.
+    constexpr int G = GATED ? 2 : 1;
+    Tile tile = {};
+    if (first_tile < num_tiles) tile = tile_of<CG>(groups, p, first_tile, 0);
+    const int width = 128 / p.split, quads = width / (4 * G), n = tile.rows * quads;
+    const int f_first = tile.f * (128 / G) + part * (width / G);
+    const float* bias = p.bias ? p.bias + static_cast<long long>(tile.e) * G * p.n : nullptr;
+    // what comes from global memory is asked for before the barrier
+    const float alpha = (p.x_scale ? __ldg(p.x_scale) : 1.0f) * (p.w_scale ? __ldg(p.w_scale + tile.e) : 1.0f);
+    float b[G][4];
+#pragma unroll
+    for (int g = 0; g < G; ++g)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int f = f_first + 4 * (static_cast<int>(threadIdx.x) % quads) + k;
+        b[g][k] = bias && f < p.n ? __ldg(bias + g * p.n + f) : 0.0f;
+      }
     __syncwarp();
     cluster_barrier();
-    if (first_tile < num_tiles) {
-      const Tile tile = tile_of<CG>(groups, p, first_tile, 0);
-      const int lanes = 128 / p.split, quads = GATED ? lanes / 8 : lanes / 4;      // of four features
-      const float alpha = (p.x_scale ? __ldg(p.x_scale) : 1.0f) * (p.w_scale ? __ldg(p.w_scale + tile.e) : 1.0f);
-      const float* bias = p.bias ? p.bias + static_cast<long long>(tile.e) * (GATED ? 2 : 1) * p.n : nullptr;
-      const int f_first = tile.f * (GATED ? 64 : 128) + part * (GATED ? lanes / 2 : lanes);
-      for (int i = threadIdx.x; i < tile.rows * quads; i += kThreads) {
-        const int r = i / quads, q = i - r * quads;
-        const int f = f_first + 4 * q;
-        // quads of a gated tile: two of gate, two of up in turn
-        const uint32_t at = staging + r * 512 + (part * lanes + (GATED ? (q >> 1) * 16 + (q & 1) * 4 : 4 * q)) * 4;
-        float sum[GATED ? 2 : 1][4];
+    // kThreads is a multiple of quads (16, 32, 64 or half of that), so a thread keeps its features
+    const int q = threadIdx.x % quads, f = f_first + 4 * q;
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const int r = i / quads;
+      // quads of a gated tile: two of gate, two of up in turn
+      const uint32_t at = staging + (r * width + (GATED ? (q >> 1) * 16 + (q & 1) * 4 : 4 * q)) * 4;
+      float sum[G][4];
 #pragma unroll
-        for (int g = 0; g < (GATED ? 2 : 1); ++g)
+      for (int g = 0; g < G; ++g)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) sum[g][k] = 0.0f;
-        for (int c = 0; c < p.split; ++c)
+        for (int k = 0; k < 4; ++k) sum[g][k] = 0.0f;
+      for (int c = 0; c < p.split; ++c)
 #pragma unroll
-          for (int g = 0; g < (GATED ? 2 : 1); ++g) {
-            float v[4];
-            load_from_cta(at + g * 32, c, v);
+        for (int g = 0; g < G; ++g) {
+          float v[4];
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3])
+                       : "r"(at + c * tile.rows * width * 4 + g * 32) : "memory");
 #pragma unroll
-            for (int k = 0; k < 4; ++k) sum[g][k] += v[k];
-          }
-        T* to = static_cast<T*>(p.y) + (static_cast<long long>(tile.lo) + tile.r0 + r) * p.y_stride + f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (f + k >= p.n) break;
-          float v = fmaf(sum[0][k], alpha, bias ? __ldg(bias + f + k) : 0.0f);
-          if (GATED) v = gate(v, fmaf(sum[GATED ? 1 : 0][k], alpha, bias ? __ldg(bias + p.n + f + k) : 0.0f));
-          if constexpr (sizeof(T) == 4) to[k] = v;
-          else reinterpret_cast<uint16_t*>(to)[k] = static_cast<uint16_t>(pack2<T>(v, v));
+          for (int k = 0; k < 4; ++k) sum[g][k] += v[k];
         }
+      T* to = static_cast<T*>(p.y) + (static_cast<long long>(tile.lo) + tile.r0 + r) * p.y_stride + f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (f + k >= p.n) break;
+        float v = fmaf(sum[0][k], alpha, b[0][k]);
+        if (GATED) v = gate(v, fmaf(sum[G - 1][k], alpha, b[G - 1][k]));
+        if constexpr (sizeof(T) == 4) to[k] = v;
+        else reinterpret_cast<uint16_t*>(to)[k] = static_cast<uint16_t>(pack2<T>(v, v));
       }
     }
   }
@@ -771,8 +783,8 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   // ---------------------------------------------------------------- common exit
   __syncwarp();
   fence_before();
-  if constexpr (CG == 1 && !SPLIT) __syncthreads();
-  else cluster_barrier();     // the other CTA's instructions and arrivals reach into this one's memory
+  if constexpr (CG == 1) __syncthreads();
+  else asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");   // the other CTA's instructions and arrivals reach into this one's memory; stores need not be waited for
   if (*abort_flag) {          // copies in flight land within microseconds
     const long long began = clock64();
     while (clock64() - began < 200000) {}
