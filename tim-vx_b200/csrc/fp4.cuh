@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "b2vx.h"
 
@@ -75,8 +76,30 @@ struct TensorScale {
   float over_g = 1.0f;     // 1 / g
   float over_6g = 1.0f;    // 1 / (6 g)
   bool ok = true;
+  uint32_t near = 3;       // below
 };
-template <int FORMAT>
+// Numbers over s g are rounded to codes from an approximate quotient, which can only go wrong next to a border between two codes.  For
+// 16-bit numbers the places where that can happen are few and known beforehand: a number lies within 2^-19 of a border b s g only
+// if b s g itself is that close to a number of the 16-bit type, which depends on the mantissas of b (1, 1.25, 1.5 or 1.75), s (eight
+// of them) and g alone.  Lane i works out, for the i-th mantissa of s, whether such numbers lie below their border (bit 0: a
+// quotient that is a little too small is right), above it (bit 1: one a little too large) or on it (both bits).
+template <typename T>
+__device__ __forceinline__ uint32_t near_borders(float g) {
+  if (sizeof(T) == 4) return 3u;
+  const float gn = __uint_as_float((__float_as_uint(g) & 0x7fffffu) | 0x3f800000u);
+  uint32_t near = 0;
+#pragma unroll
+  for (int m = 4; m < 8; ++m) {
+    const float p = 0.25f * m * (1.0f + 0.125f * (threadIdx.x & 7));      // few bits: exact
+    float v;
+    if constexpr (std::is_same<T, __half>::value) v = __half2float(__float2half_rn(p * gn));
+    else v = __bfloat162float(__float2bfloat16_rn(p * gn));
+    const float r = fmaf(p, gn, -v);                                      // its sign is exact
+    if (fabsf(r) <= 0x1p-19f * v) near |= r > 0.0f ? 1u : (r < 0.0f ? 2u : 3u);
+  }
+  return near;
+}
+template <int FORMAT, typename T>
 __device__ __forceinline__ TensorScale tensor_scale(const float* p) {
   TensorScale t;
   if (FORMAT == B2VX_FP4_BLOCK16) {
@@ -86,6 +109,7 @@ __device__ __forceinline__ TensorScale tensor_scale(const float* p) {
     t.g = g * t.lift;
     t.over_g = 1.0f / t.g;
     t.over_6g = 1.0f / (6.0f * t.g);
+    t.near = near_borders<T>(t.g);
   }
   return t;
 }
@@ -95,9 +119,7 @@ __device__ __forceinline__ uint32_t e2m1_codes_times(const float* v, float f) {
   return e2m1_codes(r);
 }
 // Where a little less and a little more than a quotient round to different codes: the border between the two decides, by a comparison
-// that is exact, since border * s has few bits and the fused product with g is rounded only after the subtraction.  (Numbers of few
-// bits over a scale of few bits often lie on a border or next to it: with a tensor scale of 1 / 56, 16-bit numbers in one block
-// of twelve.)  diff: the nibbles that differ; number(i): the lane's i-th number.
+// that is exact, since border * s has few bits and the fused product with g is rounded only after the subtraction.  diff: the nibbles that differ; number(i): the lane's i-th number.
 template <typename F>
 __device__ __forceinline__ uint32_t settle_codes(uint32_t codes, uint32_t diff, float s, float g, float lift, F number) {
   while (diff) {
@@ -145,11 +167,15 @@ __device__ __forceinline__ uint2 quantize_16(const float (&v)[16], uint32_t top,
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(over_s) : "f"(s));   // off by 2^-23; s = 0 is dealt with below
   // The numbers over s g: the approximate reciprocal, two products and 1 / g are off by less than 2^-21 together.
   const float inv = over_s * t.over_g * t.lift, less = inv * kLess, more = inv * kMore;
-  uint2 codes = make_uint2(e2m1_codes_times(v, less), e2m1_codes_times(v + 8, less));
-  const uint2 up = make_uint2(e2m1_codes_times(v, more), e2m1_codes_times(v + 8, more));
-  if ((codes.x != up.x || codes.y != up.y) && byte != 0) {
-    codes.x = settle_codes(codes.x, codes.x ^ up.x, s, t.g, t.lift, number);
-    codes.y = settle_codes(codes.y, codes.y ^ up.y, s, t.g, t.lift, [&](int i) { return number(8 + i); });
+  const uint32_t near = __shfl_sync(0xffffffffu, t.near, (__float_as_uint(s) >> 20) & 7);
+  const float f = near == 2u ? more : less;
+  uint2 codes = make_uint2(e2m1_codes_times(v, f), e2m1_codes_times(v + 8, f));
+  if (near == 3u) {
+    const uint2 up = make_uint2(e2m1_codes_times(v, more), e2m1_codes_times(v + 8, more));
+    if ((codes.x != up.x || codes.y != up.y) && byte != 0) {
+      codes.x = settle_codes(codes.x, codes.x ^ up.x, s, t.g, t.lift, number);
+      codes.y = settle_codes(codes.y, codes.y ^ up.y, s, t.g, t.lift, [&](int i) { return number(8 + i); });
+    }
   }
   if (byte == 0) codes = make_uint2(0u, 0u);                  // every number rounds to zero
   if (top >= 0x7f800000u || !t.ok) {

@@ -37,16 +37,31 @@ struct alignas(16) Sixteen {
   T v[16];
 };
 template <typename T, bool VEC>
-__device__ __forceinline__ Sixteen<T> load_16(const T* row, int c, int k) {
+__device__ __forceinline__ Sixteen<T> load_16(const T* row, int c, int k, uint4* staging, int lane) {
   Sixteen<T> t;
   constexpr int W = sizeof(t) / 16;
   if (VEC && c + 16 <= k) {
     const uint4* src = reinterpret_cast<const uint4*>(row + c);
 #pragma unroll
     for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(&t)[i] = __ldg(src + i);
-  } else {
+  } else if (VEC) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) t.v[i] = c + i < k ? row[c + i] : from_float<T>(0.0f);
+  } else {
+    // neighbouring numbers by neighbouring lanes, handed over through the warp's staging memory: each lane's sixteen numbers and 16 bytes
+    // more, so that eight lanes' 16-byte pieces fall into different banks
+    constexpr int kPitch = 16 + 16 / sizeof(T);
+    T* s = reinterpret_cast<T*>(staging);
+    const int first = c - lane * 16;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int at = i * 32 + lane;
+      s[(at >> 4) * kPitch + (at & 15)] = first + at < k ? row[first + at] : from_float<T>(0.0f);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(&t)[i] = staging[lane * (W + 1) + i];
   }
   return t;
 }
@@ -100,9 +115,11 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArg
   constexpr int B = fp4_block(FORMAT), LANES = B / 16, PER = scale_words_per_stage(FORMAT);   // lanes to a block, words to a k-block
   pdl_wait();
   pdl_trigger();   // after the wait: a product behind this kernel may read its weights before its own wait
+  __shared__ uint4 all_staging[VEC ? 1 : kWarps * 32 * (static_cast<int>(sizeof(Sixteen<T>)) / 16 + 1)];
+  uint4* staging = all_staging + (VEC ? 0 : (threadIdx.x >> 5) * 32 * (sizeof(Sixteen<T>) / 16 + 1));
   const int lane = threadIdx.x & 31;
   const uint32_t warps = gridDim.x * kWarps, units = static_cast<uint32_t>(a.rows) * split;
-  const TensorScale scale = tensor_scale<FORMAT>(a.tensor_scale);
+  const TensorScale scale = tensor_scale<FORMAT, T>(a.tensor_scale);
   const int k = static_cast<int>(a.k), k32 = (k + 31) / 32 * 32, blocks = (k + B - 1) / B;
   const T* x = static_cast<const T*>(a.x);
   for (uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5); unit < units; unit += warps) {
@@ -114,13 +131,13 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArg
     const int k_here = there ? k : 0;
     uint8_t* codes_row = a.codes + row * a.codes_pitch;
     int c = part * kChunk + lane * 16;
-    Sixteen<T> t = load_16<T, VEC>(from, c, k_here);
+    Sixteen<T> t = load_16<T, VEC>(from, c, k_here, staging, lane);
     uint8_t* tile = PACKED ? packed_place<FORMAT>(a, row, lane) : nullptr;
     for (int chunk = part; chunk < chunks; chunk += split) {
       // the next chunk is asked for before this one is worked on
       const int c_next = c + split * kChunk;
       Sixteen<T> next = t;
-      if (chunk + split < chunks) next = load_16<T, VEC>(from, c_next, k_here);
+      if (chunk + split < chunks) next = load_16<T, VEC>(from, c_next, k_here, staging, lane);
       float v[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = to_float(t.v[i]);
@@ -175,11 +192,13 @@ __global__ void __launch_bounds__(kWarps * 32) gather_fp4_kernel(const QuantizeA
 }
 
 // Rows of values: `split` warps share a row as above, sixteen columns a lane and step, two steps asked for at once.
-template <typename T, int FORMAT>
+template <typename T, int FORMAT, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
                                                                  const float* tensor_scale, uint32_t rows, int k, T* y, long long y_stride,
-                                                                 int chunks, int split, int vec) {
-  constexpr int B = fp4_block(FORMAT), U = 2;
+                                                                 int chunks, int split) {
+  constexpr int B = fp4_block(FORMAT), U = 2, W = sizeof(Sixteen<T>) / 16;
+  __shared__ uint4 all_staging[VEC ? 1 : kWarps * 32 * (W + 1)];
+  uint4* staging = all_staging + (VEC ? 0 : (threadIdx.x >> 5) * 32 * (W + 1));
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31;
@@ -202,7 +221,7 @@ __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* 
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int c = (chunk + u * split) * kChunk + lane * 16;
-        if (c >= k) break;
+        if (c - lane * 16 >= k) break;
         const float s = scale_value<FORMAT>(byte[u]);
         float v[16];
         e2m1_values(word[u][0], v);
@@ -210,13 +229,26 @@ __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* 
         Sixteen<T> out;
 #pragma unroll
         for (int j = 0; j < 16; ++j) out.v[j] = from_float<T>(FORMAT == B2VX_FP4_BLOCK16 ? v[j] * s * g : v[j] * s);
-        if (vec && c + 16 <= k) {
+        if (VEC && c + 16 <= k) {
 #pragma unroll
-          for (int i = 0; i < static_cast<int>(sizeof(out)) / 16; ++i) reinterpret_cast<uint4*>(to + c)[i] = reinterpret_cast<const uint4*>(&out)[i];
-        } else {
+          for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(to + c)[i] = reinterpret_cast<const uint4*>(&out)[i];
+        } else if (VEC) {
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             if (c + j < k) to[c + j] = out.v[j];
+        } else {       // as load_16, the other way
+          constexpr int kPitch = 16 + 16 / sizeof(T);
+          const T* values = reinterpret_cast<const T*>(staging);
+          const int first = c - lane * 16;
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < W; ++i) staging[lane * (W + 1) + i] = reinterpret_cast<const uint4*>(&out)[i];
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int at = i * 32 + lane;
+            if (first + at < k) to[first + at] = values[(at >> 4) * kPitch + (at & 15)];
+          }
         }
       }
     }
@@ -302,10 +334,11 @@ cudaError_t dequantize(const uint8_t* codes, long long codes_pitch, const uint8_
                        long long rows, long long k, void* y, long long y_stride, cudaStream_t s) {
   const int chunks = static_cast<int>((k + kChunk - 1) / kChunk);
   const int split = split_of(rows, chunks);
-  const int vec = reinterpret_cast<uintptr_t>(y) % 16 == 0 && (y_stride * sizeof(T)) % 16 == 0;
-  auto* kernel = format == B2VX_FP4_BLOCK32 ? dequantize_kernel<T, B2VX_FP4_BLOCK32> : dequantize_kernel<T, B2VX_FP4_BLOCK16>;
+  const bool vec = reinterpret_cast<uintptr_t>(y) % 16 == 0 && (y_stride * sizeof(T)) % 16 == 0;
+  auto* kernel = format == B2VX_FP4_BLOCK32 ? (vec ? dequantize_kernel<T, B2VX_FP4_BLOCK32, true> : dequantize_kernel<T, B2VX_FP4_BLOCK32, false>)
+                                            : (vec ? dequantize_kernel<T, B2VX_FP4_BLOCK16, true> : dequantize_kernel<T, B2VX_FP4_BLOCK16, false>);
   return launch_pdl(kernel, dim3(blocks_for(rows * split, kWarps)), dim3(kWarps * 32), 0, s, codes, codes_pitch, scales, scales_pitch, tensor_scale,
-                    static_cast<uint32_t>(rows), static_cast<int>(k), static_cast<T*>(y), y_stride, chunks, split, vec);
+                    static_cast<uint32_t>(rows), static_cast<int>(k), static_cast<T*>(y), y_stride, chunks, split);
 }
 
 }  // namespace
