@@ -77,6 +77,39 @@ void* tensor_scale(PyObject* o, long format, long count, const at::Device& devic
   return dense(o, what, at::kFloat, t.sizes(), device);
 }
 at::Tensor empty(at::IntArrayRef shape, at::ScalarType type, const at::Device& device) { return at::empty(shape, at::TensorOptions().dtype(type).device(device)); }
+// Several dense tensors in one allocation, each on its own multiple of 256 bytes (a call of the allocator costs more than a view).
+class Carver {
+ public:
+  explicit Carver(const at::Device& device) : device_(device) {}
+  // Adds a tensor; returns its number.
+  int add(at::IntArrayRef shape, at::ScalarType type) {
+    int64_t n = 1;
+    for (int64_t d : shape) n *= d;
+    parts_[count_] = {bytes_, type};
+    bytes_ += (n * static_cast<int64_t>(c10::elementSize(type)) + 255) / 256 * 256;
+    return count_++;
+  }
+  at::Tensor take(int i, at::IntArrayRef shape) {
+    if (!storage_.defined()) storage_ = empty({bytes_}, at::kByte, device_);
+    const Part& p = parts_[i];
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(storage_.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(p.type));
+    c10::TensorImpl* impl = t.unsafeGetTensorImpl();
+    impl->set_storage_offset(p.at / static_cast<int64_t>(c10::elementSize(p.type)));
+    impl->set_sizes_contiguous(shape);
+    return t;
+  }
+
+ private:
+  struct Part {
+    int64_t at;
+    at::ScalarType type;
+  };
+  at::Device device_;
+  at::Tensor storage_;
+  Part parts_[8] = {};
+  int count_ = 0;
+  int64_t bytes_ = 0;
+};
 at::Tensor output(PyObject* out, at::IntArrayRef shape, at::ScalarType type, const at::Device& device) {
   if (out == Py_None) return empty(shape, type, device);
   const at::Tensor& t = tensor(out, "out");
@@ -127,7 +160,11 @@ PyObject* quantize(PyObject* const* a) {
   void* scale = tensor_scale(a[2], format, 1, device, "scale");
   void* index = dense(a[3], "row_index", at::kInt, {rows}, device);
   Call call(device);
-  at::Tensor codes = empty({rows, (k + 31) / 32 * 16}, at::kByte, device), scales = empty({rows, (k + block - 1) / block}, at::kByte, device);
+  const int64_t codes_shape[2] = {rows, (k + 31) / 32 * 16}, scales_shape[2] = {rows, (k + block - 1) / block};
+  Carver carver(device);
+  carver.add(codes_shape, at::kByte);
+  carver.add(scales_shape, at::kByte);
+  at::Tensor codes = carver.take(0, codes_shape), scales = carver.take(1, scales_shape);
   const b2vx_fp4_quantize_desc d = {static_cast<int32_t>(format), dtype_code(x.scalar_type()), static_cast<uint64_t>(x.size(0)), static_cast<uint64_t>(rows),
                                     static_cast<uint64_t>(k), stride, static_cast<uint64_t>(codes.size(1)), static_cast<uint64_t>(scales.size(1))};
   call(b2vx_fp4_quantize_noalloc(&d, x.data_ptr(), static_cast<const int32_t*>(index), static_cast<const float*>(scale), codes.data_ptr(), scales.data_ptr(),
@@ -241,11 +278,16 @@ PyObject* route(PyObject* const* a) {
   const b2vx_route_desc d = {dtype_code(logits.scalar_type()), normalize != 0, static_cast<uint32_t>(experts), static_cast<uint32_t>(top_k), static_cast<uint64_t>(tokens), stride};
   size_t bytes = 0;
   call(b2vx_route_workspace_size_noalloc(&d, &bytes, call.err, sizeof(call.err)));
-  at::Tensor workspace = empty({static_cast<int64_t>(bytes)}, at::kByte, device);
-  at::Tensor ids = empty({tokens, top_k}, at::kInt, device), weights = empty({tokens, top_k}, at::kFloat, device), offsets = empty({experts + 1}, at::kInt, device),
-             row_index = empty({tokens * top_k}, at::kInt, device), slots = empty({tokens, top_k}, at::kInt, device);
+  const int64_t pairs[2] = {tokens, top_k}, rows[1] = {tokens * top_k}, starts[1] = {experts + 1}, work[1] = {static_cast<int64_t>(bytes)};
+  at::Tensor workspace;
+  if (bytes) workspace = empty(work, at::kByte, device);
+  Carver carver(device);
+  for (at::ScalarType type : {at::kInt, at::kFloat, at::kInt}) carver.add(pairs, type);
+  carver.add(rows, at::kInt);
+  carver.add(starts, at::kInt);
+  at::Tensor ids = carver.take(0, pairs), weights = carver.take(1, pairs), slots = carver.take(2, pairs), row_index = carver.take(3, rows), offsets = carver.take(4, starts);
   call(b2vx_route_noalloc(&d, logits.data_ptr(), ids.data_ptr<int32_t>(), weights.data_ptr<float>(), offsets.data_ptr<int32_t>(), row_index.data_ptr<int32_t>(),
-                          slots.data_ptr<int32_t>(), workspace.data_ptr(), bytes, call.stream, call.err, sizeof(call.err)));
+                          slots.data_ptr<int32_t>(), bytes ? workspace.data_ptr() : nullptr, bytes, call.stream, call.err, sizeof(call.err)));
   PyObject* r = PyTuple_New(5);
   PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(ids)));
   PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(weights)));

@@ -8,7 +8,7 @@
     combine_experts                 the weighted sum of each token's expert rows
 
 Work is queued on the current stream of the tensors' device and nothing waits for it.  Outputs and workspaces come from torch's allocator
-(give ``out`` for an output of your own).  Refused arguments raise pyb2vx.B2vxError with the library's message, tensors of a wrong type,
+(give ``out`` for an output of your own; what quantize_fp4 and route_experts return shares one allocation).  Refused arguments raise pyb2vx.B2vxError with the library's message, tensors of a wrong type,
 shape or device raise ValueError; nothing is launched then.  Tensors whose last dimension is contiguous are used where they
 lie; a bias, scale or index tensor has to be contiguous.
 """
