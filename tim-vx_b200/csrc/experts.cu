@@ -30,32 +30,55 @@ __device__ __forceinline__ float as_float(T v) {
   else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
   else return __bfloat162float(v);
 }
-// Order of floats as unsigned numbers; NaN counts as -infinity, -0 as 0.
+// Order of floats as unsigned numbers; NaN counts as -infinity, -0 as 0.  A key above 0 stands for a logit that can be chosen: of 32-bit
+// logits their order, of 16-bit ones their order in the upper half and 65535 minus the expert in the lower, so that one maximum
+// finds both the largest logit and, among equals, the lowest expert.
 __device__ __forceinline__ uint32_t order_of(float v) {
   if (!(v == v)) v = -__int_as_float(0x7f800000);
   const uint32_t b = __float_as_uint(v + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-__device__ __forceinline__ float from_order(uint32_t u) { return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u); }
+template <typename T>
+__device__ __forceinline__ uint32_t key_of(T v, int e) {
+  if constexpr (sizeof(T) == 4) {
+    return order_of(v);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const float f = as_float(v) + 0.0f;
+    const uint32_t b = f == f ? __half_as_ushort(__float2half_rn(f)) : 0xfc00u;   // exact
+    return ((b & 0x8000u ? ~b : b | 0x8000u) << 16) | (0xffffu - e);
+  } else {
+    return (order_of(as_float(v)) & 0xffff0000u) | (0xffffu - e);                 // the lower half of a bfloat16's order is all ones or zeros
+  }
+}
+template <typename T>
+__device__ __forceinline__ float value_of(uint32_t key) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const uint32_t u = key >> 16;
+    return __half2float(__ushort_as_half(static_cast<uint16_t>(u & 0x8000u ? u & 0x7fffu : ~u)));
+  } else {
+    const uint32_t u = sizeof(T) == 4 ? key : key & 0xffff0000u;
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : (sizeof(T) == 4 ? ~u : ~u & 0xffff0000u));
+  }
+}
 
 // One token by one warp.  PER: logits a lane holds (experts / 32, rounded up).  Sets bit `bit` of the chosen experts' masks.
 template <typename T, int PER>
 __device__ __forceinline__ void choose(const T* row, long long t, int experts, int top_k, int normalize, int lane, int bit, int32_t* ids, float* weights,
                                        uint32_t* mask) {
-  uint32_t key[PER];      // 0: taken, or not there (below -infinity's)
+  uint32_t key[PER];      // 0: taken, or not there
 #pragma unroll
-  for (int j = 0; j < PER; ++j) key[j] = j * 32 + lane < experts ? order_of(as_float(row[j * 32 + lane])) : 0u;
+  for (int j = 0; j < PER; ++j) key[j] = j * 32 + lane < experts ? key_of(row[j * 32 + lane], j * 32 + lane) : 0u;
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < PER; ++j) top = max(top, key[j]);
-  const float most = from_order(__reduce_max_sync(0xffffffffu, top));
+  const float most = value_of<T>(__reduce_max_sync(0xffffffffu, top));
   const bool none = most == -__int_as_float(0x7f800000);
   float total = 0.0f;
   if (!normalize) {
 #pragma unroll
     for (int j = 0; j < PER; ++j)
       if (key[j]) {
-        const float v = from_order(key[j]);
+        const float v = value_of<T>(key[j]);
         total += v == most ? 1.0f : expf(v - most);
       }
 #pragma unroll
@@ -65,18 +88,25 @@ __device__ __forceinline__ void choose(const T* row, long long t, int experts, i
   int id = 0;
   for (int r = 0; r < top_k; ++r) {
     uint32_t best = 0;
-    int at = 0;
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (key[j] > best) { best = key[j]; at = j; }
+    for (int j = 0; j < PER; ++j) best = max(best, key[j]);
     const uint32_t all = __reduce_max_sync(0xffffffffu, best);
-    const uint32_t e = __reduce_min_sync(0xffffffffu, best == all ? static_cast<uint32_t>(at * 32 + lane) : 0xffffffffu);
+    uint32_t e;
+    if constexpr (sizeof(T) == 2) {
+      e = 0xffffu - (all & 0xffffu);
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (static_cast<uint32_t>(j * 32 + lane) == e) key[j] = 0;
+      for (int j = 0; j < PER; ++j) key[j] = key[j] == all ? 0u : key[j];
+    } else {
+      uint32_t at = 0xffffffffu;
+#pragma unroll
+      for (int j = PER - 1; j >= 0; --j) at = key[j] == all ? static_cast<uint32_t>(j * 32 + lane) : at;
+      e = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) key[j] = static_cast<uint32_t>(j * 32 + lane) == e ? 0u : key[j];
+    }
     if (lane == r) { mine = all; id = static_cast<int>(e); }
   }
-  const float v = from_order(mine);
+  const float v = value_of<T>(mine);
   const float w = none || lane >= top_k ? 0.0f : (v == most ? 1.0f : expf(v - most));
   if (normalize) {
     total = w;
@@ -149,7 +179,7 @@ __global__ void __launch_bounds__(1024) route_kernel(const T* logits, long long 
 }
 
 template <typename T, int PER>
-__global__ void __launch_bounds__(1024) choose_kernel(const T* logits, long long stride, int tokens, int experts, int top_k, int normalize, int32_t* ids,
+__global__ void __launch_bounds__(1024, PER <= 8 ? 2 : 1) choose_kernel(const T* logits, long long stride, int tokens, int experts, int top_k, int normalize, int32_t* ids,
                                                       float* weights, uint32_t* masks) {
   extern __shared__ uint32_t mask[];
   pdl_trigger();
