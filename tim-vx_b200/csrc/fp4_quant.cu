@@ -13,6 +13,9 @@ namespace b2vx {
 namespace {
 
 constexpr int kWarps = 8;
+// Blocks of a quantization kernel an SM: what 64 registers a thread leave (block16, which works longer on a chunk and asks for two ahead)
+// or 48.  8192 x 8192 16-bit numbers to block32 41 us with five, 46 with four and two chunks ahead; to block16 46 and 46 - 54.
+constexpr int quantize_blocks(int format) { return format == B2VX_FP4_BLOCK16 ? 4 : 5; }
 // Rows that several rows of an operand refer to (a token's, for each of its experts) are quantized once and then copied, where that saves
 // more than the second launch costs: measured at 8192 rows of 1408 columns taken four times each.
 constexpr long long kTwiceElements = 1 << 22;
@@ -111,7 +114,7 @@ __device__ __forceinline__ uint8_t* packed_place(const QuantizeArgs& a, uint32_t
 
 // `split` warps share a row, each taking every split-th chunk.
 template <typename T, int FORMAT, bool VEC, bool PACKED>
-__global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArgs a, int chunks, int split) {
+__global__ void __launch_bounds__(kWarps * 32, quantize_blocks(FORMAT)) quantize_kernel(const QuantizeArgs a, int chunks, int split) {
   constexpr int B = fp4_block(FORMAT), LANES = B / 16, PER = scale_words_per_stage(FORMAT);   // lanes to a block, words to a k-block
   pdl_wait();
   pdl_trigger();   // after the wait: a product behind this kernel may read its weights before its own wait
@@ -131,13 +134,15 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArg
     const int k_here = there ? k : 0;
     uint8_t* codes_row = a.codes + row * a.codes_pitch;
     int c = part * kChunk + lane * 16;
-    Sixteen<T> t = load_16<T, VEC>(from, c, k_here, staging, lane);
+    // one or two chunks are under way while one is worked on
+    constexpr bool kTwo = FORMAT == B2VX_FP4_BLOCK16 && sizeof(T) == 2;
+    const int step = split * kChunk;
+    Sixteen<T> t = load_16<T, VEC>(from, c, k_here, staging, lane), ahead = t;
+    if (kTwo && part + split < chunks) ahead = load_16<T, VEC>(from, c + step, k_here, staging, lane);
     uint8_t* tile = PACKED ? packed_place<FORMAT>(a, row, lane) : nullptr;
     for (int chunk = part; chunk < chunks; chunk += split) {
-      // the next chunk is asked for before this one is worked on
-      const int c_next = c + split * kChunk;
       Sixteen<T> next = t;
-      if (chunk + split < chunks) next = load_16<T, VEC>(from, c_next, k_here, staging, lane);
+      if (chunk + (kTwo ? 2 : 1) * split < chunks) next = load_16<T, VEC>(from, c + (kTwo ? 2 : 1) * step, k_here, staging, lane);
       float v[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = to_float(t.v[i]);
@@ -159,8 +164,9 @@ __global__ void __launch_bounds__(kWarps * 32) quantize_kernel(const QuantizeArg
       } else if (lane % LANES == 0 && c / B < blocks) {
         a.scales[row * a.scales_pitch + c / B] = static_cast<uint8_t>(byte);
       }
-      t = next;
-      c = c_next;
+      t = kTwo ? ahead : next;
+      ahead = next;
+      c += step;
     }
   }
 }
@@ -191,12 +197,13 @@ __global__ void __launch_bounds__(kWarps * 32) gather_fp4_kernel(const QuantizeA
   }
 }
 
-// Rows of values: `split` warps share a row as above, sixteen columns a lane and step, two steps asked for at once.
+// Rows of values: `split` warps share a row as above, eight columns a lane and step (whole 16-byte stores of 16-bit numbers side by side),
+// four steps asked for at once.
 template <typename T, int FORMAT, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
                                                                  const float* tensor_scale, uint32_t rows, int k, T* y, long long y_stride,
                                                                  int chunks, int split) {
-  constexpr int B = fp4_block(FORMAT), U = 2, W = sizeof(Sixteen<T>) / 16;
+  constexpr int B = fp4_block(FORMAT), U = 4, kStep = 256, W = sizeof(T) / 2, kPitch = 8 + 16 / sizeof(T);   // W: 16-byte pieces of eight numbers
   __shared__ uint4 all_staging[VEC ? 1 : kWarps * 32 * (W + 1)];
   uint4* staging = all_staging + (VEC ? 0 : (threadIdx.x >> 5) * 32 * (W + 1));
   pdl_trigger();
@@ -209,45 +216,42 @@ __global__ void __launch_bounds__(kWarps * 32) dequantize_kernel(const uint8_t* 
     const uint8_t *codes_row = codes + row * codes_pitch, *scales_row = scales + row * scales_pitch;
     T* to = y + row * y_stride;
     for (int chunk = static_cast<int>(unit - row * split); chunk < chunks; chunk += U * split) {
-      uint32_t word[U][2], byte[U];
+      uint32_t word[U], byte[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int c = (chunk + u * split) * kChunk + lane * 16;
-        const uint32_t* from = reinterpret_cast<const uint32_t*>(codes_row + c / 2);
-        word[u][0] = c < k ? __ldg(from) : 0u;
-        word[u][1] = c < k ? __ldg(from + 1) : 0u;
+        const int c = (chunk + u * split) * kStep + lane * 8;
+        word[u] = c < k ? __ldg(reinterpret_cast<const uint32_t*>(codes_row + c / 2)) : 0u;
         byte[u] = c < k ? __ldg(scales_row + c / B) : 0u;
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int c = (chunk + u * split) * kChunk + lane * 16;
-        if (c - lane * 16 >= k) break;
+        const int first = (chunk + u * split) * kStep, c = first + lane * 8;
+        if (first >= k) break;
         const float s = scale_value<FORMAT>(byte[u]);
-        float v[16];
-        e2m1_values(word[u][0], v);
-        e2m1_values(word[u][1], v + 8);
-        Sixteen<T> out;
+        float v[8];
+        e2m1_values(word[u], v);
+        struct alignas(16) {
+          T v[8];
+        } out;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) out.v[j] = from_float<T>(FORMAT == B2VX_FP4_BLOCK16 ? v[j] * s * g : v[j] * s);
-        if (VEC && c + 16 <= k) {
+        for (int j = 0; j < 8; ++j) out.v[j] = from_float<T>(FORMAT == B2VX_FP4_BLOCK16 ? v[j] * s * g : v[j] * s);
+        if (VEC && c + 8 <= k) {
 #pragma unroll
           for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(to + c)[i] = reinterpret_cast<const uint4*>(&out)[i];
         } else if (VEC) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
+          for (int j = 0; j < 8; ++j)
             if (c + j < k) to[c + j] = out.v[j];
         } else {       // as load_16, the other way
-          constexpr int kPitch = 16 + 16 / sizeof(T);
           const T* values = reinterpret_cast<const T*>(staging);
-          const int first = c - lane * 16;
           __syncwarp();
 #pragma unroll
           for (int i = 0; i < W; ++i) staging[lane * (W + 1) + i] = reinterpret_cast<const uint4*>(&out)[i];
           __syncwarp();
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 8; ++i) {
             const int at = i * 32 + lane;
-            if (first + at < k) to[first + at] = values[(at >> 4) * kPitch + (at & 15)];
+            if (first + at < k) to[first + at] = values[(at >> 3) * kPitch + (at & 7)];
           }
         }
       }
@@ -301,12 +305,12 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const uint16_t* x, lon
   }
 }
 
-int blocks_for(long long threads, int per_block) {
-  return static_cast<int>(std::max<long long>(1, std::min<long long>((threads + per_block - 1) / per_block, 148 * 5)));
+int blocks_for(long long units, int per_block, int per_sm) {
+  return static_cast<int>(std::max<long long>(1, std::min<long long>((units + per_block - 1) / per_block, 148 * per_sm)));
 }
 
-// Warps that share a row: up to as many as it has chunks, so that there are about four units of work for each warp that fits the GPU (40 an
-// SM) and an uneven last round costs little.
+// Warps that share a row: up to as many as it has chunks, so that there are about four units of work for each warp that fits the GPU and an
+// uneven last round costs little.
 int split_of(long long rows, int chunks) {
   const long long fill = 4 * 148 * 40;
   return static_cast<int>(std::max<long long>(1, std::min<long long>(chunks, fill / std::max<long long>(1, rows))));
@@ -316,7 +320,7 @@ template <typename T, int FORMAT, bool VEC>
 cudaError_t quantize(const QuantizeArgs& a, cudaStream_t s) {
   const int chunks = static_cast<int>((a.k + kChunk - 1) / kChunk);
   const int split = split_of(a.rows, chunks);
-  const int grid = blocks_for(a.rows * split, kWarps);
+  const int grid = blocks_for(a.rows * split, kWarps, quantize_blocks(FORMAT));
   if (a.scales_pitch == 0) return launch_pdl(quantize_kernel<T, FORMAT, VEC, true>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
   return launch_pdl(quantize_kernel<T, FORMAT, VEC, false>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
 }
@@ -332,12 +336,12 @@ cudaError_t quantize_format(const QuantizeArgs& a, cudaStream_t s) {
 template <typename T>
 cudaError_t dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch, const float* tensor_scale, int format,
                        long long rows, long long k, void* y, long long y_stride, cudaStream_t s) {
-  const int chunks = static_cast<int>((k + kChunk - 1) / kChunk);
-  const int split = split_of(rows, chunks);
+  const int chunks = static_cast<int>((k + 255) / 256);
+  const int split = split_of(rows, (chunks + 3) / 4);
   const bool vec = reinterpret_cast<uintptr_t>(y) % 16 == 0 && (y_stride * sizeof(T)) % 16 == 0;
   auto* kernel = format == B2VX_FP4_BLOCK32 ? (vec ? dequantize_kernel<T, B2VX_FP4_BLOCK32, true> : dequantize_kernel<T, B2VX_FP4_BLOCK32, false>)
                                             : (vec ? dequantize_kernel<T, B2VX_FP4_BLOCK16, true> : dequantize_kernel<T, B2VX_FP4_BLOCK16, false>);
-  return launch_pdl(kernel, dim3(blocks_for(rows * split, kWarps)), dim3(kWarps * 32), 0, s, codes, codes_pitch, scales, scales_pitch, tensor_scale,
+  return launch_pdl(kernel, dim3(blocks_for(rows * split, kWarps, 6)), dim3(kWarps * 32), 0, s, codes, codes_pitch, scales, scales_pitch, tensor_scale,
                     static_cast<uint32_t>(rows), static_cast<int>(k), static_cast<T*>(y), y_stride, chunks, split);
 }
 
@@ -365,7 +369,7 @@ cudaError_t launch_fp4_operand(const QuantizeArgs& a, void* between, cudaStream_
   cudaError_t e = launch_fp4_quantize(once, s);
   if (e != cudaSuccess) return e;
   auto* kernel = a.format == B2VX_FP4_BLOCK32 ? gather_fp4_kernel<B2VX_FP4_BLOCK32> : gather_fp4_kernel<B2VX_FP4_BLOCK16>;
-  return launch_pdl(kernel, dim3(blocks_for(a.rows, kWarps)), dim3(kWarps * 32), 0, s, a, static_cast<const uint8_t*>(once.codes),
+  return launch_pdl(kernel, dim3(blocks_for(a.rows, kWarps, 8)), dim3(kWarps * 32), 0, s, a, static_cast<const uint8_t*>(once.codes),
                     static_cast<const uint8_t*>(once.scales), once.scales_pitch);
 }
 cudaError_t launch_fp4_dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
@@ -379,14 +383,14 @@ cudaError_t launch_fp4_pack_scales(const uint8_t* scales, int format, long long 
                                    cudaStream_t s) {
   const long long blocks = (k + fp4_block(format) - 1) / fp4_block(format), words = scale_words(k, format);
   const long long total = static_cast<long long>(packed_scale_bytes(matrices, n, gated, k, format) / 4);
-  return launch_pdl(pack_scales_kernel, dim3(blocks_for(total, 256)), dim3(256), 0, s, scales, matrices, n, gated, blocks, words,
+  return launch_pdl(pack_scales_kernel, dim3(blocks_for(total, 256, 8)), dim3(256), 0, s, scales, matrices, n, gated, blocks, words,
                     scale_words_per_stage(format), reinterpret_cast<uint32_t*>(packed));
 }
 cudaError_t launch_gather_rows(const void* x, long long x_stride, long long x_rows, const int32_t* row_index, long long rows, long long k, void* y,
                                cudaStream_t s) {
   const int pieces = static_cast<int>(k / 8);
   const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && x_stride % 8 == 0;
-  return launch_pdl(gather_rows_kernel, dim3(blocks_for(rows * pieces, 256)), dim3(256), 0, s, static_cast<const uint16_t*>(x), x_stride, x_rows,
+  return launch_pdl(gather_rows_kernel, dim3(blocks_for(rows * pieces, 256, 8)), dim3(256), 0, s, static_cast<const uint16_t*>(x), x_stride, x_rows,
                     row_index, rows, k, pieces, static_cast<uint4*>(y), vec);
 }
 
