@@ -26,6 +26,10 @@
 // the tile's features belongs to, and after a barrier of the cluster that one adds them up, in the order of the CTAs.  (One row through 4096 x 4096 has
 // 32 tiles: 32 SMs draw their 128 rows of W at 65 bytes a clock, a fifth of what memory gives.)
 //
+// RAW (with SPLIT, up to 16 rows): x comes as it is, and the epilogue warps, idle until the sums are there, quantize the CTA's part of it
+// into shared memory, where it stays; the ring then holds W alone.  Every tile's CTAs repeat that work, but it saves a launch
+// and what the products wait for it.
+//
 // Every wait is bounded as in gemm_tc.cu: on a time-out the CTA records a code and leaves through its common exit.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -35,6 +39,7 @@
 #include <atomic>
 
 #include "block_linear.cuh"
+#include "fp4.cuh"
 #include "pdl.cuh"
 #include "tma.cuh"
 
@@ -48,6 +53,7 @@ constexpr int kMaxStages = 10;
 constexpr uint32_t kBufferColumns = 256;                   // of tensor memory: an accumulator of up to 224 columns (256 without scales) and a slot of scales behind it
 constexpr int kGroup = 2;                                  // k-blocks of a stage, and slots of scales in tensor memory
 constexpr int kBoxRows = 32;
+constexpr int kRawRows = 16;                               // rows of x that a product quantizes itself
 constexpr int kSlabRows = 32;
 constexpr int kSlabBytes = kSlabRows * 256;                // 128 features of 16 bits, two boxes of 64
 constexpr int kStagingBytes = 2 * kSlabBytes;              // one for each set
@@ -67,7 +73,10 @@ struct LinearParams {
   int sfb_atoms;              // scale tiles of x to a tile of bn rows
   int x_scale_tiles;          // packed scale tiles along the rows of x
   int split, split_blocks;    // CTAs that share a tile's K, k-blocks of each
-  uint32_t staging_bytes;
+  uint32_t staging_bytes, x_bytes;   // RAW: of the quantized part of x
+  const void* x;              // RAW: rows, x_pitch bytes apart
+  long long x_pitch;
+  int x_dtype, x_vec, k;      // x_vec: rows of x start on 16 bytes
   int after_operand;
   uint32_t block_bytes, stage_bytes;
   uint32_t idesc;             // without N
@@ -89,6 +98,7 @@ struct Maps {
 struct alignas(16) Header {
   unsigned long long full[kMaxStages], empty[kMaxStages];
   unsigned long long acc_full[2], acc_empty[2];
+  unsigned long long x_ready;
   uint32_t tmem_base;
   int abort_flag;
   int num_tiles;
@@ -307,14 +317,50 @@ __device__ __noinline__ void store_elements(T* to, long long step, uint32_t from
 }
 __device__ __forceinline__ float gate(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
 
-template <int KIND, int CG, bool GATED, bool SPLIT, typename T>
+// RAW: k-blocks kb .. kb + blocks - 1 of the rows of x into shared memory, as the loads of a quantized x would put them there (16-byte pieces
+// exchanged by the row's number: the 128-byte swizzle).  A warp takes two k-blocks of a row at a time.  Rows up to 15 that do not
+// exist keep what lies there; what comes of them is not stored.
+template <int KIND, typename X>
+__device__ __forceinline__ void quantize_part(const LinearParams& p, int kb, int blocks, uint32_t codes, uint32_t sf, int warp, int lane) {
+  constexpr int NW = scale_words_per_stage(KIND), LANES = fp4_block(KIND) / 16;
+  const TensorScale scale = tensor_scale<KIND, X>(p.x_scale);
+  const int chunks = (blocks + 1) / 2;
+  for (int u = warp; u < p.rows * chunks; u += kEpilogueWarps) {
+    const int r = u / chunks, chunk = u - r * chunks, block = 2 * chunk + (lane >> 4), c = (kb + 2 * chunk) * 256 + lane * 16;
+    const X* row = reinterpret_cast<const X*>(static_cast<const uint8_t*>(p.x) + r * p.x_pitch);
+    Sixteen<X> t;
+    if (p.x_vec) {
+      t = load_16<X, true>(row, c, p.k, nullptr, lane);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t.v[i] = c + i < p.k ? row[c + i] : from_float<X>(0.0f);
+    }
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = to_float(t.v[i]);
+    uint32_t byte;
+    const uint2 code = quantize_16<KIND>(v, top_of(t), scale, byte, [&](int i) { return to_float(row[c + i]); });
+    if (c >= p.k) byte = 0;
+    const uint32_t word = scale_word<KIND>(byte);
+    if (block >= blocks) continue;
+    const int at = lane % 16 * 8;
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};"
+                 ::"r"(codes + block * (kRawRows * kStageBytes) + (r >> 3) * 1024 + (r & 7) * 128 + (((at >> 4) ^ (r & 7)) << 4) + (at & 8)), "r"(code.x), "r"(code.y) : "memory");
+    if (lane % (4 * LANES) == 0)
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(sf + (block * NW + lane % 16 / (4 * LANES)) * kScaleTile + r * 16), "r"(word) : "memory");
+  }
+}
+
+template <int KIND, int CG, bool GATED, bool SPLIT, bool RAW, typename T>
 __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_constant__ Maps maps, const LinearParams p) {
   constexpr int NW = KIND == 0 ? 0 : (KIND == B2VX_FP4_BLOCK32 ? 2 : 4);   // scale words per stage
   extern __shared__ uint8_t smem_raw[];
   pdl_trigger();
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t ring = (raw + 1023u) & ~1023u;
-  const uint32_t staging = ring + p.stages * p.stage_bytes;
+  const uint32_t x_codes = ring + p.stages * p.stage_bytes;       // RAW: a k-block's 16 rows of 128 bytes after the other, then their scale tiles
+  const uint32_t x_sf = x_codes + p.split_blocks * kRawRows * kStageBytes;
+  const uint32_t staging = x_codes + (RAW ? p.x_bytes : 0u);
   Header* h = reinterpret_cast<Header*>(smem_raw + (staging - raw) + p.staging_bytes);
   Group* groups = reinterpret_cast<Group*>(h + 1);
   volatile int* abort_flag = &h->abort_flag;
@@ -325,17 +371,18 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   const int part = SPLIT ? static_cast<int>(cluster_rank()) : 0;
   const int kb_first = SPLIT ? part * p.split_blocks : 0, kb_end = SPLIT ? min(p.k_blocks, kb_first + p.split_blocks) : p.k_blocks;
   // a k-block: [128 rows of W | rows of x | scales of W | scales of x]
-  const uint32_t x_off = kWTile, sfa_off = x_off + static_cast<uint32_t>(p.x_box) * kStageBytes, sfb_off = sfa_off + NW * kScaleTile;
+  const uint32_t x_off = kWTile, sfa_off = x_off + (RAW ? 0u : static_cast<uint32_t>(p.x_box) * kStageBytes), sfb_off = sfa_off + NW * kScaleTile;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < p.stages; ++i) {
-      mbar_init(smem_u32(&h->full[i]), NW ? 3 : 2);
+      mbar_init(smem_u32(&h->full[i]), NW && !RAW ? 3 : 2);
       mbar_init(smem_u32(&h->empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&h->acc_full[i]), 1);
       mbar_init(smem_u32(&h->acc_empty[i]), CG * kEpilogueWarps);
     }
+    mbar_init(smem_u32(&h->x_ready), kEpilogueWarps);
     h->abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -350,11 +397,9 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   }
   if (threadIdx.x == 64) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.w)) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.x)) : "memory");
-    if (NW) {
-      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.w_scales)) : "memory");
-      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.x_scales)) : "memory");
-    }
+    if (NW) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.w_scales)) : "memory");
+    if (!RAW) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.x)) : "memory");
+    if (NW && !RAW) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&maps.x_scales)) : "memory");
   }
   // Behind the kernel that made the operand x, which began its work after everything before it had ended, only the loads of x wait.
   if (!p.after_operand) pdl_wait();
@@ -434,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
         if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
       }
     }
-  } else if (warp == 2) {
+  } else if (!RAW && warp == 2) {
     // ------------------------------------------------------------ producer of x
     pdl_wait();
     const uint32_t announce = CG == 1 ? full0 : in_first_cta(full0);
@@ -473,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     // ------------------------------------------------------------ producer of scales
     pdl_wait();
     const uint32_t announce = CG == 1 ? full0 : in_first_cta(full0);
-    const uint32_t tx = CG * (1 + p.sfb_atoms) * NW * kScaleTile;
+    const uint32_t tx = CG * (1 + (RAW ? 0 : p.sfb_atoms)) * NW * kScaleTile;
     uint32_t s = 0, ph = 0;
     bool ok = true;
     for (int t = first_tile, e = 0; t < num_tiles; t += tile_step) {
@@ -492,7 +537,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
             if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, blocks * tx);
             for (int b = 0; b < blocks; ++b, dst += p.block_bytes) {
               load_2d<CG>(dst + sfa_off, &maps.w_scales, 0, sfa + b * p.scale_tiles * NW, full);
-              load_2d<CG>(dst + sfb_off, &maps.x_scales, 0, sfb + b * p.x_scale_tiles * NW, full);
+              if (!RAW) load_2d<CG>(dst + sfb_off, &maps.x_scales, 0, sfb + b * p.x_scale_tiles * NW, full);
             }
           }
         }
@@ -522,10 +567,12 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const uint32_t d = buf * kBufferColumns;
       // One k-block: its scales into slot `slot` of tensor memory, then four K steps.  The slot was last read by the instructions of
       // the stage before; copies and products of one thread execute in the order issued.
-      auto k_block = [&](uint32_t at, int slot, bool first) {
+      auto k_block = [&](uint32_t at, int slot, int kb, bool first) {
         const uint32_t sfa = p.bn + slot * kBufferColumns, sfb = sfa + NW * 4;
+        const uint32_t x_at = RAW ? ((x_codes >> 4) | kDescLow) + (kb - kb_first) * (kRawRows * kStageBytes >> 4) : at + (x_off >> 4);
         if constexpr (NW > 0) {
-          const uint32_t sfa_low = at + (sfa_off >> 4), sfb_low = at + (sfb_off >> 4);
+          const uint32_t sfa_low = at + (sfa_off >> 4);
+          const uint32_t sfb_low = RAW ? ((x_sf >> 4) | kDescLow) + (kb - kb_first) * (NW * kScaleTile >> 4) : at + (sfb_off >> 4);
 #pragma unroll
           for (int w = 0; w < NW; ++w) copy_scales<CG>(sfa + w * 4, sfa_low + w * (kScaleTile >> 4));
 #pragma unroll
@@ -540,17 +587,18 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
           const int w = KIND == B2VX_FP4_BLOCK32 ? k >> 1 : k;
           // the first of the word's bytes that this K step uses
           const uint32_t id = KIND == B2VX_FP4_BLOCK32 ? (k & 1) * 2u : 0u;
-          mma<KIND, CG>(d, at + 2 * k, at + (x_off >> 4) + 2 * k, idesc | (id << 4) | (id << 29), sfa + w * 4, sfb + w * 8, !(first && k == 0));
+          mma<KIND, CG>(d, at + 2 * k, x_at + 2 * k, idesc | (id << 4) | (id << 29), sfa + w * 4, sfb + w * 8, !(first && k == 0));
         }
       };
       for (int kb = kb_first; kb < kb_end; kb += kGroup) {
         // the next tile is worked out while the instructions of this one's last stages run
         if (kb + kGroup >= kb_end && t + tile_step < num_tiles) tile = tile_of<CG>(groups, p, t + tile_step, tile.e);
+        if (RAW && kb == kb_first) mbar_wait(smem_u32(&h->x_ready), 0, abort_flag, p.status, 107);
         mbar_wait(full0 + 8 * s, ph, abort_flag, p.status, 103);
         if (elect_one()) {
           fence_after();
-          k_block(low, 0, kb == kb_first);
-          if (kb + 1 < kb_end) k_block(low + block_low, 1, false);
+          k_block(low, 0, kb, kb == kb_first);
+          if (kb + 1 < kb_end) k_block(low + block_low, 1, kb + 1, false);
           commit<CG>(empty0 + 8 * s);
         }
         __syncwarp();
@@ -563,6 +611,14 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   } else if (SPLIT && warp >= kFirstEpilogueWarp) {
     // ------------------------------------------------------------ partial sums, to the CTA whose lanes they are: [CTA][row][its lanes]
     const int ew = warp - kFirstEpilogueWarp, quarter = ew & 3, set = ew >> 2;
+    if constexpr (RAW) {
+      if (p.x_dtype == B2VX_DT_FLOAT32) quantize_part<KIND, float>(p, kb_first, kb_end - kb_first, x_codes, x_sf, ew, lane);
+      else if (p.x_dtype == B2VX_DT_FLOAT16) quantize_part<KIND, __half>(p, kb_first, kb_end - kb_first, x_codes, x_sf, ew, lane);
+      else quantize_part<KIND, __nv_bfloat16>(p, kb_first, kb_end - kb_first, x_codes, x_sf, ew, lane);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&h->x_ready));
+    }
     if (first_tile < num_tiles) {
       const Tile tile = tile_of<CG>(groups, p, first_tile, 0);
       const int width = 128 / p.split, l = quarter * 32 + lane, owner = l / width;
@@ -748,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       }
     __syncwarp();
     cluster_barrier();
-    // kThreads is a multiple of quads (16, 32, 64 or half of that), so a thread keeps its features
+    // kThreads is a multiple of quads (a power of two up to 32), so a thread keeps its features
     const int q = threadIdx.x % quads, f = f_first + 4 * q;
     for (int i = threadIdx.x; i < n; i += kThreads) {
       const int r = i / quads;
@@ -824,9 +880,9 @@ bool encode_scales(CUtensorMap* map, const void* base, uint64_t tiles, uint32_t 
   const cuuint32_t box[2] = {kScaleTile / 4, box_tiles};
   return encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
-template <int KIND, int CG, bool GATED, bool SPLIT, typename T>
+template <int KIND, int CG, bool GATED, bool SPLIT, bool RAW, typename T>
 cudaError_t start(const Maps& maps, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
-  auto* kernel = block_linear_kernel<KIND, CG, GATED, SPLIT, T>;
+  auto* kernel = block_linear_kernel<KIND, CG, GATED, SPLIT, RAW, T>;
   // once per GPU (a repeated setting by racing first calls does no harm): the attribute costs a call a microsecond of the host's time
   static std::atomic<bool> ready[kMaxDevices];
   int dev = 0;
@@ -859,20 +915,44 @@ cudaError_t start(const Maps& maps, const LinearParams& p, int grid, size_t smem
   cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, maps, p);
 }
-template <int KIND, int CG, bool GATED, bool SPLIT>
+template <int KIND, int CG, bool GATED, bool SPLIT, bool RAW>
 cudaError_t start_typed(const Maps& m, const LinearParams& p, int grid, size_t smem, cudaStream_t s) {
-  if (p.y_dtype == B2VX_DT_FLOAT32) return start<KIND, CG, GATED, SPLIT, float>(m, p, grid, smem, s);
-  if (p.y_dtype == B2VX_DT_FLOAT16) return start<KIND, CG, GATED, SPLIT, __half>(m, p, grid, smem, s);
-  return start<KIND, CG, GATED, SPLIT, __nv_bfloat16>(m, p, grid, smem, s);
+  if (p.y_dtype == B2VX_DT_FLOAT32) return start<KIND, CG, GATED, SPLIT, RAW, float>(m, p, grid, smem, s);
+  if (p.y_dtype == B2VX_DT_FLOAT16) return start<KIND, CG, GATED, SPLIT, RAW, __half>(m, p, grid, smem, s);
+  return start<KIND, CG, GATED, SPLIT, RAW, __nv_bfloat16>(m, p, grid, smem, s);
 }
-template <int KIND>
-cudaError_t start_kind(const Maps& m, const LinearParams& p, int cg, int gated, int grid, size_t smem, cudaStream_t s) {
-  if (cg == 2) return gated ? start_typed<KIND, 2, true, false>(m, p, grid, smem, s) : start_typed<KIND, 2, false, false>(m, p, grid, smem, s);
-  if (p.split > 1) return gated ? start_typed<KIND, 1, true, true>(m, p, grid, smem, s) : start_typed<KIND, 1, false, true>(m, p, grid, smem, s);
-  return gated ? start_typed<KIND, 1, true, false>(m, p, grid, smem, s) : start_typed<KIND, 1, false, false>(m, p, grid, smem, s);
+template <int KIND, bool GATED>
+cudaError_t start_kind(const Maps& m, const LinearParams& p, int cg, bool clusters, bool raw, int grid, size_t smem, cudaStream_t s) {
+  if (cg == 2) return start_typed<KIND, 2, GATED, false, false>(m, p, grid, smem, s);
+  if constexpr (KIND != 0)
+    if (raw) return start_typed<KIND, 1, GATED, true, true>(m, p, grid, smem, s);
+  if (clusters) return start_typed<KIND, 1, GATED, true, false>(m, p, grid, smem, s);
+  return start_typed<KIND, 1, GATED, false, false>(m, p, grid, smem, s);
+}
+
+// CTAs to a tile's K: as many of 8, 4, 2 as leave every tile a cluster of its own in one round, every CTA a stage of K and none without;
+// else 1.
+struct Split {
+  int ctas, blocks;
+};
+Split split_of(long long tiles, int k_blocks, int sm_count) {
+  for (int c = 8; c > 1; c /= 2) {
+    const int blocks = (k_blocks + c - 1) / c;
+    if (tiles * c <= sm_count && blocks >= kGroup && (c - 1) * blocks < k_blocks) return {c, blocks};
+  }
+  return {1, k_blocks};
 }
 
 }  // namespace
+
+bool linear_raw(int format, long long rows, long long n, long long k, int experts, int gated, int sm_count) {
+  if (!format || experts != 1 || rows > kRawRows) return false;
+  const long long tiles = weight_tiles(n, gated);
+  if (tiles > sm_count) return false;
+  // what a CTA quantizes: 48 KB of shared memory, and two rounds of 8 warps with 512 columns each for every row up to 16
+  const Split split = split_of(tiles, static_cast<int>((k + 255) / 256), sm_count);
+  return split.blocks * (kRawRows * kStageBytes + scale_words_per_stage(format) * kScaleTile) <= 48 * 1024 && rows * split.blocks <= 128;
+}
 
 cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why) {
   *why = "";
@@ -892,22 +972,23 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   p.x_box = p.bn / cg;
   p.feature_tiles = (p.scale_tiles + cg - 1) / cg;
   p.sfb_atoms = fp4 ? (p.bn + 127) / 128 : 0;
-  p.block_bytes = (128 + p.x_box) * kStageBytes + (1 + p.sfb_atoms) * nw * kScaleTile;
+  p.block_bytes = a.raw ? kWTile + nw * kScaleTile : (128 + p.x_box) * kStageBytes + (1 + p.sfb_atoms) * nw * kScaleTile;
   p.block_bytes = (p.block_bytes + 1023u) & ~1023u;
   const int elem = a.y_dtype == B2VX_DT_FLOAT32 ? 4 : 2;
   p.y_vec = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.y_stride * elem % 16 == 0;
-  // CTAs to a tile's K: as many of 8, 4, 2 as leave every tile a cluster of its own in one round and every CTA a stage of K.
   const long long most = (a.rows / p.bn + groups) * p.feature_tiles;
-  p.split = 1;
-  for (int c = 8; cg == 1 && c > 1 && p.split == 1; c /= 2) {
-    const int blocks = (p.k_blocks + c - 1) / c;
-    if (most * c <= a.sm_count && blocks >= kGroup && (c - 1) * blocks < p.k_blocks) {
-      p.split = c;
-      p.split_blocks = blocks;
-    }
-  }
-  p.staging_bytes = p.split > 1 ? p.bn * 512 : kStagingBytes;
-  const int behind = static_cast<int>(p.staging_bytes) + static_cast<int>(sizeof(Header)) + static_cast<int>(sizeof(Group)) * (a.experts + 1) + 1024;   // and the ring's alignment
+  const Split split = cg == 1 ? split_of(most, p.k_blocks, a.sm_count) : Split{1, p.k_blocks};
+  p.split = split.ctas;
+  p.split_blocks = split.blocks;
+  const bool clusters = a.raw || p.split > 1;
+  p.x = a.x;
+  p.x_pitch = a.x_pitch;
+  p.x_dtype = a.x_dtype;
+  p.x_vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_pitch % 16 == 0;
+  p.k = static_cast<int>(a.k);
+  p.x_bytes = a.raw ? (p.split_blocks * (kRawRows * kStageBytes + nw * kScaleTile) + 1023u) & ~1023u : 0u;
+  p.staging_bytes = clusters ? p.bn * 512 : kStagingBytes;
+  const int behind = static_cast<int>(p.staging_bytes + p.x_bytes) + static_cast<int>(sizeof(Header)) + static_cast<int>(sizeof(Group)) * (a.experts + 1) + 1024;   // and the ring's alignment
   const int room = static_cast<int>((kSmemBudget - behind) / p.block_bytes);      // k-blocks that fit
   p.stages = std::min(kMaxStages, room / kGroup);
   p.stage_bytes = kGroup * p.block_bytes;
@@ -939,16 +1020,23 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
     return cudaErrorInvalidValue;
   }
   bool ok = a.gated ? encode_gated(&maps.w, a.w, kbytes, a.n, a.experts) : encode_rows(&maps.w, a.w, kbytes, kbytes, a.n, a.experts, 3, 128);
-  ok = ok && encode_rows(&maps.x, a.x, kbytes, x_pitch, rows, 1, 2, p.x_box) && encode_rows(&maps.x32, a.x, kbytes, x_pitch, rows, 1, 2, kBoxRows);
-  if (fp4) ok = ok && encode_scales(&maps.w_scales, a.w_scales, w_tiles, nw) && encode_scales(&maps.x_scales, a.x_scales, x_tiles, nw * p.sfb_atoms);
+  if (fp4) ok = ok && encode_scales(&maps.w_scales, a.w_scales, w_tiles, nw);
+  if (!a.raw) {
+    ok = ok && encode_rows(&maps.x, a.x, kbytes, x_pitch, rows, 1, 2, p.x_box) && encode_rows(&maps.x32, a.x, kbytes, x_pitch, rows, 1, 2, kBoxRows);
+    if (fp4) ok = ok && encode_scales(&maps.x_scales, a.x_scales, x_tiles, nw * p.sfb_atoms);
+  }
   if (!ok) {
     *why = "tensor map refused";
     return cudaErrorInvalidValue;
   }
-  const int grid = p.split > 1 ? static_cast<int>(most) * p.split : static_cast<int>(std::max<long long>(1, std::min<long long>(a.sm_count / cg, most))) * cg;
-  if (a.format == 0) return start_kind<0>(maps, p, cg, a.gated, grid, smem, s);
-  if (a.format == B2VX_FP4_BLOCK32) return start_kind<B2VX_FP4_BLOCK32>(maps, p, cg, a.gated, grid, smem, s);
-  return start_kind<B2VX_FP4_BLOCK16>(maps, p, cg, a.gated, grid, smem, s);
+  const int grid = clusters ? static_cast<int>(most) * p.split : static_cast<int>(std::max<long long>(1, std::min<long long>(a.sm_count / cg, most))) * cg;
+  auto start_format = [&](auto kind) {
+    constexpr int KIND = decltype(kind)::value;
+    return a.gated ? start_kind<KIND, true>(maps, p, cg, clusters, a.raw, grid, smem, s) : start_kind<KIND, false>(maps, p, cg, clusters, a.raw, grid, smem, s);
+  };
+  if (a.format == 0) return start_format(std::integral_constant<int, 0>{});
+  if (a.format == B2VX_FP4_BLOCK32) return start_format(std::integral_constant<int, B2VX_FP4_BLOCK32>{});
+  return start_format(std::integral_constant<int, B2VX_FP4_BLOCK16>{});
 }
 
 }  // namespace b2vx

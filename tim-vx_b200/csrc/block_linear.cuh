@@ -96,11 +96,14 @@ struct LinearArgs {
   const int32_t* offsets;
   void* y;
   long long y_stride;          // elements
+  bool raw;                    // x is rows of x_dtype numbers, x_pitch apart, that the product quantizes itself (linear_raw)
   bool after_operand;          // the kernel before this one in the stream made x and x_scales, and waited for all before it
   int* status;
   int sm_count;
 };
 cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why);
+// Whether the product quantizes x itself: one matrix, up to 16 rows, a cluster for every tile, little to quantize for each CTA.
+bool linear_raw(int format, long long rows, long long n, long long k, int experts, int gated, int sm_count);
 
 }  // namespace b2vx
 #endif  // B2VX_BLOCK_LINEAR_CUH_

@@ -239,7 +239,11 @@ extern "C" b2vx_status b2vx_linear_noalloc(const b2vx_linear_desc* d, const b2vx
   l.after_operand = !direct;
   l.status = pd->status; l.sm_count = pd->sm_count;
   cudaError_t e = cudaSuccess;
-  if (fp4) {
+  if (fp4 && !a->row_index && linear_raw(l.format, l.rows, l.n, l.k, l.experts, l.gated, l.sm_count) && !a->offsets) {
+    l.raw = true;
+    l.after_operand = false;
+    l.x = a->x; l.x_pitch = static_cast<long long>(d->x_stride * size_of(d->x_dtype));
+  } else if (fp4) {
     QuantizeArgs q = {};
     q.x = a->x; q.x_dtype = d->x_dtype;
     q.x_stride = static_cast<long long>(d->x_stride); q.x_rows = static_cast<long long>(d->x_rows);

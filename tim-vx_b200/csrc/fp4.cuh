@@ -69,6 +69,74 @@ __device__ __forceinline__ float e2m1_magnitude(uint32_t c) {
   return c < 2 ? 0.5f * c : __int_as_float((((c >> 1) + 126u) << 23) | ((c & 1u) << 22));
 }
 
+template <typename T>
+__device__ __forceinline__ float to_float(T v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
+  else return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_float(float v) {
+  if constexpr (sizeof(T) == 4) return v;
+  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
+
+// Sixteen numbers from column c on, zeros from column k on, as they lie.  VEC: rows start on 16 bytes, so whole pieces load in 16 bytes.
+template <typename T>
+struct alignas(16) Sixteen {
+  T v[16];
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ Sixteen<T> load_16(const T* row, int c, int k, uint4* staging, int lane) {
+  Sixteen<T> t;
+  constexpr int W = sizeof(t) / 16;
+  if (VEC && c + 16 <= k) {
+    const uint4* src = reinterpret_cast<const uint4*>(row + c);
+#pragma unroll
+    for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(&t)[i] = __ldg(src + i);
+  } else if (VEC) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t.v[i] = c + i < k ? row[c + i] : from_float<T>(0.0f);
+  } else {
+    // neighbouring numbers by neighbouring lanes, handed over through the warp's staging memory: each lane's sixteen numbers and 16 bytes
+    // more, so that eight lanes' 16-byte pieces fall into different banks
+    constexpr int kPitch = 16 + 16 / sizeof(T);
+    T* s = reinterpret_cast<T*>(staging);
+    const int first = c - lane * 16;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int at = i * 32 + lane;
+      s[(at >> 4) * kPitch + (at & 15)] = first + at < k ? row[first + at] : from_float<T>(0.0f);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(&t)[i] = staging[lane * (W + 1) + i];
+  }
+  return t;
+}
+// The largest magnitude, as float bits.
+template <typename T>
+__device__ __forceinline__ uint32_t top_of(const Sixteen<T>& t) {
+  if constexpr (sizeof(T) == 4) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(t.v[i]) & 0x7fffffffu);
+    return top;
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&t);
+    constexpr uint32_t kMagnitudes = 0x7fff7fffu;
+    uint32_t two = w[0] & kMagnitudes;
+#pragma unroll
+    for (int i = 1; i < 7; i += 2) two = __vimax3_u16x2(two, w[i] & kMagnitudes, w[i + 1] & kMagnitudes);
+    two = __vmaxu2(two, w[7] & kMagnitudes);
+    const uint32_t top = max(two & 0xffffu, two >> 16);
+    if constexpr (std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top)))) & 0x7fffffffu;
+    else return top << 16;
+  }
+}
+
 // What quantization needs of block16's tensor scale, worked out once by a thread.
 struct TensorScale {
   float g = 1.0f;          // times lift
@@ -183,6 +251,15 @@ __device__ __forceinline__ uint2 quantize_16(const float (&v)[16], uint32_t top,
     codes = make_uint2(0u, 0u);
   }
   return codes;
+}
+
+// Four neighbouring blocks' bytes as a word, in the first of their lanes.
+template <int FORMAT>
+__device__ __forceinline__ uint32_t scale_word(uint32_t byte) {
+  constexpr int LANES = FORMAT == B2VX_FP4_BLOCK32 ? 2 : 1;
+  uint32_t word = byte | __shfl_down_sync(0xffffffffu, byte, LANES) << 8;
+  word |= __shfl_down_sync(0xffffffffu, word, 2 * LANES) << 16;
+  return word;
 }
 
 }  // namespace b2vx

@@ -21,74 +21,6 @@ constexpr int quantize_blocks(int format) { return format == B2VX_FP4_BLOCK16 ? 
 constexpr long long kTwiceElements = 1 << 22;
 constexpr int kChunk = 512;   // columns of a warp per step, two k-blocks of the products
 
-template <typename T>
-__device__ __forceinline__ float to_float(T v) {
-  if constexpr (sizeof(T) == 4) return v;
-  else if constexpr (std::is_same<T, __half>::value) return __half2float(v);
-  else return __bfloat162float(v);
-}
-template <typename T>
-__device__ __forceinline__ T from_float(float v) {
-  if constexpr (sizeof(T) == 4) return v;
-  else if constexpr (std::is_same<T, __half>::value) return __float2half_rn(v);
-  else return __float2bfloat16_rn(v);
-}
-
-// Sixteen numbers from column c on, zeros from column k on, as they lie.  VEC: rows start on 16 bytes, so whole pieces load in 16 bytes.
-template <typename T>
-struct alignas(16) Sixteen {
-  T v[16];
-};
-template <typename T, bool VEC>
-__device__ __forceinline__ Sixteen<T> load_16(const T* row, int c, int k, uint4* staging, int lane) {
-  Sixteen<T> t;
-  constexpr int W = sizeof(t) / 16;
-  if (VEC && c + 16 <= k) {
-    const uint4* src = reinterpret_cast<const uint4*>(row + c);
-#pragma unroll
-    for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(&t)[i] = __ldg(src + i);
-  } else if (VEC) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t.v[i] = c + i < k ? row[c + i] : from_float<T>(0.0f);
-  } else {
-    // neighbouring numbers by neighbouring lanes, handed over through the warp's staging memory: each lane's sixteen numbers and 16 bytes
-    // more, so that eight lanes' 16-byte pieces fall into different banks
-    constexpr int kPitch = 16 + 16 / sizeof(T);
-    T* s = reinterpret_cast<T*>(staging);
-    const int first = c - lane * 16;
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int at = i * 32 + lane;
-      s[(at >> 4) * kPitch + (at & 15)] = first + at < k ? row[first + at] : from_float<T>(0.0f);
-    }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < W; ++i) reinterpret_cast<uint4*>(&t)[i] = staging[lane * (W + 1) + i];
-  }
-  return t;
-}
-// The largest magnitude, as float bits.
-template <typename T>
-__device__ __forceinline__ uint32_t top_of(const Sixteen<T>& t) {
-  if constexpr (sizeof(T) == 4) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(t.v[i]) & 0x7fffffffu);
-    return top;
-  } else {
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(&t);
-    constexpr uint32_t kMagnitudes = 0x7fff7fffu;
-    uint32_t two = w[0] & kMagnitudes;
-#pragma unroll
-    for (int i = 1; i < 7; i += 2) two = __vimax3_u16x2(two, w[i] & kMagnitudes, w[i + 1] & kMagnitudes);
-    two = __vmaxu2(two, w[7] & kMagnitudes);
-    const uint32_t top = max(two & 0xffffu, two >> 16);
-    if constexpr (std::is_same<T, __half>::value) return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(top)))) & 0x7fffffffu;
-    else return top << 16;
-  }
-}
-
 // The group of a row: how many groups end at or before it.
 __device__ __forceinline__ int group_of(const int32_t* offsets, int experts, long long row, int lane) {
   int n = 0;
@@ -156,8 +88,7 @@ __global__ void __launch_bounds__(kWarps * 32, quantize_blocks(FORMAT)) quantize
       }
       if (PACKED) {
         if (c >= k) byte = 0;
-        uint32_t word = byte | __shfl_down_sync(0xffffffffu, byte, LANES) << 8;
-        word |= __shfl_down_sync(0xffffffffu, word, 2 * LANES) << 16;
+        const uint32_t word = scale_word<FORMAT>(byte);
         const int k_block = c / 256, w = lane % 16 / (4 * LANES);
         if (lane % (4 * LANES) == 0 && tile && k_block * 256 < k)
           *reinterpret_cast<uint32_t*>(tile + (static_cast<long long>(k_block) * a.scale_tiles * PER + w) * kScaleTile) = word;
