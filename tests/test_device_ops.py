@@ -193,6 +193,14 @@ def test_tensors_must_be_on_a_gpu():
         D.quantize_fp4(torch.zeros(2, 32), "block16")
     with pytest.raises(ValueError, match="last dimension"):
         D.quantize_fp4(torch.zeros(32, 2).t())
+    with pytest.raises(ValueError, match="gradient"):
+        D.quantize_fp4(torch.zeros(2, 32, requires_grad=True))
+    with pytest.raises(ValueError, match="must be a tensor"):
+        D.quantize_fp4([[1.0] * 32])
+    with pytest.raises(ValueError, match="multiple of 16"):
+        D.Fp4Weight(torch.zeros(24, 32, dtype=torch.uint8), torch.zeros(24, 2, dtype=torch.uint8), gated=True)
+    with pytest.raises(ValueError, match="shape"):
+        D.Fp4Weight(torch.zeros(24, 32, dtype=torch.uint8), torch.zeros(24, 4, dtype=torch.uint8))
     with pytest.raises(ValueError, match="offsets"):
         D.expert_linear(torch.zeros(2, 32, dtype=torch.bfloat16), torch.zeros(3, 8, 32, dtype=torch.bfloat16), None)
     with pytest.raises(ValueError, match="columns"):

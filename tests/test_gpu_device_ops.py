@@ -155,6 +155,27 @@ def test_quantize_borders_block16(g):
     same_quantized(D.quantize_fp4(x, "block16", scale=torch.tensor([g], device="cuda")), x, g)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("g", [1.0, 1 / 56, 0.5, 3 / 1024, 0.0131, 1.0009765625])
+def test_quantize_16_bit_numbers_near_borders(dtype, g):
+    """16-bit numbers that lie on borders, and the 16-bit numbers next to those that lie near one, for tensor scales of few and of many bits."""
+    g = float(np.float32(g))
+    rows = []
+    for b in list(range(40, 80)) + [1, 7, 8, 126]:
+        unit = np.float64(E4M3[b]) * g
+        near = np.concatenate([(E2M1[1:] + E2M1[:-1]) / 2 * unit, E2M1 * unit])
+        x = torch.from_numpy(near).to(dtype)
+        row = torch.zeros(16, dtype=dtype)
+        row[:15] = x
+        for step in (0, 1, -1):
+            r = (row.view(torch.int16) + torch.where(row != 0, step, 0).to(torch.int16)).view(dtype)
+            r[15] = torch.tensor(6 * unit, dtype=dtype)
+            rows.append(r)
+            rows.append(-r)
+    x = torch.stack(rows).cuda()
+    same_quantized(D.quantize_fp4(x, "block16", scale=torch.tensor([g], device="cuda")), x, g)
+
+
 def test_quantize_borders_block32():
     rows = []
     for e in (-140, -127, -126, -125, -100, -1, 0, 3, 100, 124, 125):
@@ -324,7 +345,8 @@ def test_linear(fmt, rows, n, k):
     close(y, *expected(xv, wv, None if bias is None else f64(bias), False))
 
 
-@pytest.mark.parametrize("rows,n,k", [(1, 4096, 4096), (8, 2048, 8192), (3, 5000, 6016), (16, 1024, 16384), (300, 8192, 2048), (2100, 4100, 512)])
+@pytest.mark.parametrize("rows,n,k", [(1, 4096, 4096), (8, 2048, 8192), (3, 5000, 6016), (16, 1024, 16384), (300, 8192, 2048), (2100, 4100, 512), (1, 18000, 8192),
+                                      (16, 900, 3104), (17, 900, 3104), (64, 20000, 1056), (1, 40, 65536)])
 @pytest.mark.parametrize("fmt", ["block32", "block16"])
 def test_linear_large(fmt, rows, n, k):
     x = gaussian(rows, k, torch.bfloat16, rows, 1.0)
@@ -357,6 +379,29 @@ def test_linear_views(fmt, offset, x_stride, y_stride):
     mask = torch.ones_like(buf, dtype=torch.bool)
     mask.as_strided((rows, n), (y_stride, 1), offset % 7).fill_(False)
     assert (buf[mask] == -77.0).all()
+
+
+@pytest.mark.parametrize("fmt", ["block32", "block16", "none"])
+@pytest.mark.parametrize("rows", [1, 5, 20, 64])
+def test_linear_views_few_rows(fmt, rows):
+    """The same with few rows: products that quantize x themselves, that share K, and that do neither."""
+    for n, k, offset, x_stride, y_stride in ((130, 1056, 1, 1061, 131), (19000, 96, 3, 99, 19001)):
+        store = gaussian(rows + 1, x_stride + offset, torch.float16, 9, 1.0).flatten()
+        x = store.as_strided((rows, k), (x_stride, 1), offset)
+        xv, s = operand(x, fmt)
+        if fmt == "none":
+            w = (gaussian(n, k, torch.float32, 4, 1.0) / k ** 0.5).half()
+            wv = f64(w)
+        else:
+            w, wv = weight_of(0, n, k, fmt, 4)
+            wv = wv[0]
+        buf = torch.full((rows * y_stride + 7,), -77.0, dtype=torch.float16, device="cuda")
+        y = buf.as_strided((rows, n), (y_stride, 1), 3)
+        D.linear(x, w, x_scale=s, out=y)
+        close(y, *expected(xv, wv, None, False))
+        mask = torch.ones_like(buf, dtype=torch.bool)
+        mask.as_strided((rows, n), (y_stride, 1), 3).fill_(False)
+        assert (buf[mask] == -77.0).all()
 
 
 def test_linear_row_index_and_types():
@@ -443,6 +488,27 @@ def test_expert_linear(fmt, gated, counts):
         lo, hi = starts[e], starts[e + 1]
         if hi > lo:
             close(y[lo:hi], *expected(xv[index.cpu().numpy()[lo:hi]], wv[e], b[e], gated))
+
+
+@pytest.mark.parametrize("fmt", ["block32", "block16", "none"])
+@pytest.mark.parametrize("out_dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("rows", [3, 40, 400])
+def test_gated_output_types(fmt, out_dtype, rows):
+    """One group of a gated product, few rows (K shared), a narrow tile and tiles of two CTAs; an odd place and stride of y."""
+    n, k = 200, 1120
+    dtype = torch.float32 if fmt != "none" else torch.bfloat16
+    x = gaussian(rows, k, dtype, 31, 1.0)
+    xv, s = operand(x, fmt)
+    if fmt == "none":
+        w = (gaussian(2 * n, k, torch.float32, 5, 1.0) / k ** 0.5).bfloat16().reshape(1, 2 * n, k)
+        wv = f64(w)
+    else:
+        w, wv = weight_of(1, 2 * n, k, fmt, 5, True)
+    bias = gaussian(1, 2 * n, torch.float32, 6, 0.0)
+    buf = torch.full((rows, n + 5), -77.0, dtype=out_dtype, device="cuda")
+    D.expert_linear(x, w, torch.tensor([0, rows], dtype=torch.int32, device="cuda"), bias=bias, gated=True, x_scale=s, out=buf[:, 3:3 + n])
+    close(buf[:, 3:3 + n], *expected(xv, wv[0], f64(bias)[0], True))
+    assert (buf[:, :3] == -77.0).all() and (buf[:, 3 + n:] == -77.0).all()
 
 
 @pytest.mark.parametrize("fmt", ["block32", "none"])
@@ -544,6 +610,27 @@ def test_route_ties_and_special_values():
     z = z.cuda()
     for normalize in (True, False):
         for k in (1, 5, 32):
+            same_routes(D.route_experts(z, k, normalize), z, k, normalize)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("tokens", [60, 200])
+def test_route_special_values_of_16_bits(dtype, tokens):
+    inf, nan = float("inf"), float("nan")
+    z = torch.randint(-3, 3, (tokens, 100)).to(dtype)
+    z[1] = -inf
+    z[2] = nan
+    z[3, 10:] = -inf
+    z[4, 5], z[4, 6] = inf, inf
+    z[5, 1], z[5, 2] = nan, 3.0
+    z[6] = -0.0
+    z[6, 3] = 0.0
+    z[7] = torch.linspace(-1e-7, 1e-7, 100).to(dtype)
+    z[8, ::7] = torch.finfo(dtype).max
+    z[9] = torch.finfo(dtype).min
+    z = z.cuda()
+    for normalize in (True, False):
+        for k in (1, 6, 32):
             same_routes(D.route_experts(z, k, normalize), z, k, normalize)
 
 
@@ -662,6 +749,25 @@ def test_captured_layers():
         for o, w in zip(outs, want):
             assert torch.equal(o, w)
         assert torch.equal(other, want[0])
+
+
+def test_two_streams_at_once():
+    """Layers on two streams, nothing waited for in between."""
+    layers = [Layer("block32", 16, 512, 192, 4, 60), Layer("block16", 16, 512, 192, 4, 70)]
+    xs = [gaussian(n, 512, torch.bfloat16, 9 + n, 0.0) for n in (1, 37, 400)]
+    want = [[layer(x)[0].clone() for x in xs] for layer in layers]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(6):
+        for i, x in enumerate(xs):
+            for s in range(2):
+                with torch.cuda.stream(streams[s]):
+                    got[s].append((i, layers[s](x)[0]))
+    torch.cuda.synchronize()
+    for s in range(2):
+        for i, y in got[s]:
+            assert torch.equal(y, want[s][i])
 
 
 def test_results_do_not_depend_on_the_run():

@@ -949,9 +949,10 @@ bool linear_raw(int format, long long rows, long long n, long long k, int expert
   if (!format || experts != 1 || rows > kRawRows) return false;
   const long long tiles = weight_tiles(n, gated);
   if (tiles > sm_count) return false;
-  // what a CTA quantizes: 48 KB of shared memory, and two rounds of 8 warps with 512 columns each for every row up to 16
+  // What a CTA quantizes: up to 32 k-blocks of a row, two rounds of its 8 warps.  4096 x 4096 (4 k-blocks a CTA) with 1 / 8 / 16 rows:
+  // 7.7 / 7.6 / 7.7 us with a launch of its own for that, 6.3 / 6.8 / 8.2 without; 8192 x 8192 (16) with 1 / 4 rows 11.8 / 11.8 and 9.9 / 12.3.
   const Split split = split_of(tiles, static_cast<int>((k + 255) / 256), sm_count);
-  return split.blocks * (kRawRows * kStageBytes + scale_words_per_stage(format) * kScaleTile) <= 48 * 1024 && rows * split.blocks <= 128;
+  return rows * split.blocks <= 32;
 }
 
 cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why) {
@@ -987,7 +988,7 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   p.x_vec = reinterpret_cast<uintptr_t>(a.x) % 16 == 0 && a.x_pitch % 16 == 0;
   p.k = static_cast<int>(a.k);
   p.x_bytes = a.raw ? (p.split_blocks * (kRawRows * kStageBytes + nw * kScaleTile) + 1023u) & ~1023u : 0u;
-  p.staging_bytes = clusters ? p.bn * 512 : kStagingBytes;
+  p.staging_bytes = clusters ? (a.raw ? kRawRows : p.bn) * 512 : kStagingBytes;
   const int behind = static_cast<int>(p.staging_bytes + p.x_bytes) + static_cast<int>(sizeof(Header)) + static_cast<int>(sizeof(Group)) * (a.experts + 1) + 1024;   // and the ring's alignment
   const int room = static_cast<int>((kSmemBudget - behind) / p.block_bytes);      // k-blocks that fit
   p.stages = std::min(kMaxStages, room / kGroup);
