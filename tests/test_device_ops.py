@@ -75,7 +75,8 @@ def test_dequantize_refuses_pointers():
     (dict(w_format=4), "w_format"), (dict(x_dtype=1), "float32"), (dict(y_dtype=2), "float32"), (dict(w_format=0, x_dtype=9), "16-bit"),
     (dict(gated=2), "gated"), (dict(gated=1, n=60), "gated"), (dict(experts=1025), "1024"), (dict(n=1 << 30), "range"), (dict(k=0, x_stride=0), "zero"), (dict(k=100, x_stride=100), "multiple"),
     (dict(w_format=0, k=100, x_stride=100), "multiple"), (dict(x_stride=95), "x_stride"), (dict(y_stride=63), "y_stride"),
-    (dict(rows=1 << 28, x_rows=1 << 28, n=1 << 20, y_stride=1 << 20), "tiles")])
+    (dict(rows=1 << 28, x_rows=1 << 28, n=1 << 20, y_stride=1 << 20), "tiles"), (dict(n=1 << 28, y_stride=1 << 28), "range"),
+    (dict(experts=1024, n=1 << 22, k=1 << 16, x_stride=1 << 16, y_stride=1 << 22), "tiles")])
 def test_linear_refuses(change, words):
     size = C.c_size_t()
     d = desc(ABI.LinearDesc, LINEAR, **change)

@@ -1016,10 +1016,6 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   Maps maps = {};
   const uint64_t rows = static_cast<uint64_t>(a.rows), x_pitch = static_cast<uint64_t>(a.x_pitch);
   const uint64_t w_tiles = static_cast<uint64_t>(a.experts) * p.k_blocks * p.scale_tiles * nw, x_tiles = static_cast<uint64_t>(p.k_blocks) * p.x_scale_tiles * nw;
-  if (w_tiles >= 1ull << 31 || x_tiles >= 1ull << 31) {
-    *why = "the product has too many scale tiles";
-    return cudaErrorInvalidValue;
-  }
   bool ok = a.gated ? encode_gated(&maps.w, a.w, kbytes, a.n, a.experts) : encode_rows(&maps.w, a.w, kbytes, kbytes, a.n, a.experts, 3, 128);
   if (fp4) ok = ok && encode_scales(&maps.w_scales, a.w_scales, w_tiles, nw);
   if (!a.raw) {

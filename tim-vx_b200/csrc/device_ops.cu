@@ -116,9 +116,19 @@ b2vx_status check_linear(const b2vx_linear_desc* d, char* err, size_t err_len) {
   B2VX_NEED(d->w_format ? d->k % 32 == 0 : d->k % 8 == 0, "k must be a multiple of 32 for 4-bit and of 8 for 16-bit weights");
   B2VX_NEED(d->x_stride >= d->k && d->x_stride <= kMaxStride, "x_stride is smaller than a row or out of range");
   B2VX_NEED(d->y_stride >= d->n && d->y_stride <= kMaxStride, "y_stride is smaller than a row or out of range");
-  // tiles are counted in 32 bits
-  const double tiles = (static_cast<double>(d->rows) / 64 + (d->experts ? d->experts : 1)) * (static_cast<double>(d->n) / 128 + 1);
-  B2VX_NEED(tiles < 2e9, "the product has too many tiles");
+  // tiles of the product and scale tiles of its operands are counted in 32 bits, feature tiles divided as floats
+  B2VX_NEED(d->n <= 1u << 27, "an extent is out of range");
+  const int experts = d->experts ? static_cast<int>(d->experts) : 1;
+  const double feature_tiles = static_cast<double>(weight_tiles(static_cast<long long>(d->n), d->gated)) + 1;
+  double most = (static_cast<double>(d->rows) / 64 + experts) * feature_tiles;
+  if (d->w_format) {
+    const double words = static_cast<double>(scale_words(static_cast<long long>(d->k), d->w_format));
+    const int bn = tile_rows(static_cast<long long>(d->rows), experts, d->w_format);
+    const double x_tiles = static_cast<double>(expert_scale_tiles(static_cast<long long>(d->rows), experts, bn)) + 2;
+    most = most > words * experts * feature_tiles ? most : words * experts * feature_tiles;
+    most = most > words * x_tiles ? most : words * x_tiles;
+  }
+  B2VX_NEED(most < 2e9, "the product has too many tiles");
   return B2VX_OK;
 }
 
