@@ -322,7 +322,8 @@ b2vx_status b2vx_conv2d_first_layer_noalloc(const b2vx_conv2d_noalloc_desc* d, c
  * be captured into a CUDA graph, after the first call on that GPU; calls or
  * captured graphs that may overlap need a workspace each.  Arguments are checked
  * before anything is launched; refusals return a status and write a message to err
- * (err may be NULL).  Counts of zero are fine: nothing is launched.
+ * (err may be NULL).  Counts of zero are fine: nothing is launched.  Outputs must not
+ * overlap inputs, but for the residual of a weighted sum.
  *
  * 4-bit values are e2m1: codes 0..7 stand for 0, 0.5, 1, 1.5, 2, 3, 4, 6, bit 3 is
  * the sign; two to a byte, the even column in the low half.

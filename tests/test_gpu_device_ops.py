@@ -722,6 +722,36 @@ def test_expert_layer(fmt, tokens):
     close(y, terms.sum(axis=1) + f64(x), 6 * 2.0 ** -24 * (np.abs(terms).sum(axis=1) + np.abs(f64(x))))
 
 
+def test_nothing_to_do():
+    w, _ = weight_of(3, 16, 64, "block32", 1)
+    wb = torch.zeros(3, 16, 64, dtype=torch.bfloat16, device="cuda")
+    offsets = torch.zeros(4, dtype=torch.int32, device="cuda")
+    none = torch.empty(0, 64, dtype=torch.bfloat16, device="cuda")
+    for weight in (w, wb):
+        assert D.expert_linear(none, weight, offsets).shape == (0, 16)
+    assert D.linear(none, torch.zeros(16, 64, dtype=torch.bfloat16, device="cuda")).shape == (0, 16)
+    index = torch.full((5,), -1, dtype=torch.int32, device="cuda")
+    offsets[1:] = 5
+    for weight in (w, wb):                                  # rows, but no row of x behind them
+        assert not D.expert_linear(none, weight, offsets, row_index=index).any()
+    q = D.quantize_fp4(none)
+    assert q.codes.shape == (0, 32) and D.dequantize_fp4(q).shape == (0, 64)
+    assert not D.quantize_fp4(none, row_index=index).codes.any()
+    assert D.combine_experts(none, torch.zeros(0, 2, dtype=torch.int32, device="cuda"), torch.zeros(0, 2, device="cuda")).shape == (0, 64)
+    y = D.combine_experts(none, torch.zeros(3, 2, dtype=torch.int32, device="cuda"), torch.ones(3, 2, device="cuda"))
+    assert y.shape == (3, 64) and not y.any()
+
+
+def test_outputs_must_not_overlap_inputs():
+    x = torch.zeros(8, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="overlaps"):
+        D.linear(x, torch.zeros(64, 64, dtype=torch.bfloat16, device="cuda"), out=x)
+    with pytest.raises(ValueError, match="overlaps"):
+        D.combine_experts(x, torch.zeros(4, 2, dtype=torch.int32, device="cuda"), torch.zeros(4, 2, device="cuda"), out=x[4:])
+    with pytest.raises(ValueError, match="overlap"):
+        D.linear(x, torch.zeros(64, 64, dtype=torch.bfloat16, device="cuda"), out=torch.zeros(64, dtype=torch.bfloat16, device="cuda").expand(8, 64))
+
+
 def test_captured_layers():
     """Two captured graphs, each replayed on new inputs, interleaved with eager calls on another stream."""
     layers = [Layer("block32", 9, 256, 96, 2, 40), Layer("block16", 5, 128, 64, 2, 50)]

@@ -118,6 +118,16 @@ at::Tensor output(PyObject* out, at::IntArrayRef shape, at::ScalarType type, con
   need(t.size(0) <= 1 || t.stride(0) >= t.size(1), "out has rows that overlap");
   return t;
 }
+// Whether the memory from a's first to its last element meets b's.
+bool overlap(const at::Tensor& a, const at::Tensor& b) {
+  if (!a.numel() || !b.numel()) return false;
+  auto end = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return static_cast<const char*>(t.data_ptr()) + (last + 1) * static_cast<int64_t>(t.element_size());
+  };
+  return static_cast<const char*>(a.data_ptr()) < end(b) && static_cast<const char*>(b.data_ptr()) < end(a);
+}
 uint64_t row_stride(const at::Tensor& t) { return static_cast<uint64_t>(t.size(0) > 1 ? t.stride(0) : t.size(1)); }
 
 // The device of a call as the current one, its current stream, and the place for a message.
@@ -242,6 +252,7 @@ PyObject* product(PyObject* const* a) {
   p.bias = static_cast<const float*>(experts ? dense(a[8], "bias", at::kFloat, {experts, w_rows}, device) : dense(a[8], "bias", at::kFloat, {w_rows}, device));
   Call call(device);
   at::Tensor y = output(a[11], {rows, n}, a[10] == Py_None ? x.scalar_type() : scalar_type(a[10]), device);
+  if (a[11] != Py_None) need(!overlap(y, x), "out overlaps x");
   b2vx_linear_desc d = {};
   d.w_format = static_cast<int32_t>(format);
   d.x_dtype = dtype_code(x.scalar_type());
@@ -319,6 +330,7 @@ PyObject* combine(PyObject* const* a) {
   Call call(device);
   at::Tensor y = output(a[4], {tokens, n}, z.scalar_type(), device);
   need(y.scalar_type() == z.scalar_type(), "out must have z's type");
+  if (a[4] != Py_None) need(!overlap(y, z), "out overlaps z");
   const b2vx_combine_desc d = {dtype_code(z.scalar_type()), static_cast<uint32_t>(top_k), static_cast<uint64_t>(tokens), static_cast<uint64_t>(n),
                                static_cast<uint64_t>(z.size(0)), stride, r_stride, row_stride(y)};
   call(b2vx_combine_noalloc(&d, z.data_ptr(), static_cast<const int32_t*>(s), static_cast<const float*>(w), residual, y.data_ptr(), call.stream, call.err, sizeof(call.err)));

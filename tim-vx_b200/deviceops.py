@@ -10,7 +10,7 @@
 Work is queued on the current stream of the tensors' device and nothing waits for it.  Outputs and workspaces come from torch's allocator
 (give ``out`` for an output of your own; what quantize_fp4 and route_experts return shares one allocation).  Refused arguments raise pyb2vx.B2vxError with the library's message, tensors of a wrong type,
 shape or device raise ValueError; nothing is launched then.  Tensors whose last dimension is contiguous are used where they
-lie; a bias, scale or index tensor has to be contiguous.
+lie; a bias, scale or index tensor has to be contiguous.  ``out`` may be the residual of combine_experts, but must not overlap another input.
 """
 import collections
 
