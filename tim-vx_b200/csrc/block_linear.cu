@@ -102,6 +102,7 @@ struct alignas(16) Header {
   uint32_t tmem_base;
   int abort_flag;
   int num_tiles;
+  int scan[32];
 };
 // Behind the header, for each group and one more: first row, first tile, tiles along its rows, rows of each of them.
 struct Group {
@@ -403,42 +404,76 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   }
   // Behind the kernel that made the operand x, which began its work after everything before it had ended, only the loads of x wait.
   if (!p.after_operand) pdl_wait();
-  // The groups.  Offsets are device data that nobody has checked: they are cut to rising values among the rows that exist.
-  if (warp == 0) {
-    int high = 0, total = 0;
-    for (int e0 = 0; e0 <= p.experts; e0 += 32) {
-      const int e = e0 + lane;
-      int v = e < p.experts ? 0 : p.rows;
-      if (p.offsets) v = e <= p.experts ? min(max(p.offsets[e], 0), p.rows) : 0;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, v, d);
-        if (lane >= d) v = max(v, up);
-      }
-      v = max(v, high);
-      // this chunk's last value is the next chunk's first bound; group e - 1 ends at v
-      const int prev = __shfl_up_sync(0xffffffffu, v, 1);
-      const int from = lane ? prev : high;
-      high = __shfl_sync(0xffffffffu, v, 31);
-      const bool ends = e >= 1 && e <= p.experts;
-      const int row_tiles = ends ? (v - from + p.bn - 1) / p.bn : 0;
-      int sum = row_tiles * p.feature_tiles;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, sum, d);
-        if (lane >= d) sum += up;
-      }
-      if (e <= p.experts) {
-        groups[e].lo = v;
-        groups[e].start = total + sum;
-      }
-      if (ends) {
-        groups[e - 1].tiles = row_tiles;
-        groups[e - 1].per = rows_of_tile(v - from, p.bn);
-      }
-      total += __shfl_sync(0xffffffffu, sum, 31);
+  // The groups.  Offsets are device data that nobody has checked: they are cut to rising values among the rows that exist.  Up to three
+  // neighbouring offsets a thread, a scan of maxima and one of tiles over the whole block: a decode step waits for this (a warp alone, chunk
+  // by chunk, took 3 us for 128 experts).
+  if (!p.offsets) {
+    if (threadIdx.x == 0) {
+      const int n = (p.rows + p.bn - 1) / p.bn;
+      groups[0] = {0, 0, n, rows_of_tile(p.rows, p.bn)};
+      groups[1] = {p.rows, n * p.feature_tiles, 0, 0};
+      h->num_tiles = n * p.feature_tiles;
     }
-    if (lane == 0) h->num_tiles = total;
+  } else {
+    constexpr int kEach = (kMaxExperts + kThreads) / kThreads;
+    const int each = p.experts < kThreads ? 1 : kEach, first = static_cast<int>(threadIdx.x) * each;
+    int v[kEach], high = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      v[i] = 0;
+      if (i < each && first + i <= p.experts) v[i] = min(max(__ldg(p.offsets + first + i), 0), p.rows);
+      high = v[i] = max(high, v[i]);
+    }
+    int all = high;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, all, d);
+      if (lane >= d) all = max(all, up);
+    }
+    if (lane == 31) h->scan[warp] = all;
+    int from = __shfl_up_sync(0xffffffffu, all, 1);
+    if (lane == 0) from = 0;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w)
+      if (w < warp) from = max(from, h->scan[w]);
+    // entry first + i: where group first + i begins and the one before it ends
+    int tiles[kEach], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int e = first + i, begin = from;
+      from = max(from, v[i]);
+      tiles[i] = 0;
+      if (i >= each || e > p.experts) continue;
+      v[i] = from;
+      if (e == 0) continue;
+      const int count = from - begin, n = count <= p.bn ? (count ? 1 : 0) : (count + p.bn - 1) / p.bn;
+      groups[e - 1].tiles = n;
+      groups[e - 1].per = n > 1 ? rows_of_tile(count, p.bn) : (count + 31) / 32 * 32;
+      tiles[i] = n * p.feature_tiles;
+      sum += tiles[i];
+    }
+    int before = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, before, d);
+      if (lane >= d) before += up;
+    }
+    if (lane == 31) h->scan[16 + warp] = before;
+    before -= sum;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w)
+      if (w < warp) before += h->scan[16 + w];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      before += tiles[i];
+      if (i < each && first + i <= p.experts) {
+        groups[first + i].lo = v[i];
+        groups[first + i].start = before;
+        if (first + i == p.experts) h->num_tiles = before;
+      }
+    }
   }
   fence_before();
   if constexpr (CG == 1 && !SPLIT) __syncthreads();
