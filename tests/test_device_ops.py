@@ -208,3 +208,26 @@ def test_tensors_must_be_on_a_gpu():
         D.linear(torch.zeros(2, 32, dtype=torch.bfloat16), torch.zeros(8, 64, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="two dimensions"):
         D.combine_experts(torch.zeros(4, 8), torch.zeros(4, dtype=torch.int32), torch.zeros(4))
+
+
+def test_addresses_of_words_must_be_aligned():
+    lib, odd = ABI.library(), PTR + 2
+    d = desc(ABI.QuantizeDesc, QUANTIZE)
+    assert "aligned" in refused(lib.b2vx_fp4_quantize_noalloc, d, PTR, odd, None, PTR, PTR, None)
+    d = desc(ABI.QuantizeDesc, dict(QUANTIZE, format=2, scales_pitch=6))
+    assert "aligned" in refused(lib.b2vx_fp4_quantize_noalloc, d, PTR, None, odd, PTR, PTR, None)
+    d = desc(ABI.DequantizeDesc, dict(DEQUANTIZE, format=2, scales_pitch=6))
+    assert "aligned" in refused(lib.b2vx_fp4_dequantize_noalloc, d, PTR, PTR, odd, PTR, None)
+    d = desc(ABI.LinearDesc, dict(LINEAR, w_format=2, experts=4))
+    for name in ("bias", "x_scale", "w_scale", "offsets", "row_index"):
+        words = dict(dict(bias=PTR, x_scale=PTR, w_scale=PTR, offsets=PTR, row_index=PTR), **{name: odd})
+        a = desc(ABI.LinearArgs, dict(words, x=PTR, w=PTR, w_scales=PTR, y=PTR, workspace=PTR, workspace_bytes=1 << 30))
+        assert "aligned" in refused(lib.b2vx_linear_noalloc, C.byref(d), C.byref(a), None)
+    d = C.byref(desc(ABI.RouteDesc, ROUTE))
+    for i in range(1, 6):
+        args = [PTR] * 6
+        args[i] = odd
+        assert "aligned" in refused(lib.b2vx_route_noalloc, d, *args, PTR, 1 << 20, None)
+    d = C.byref(desc(ABI.CombineDesc, COMBINE))
+    for args in ((PTR, odd, PTR, PTR, PTR), (PTR, PTR, odd, PTR, PTR)):
+        assert "aligned" in refused(lib.b2vx_combine_noalloc, d, *args, None)

@@ -3,6 +3,8 @@
 Quantization is compared code by code and byte by byte.  Products: a kernel adds float32 partial sums, one for every 16 to 64 columns of K, each
 rounded (or cut) to 2^-23 of at most S = sum |x w| |alpha| + |bias|, so a result may be off by (k / 16 + 4) 2^-23 S and half a step of its type."""
 import ctypes as C
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -808,3 +810,40 @@ def test_results_do_not_depend_on_the_run():
         y, r, _, _ = layer(x)
         for a, b in zip(first, (y, *r)):
             assert torch.equal(a, b)
+
+
+FIRST = """
+import sys
+sys.path[:0] = %r
+import torch, deviceops as D
+torch.manual_seed(0)
+x, w = (torch.randn(n, 64, device="cuda").bfloat16() for n in (5, 24))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = D.linear(x, w)
+g.replay()
+D.check("cuda")
+want = x.double() @ w.double().T
+assert ((y.double() - want).abs() <= want.abs() * 2.0 ** -8 + 1e-4).all()
+print("same")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    # sums of 64 products of at most 25 or so: float32 is off by less than 1e-4
+    out = subprocess.run([sys.executable, "-c", FIRST % sys.path], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip() == "same", out.stderr
+
+
+def test_no_memory_is_torchs_own_error():
+    x = torch.zeros(8192, 32, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(1 << 17, 32, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.empty_cache()
+    torch.cuda.set_per_process_memory_fraction(0.005)   # 0.9 GB; the result has 2
+    try:
+        with pytest.raises(torch.cuda.OutOfMemoryError):
+            D.linear(x, w)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert not D.linear(x, w[:64]).any()

@@ -13,6 +13,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cstdint>
 #include <stdexcept>
 #include <string>
 
@@ -233,7 +234,7 @@ PyObject* product(PyObject* const* a) {
   need(w.is_contiguous(), "weight must be contiguous");
   need(w.device() == device, "weight is on another device");
   const int64_t experts = w.dim() == 3 ? w.size(0) : 0, w_rows = w.size(-2), k = format ? w.size(-1) * 2 : w.size(-1);
-  need(w.dim() == 2 || experts > 0, "weight has no experts");
+  need(w.dim() == 2 || (experts > 0 && experts <= UINT32_MAX), "weight has no experts or too many");
   b2vx_linear_args p = {};
   if (format) {
     need(w.scalar_type() == at::kByte, "codes must have the type uint8");
@@ -285,6 +286,7 @@ PyObject* route(PyObject* const* a) {
   const int64_t tokens = logits.size(0), experts = logits.size(1);
   const at::Device device = logits.device();
   need(top_k >= 0 && top_k <= 1024, "top_k is out of range");
+  need(experts <= UINT32_MAX, "logits has too many columns");
   Call call(device);
   const b2vx_route_desc d = {dtype_code(logits.scalar_type()), normalize != 0, static_cast<uint32_t>(experts), static_cast<uint32_t>(top_k), static_cast<uint64_t>(tokens), stride};
   size_t bytes = 0;
@@ -314,6 +316,7 @@ PyObject* combine(PyObject* const* a) {
   const uint64_t stride = rows_of(z, "z");
   const at::Tensor& slots = tensor(a[1], "slots");
   need(slots.dim() == 2, "slots must be a tensor of two dimensions");
+  need(slots.size(1) <= 1024, "top_k is out of range");
   const int64_t tokens = slots.size(0), top_k = slots.size(1), n = z.size(1);
   const at::Device device = z.device();
   const void* s = dense(a[1], "slots", at::kInt, {tokens, top_k}, device);
@@ -348,6 +351,13 @@ PyObject* check(PyObject* const* a) {
   Py_RETURN_NONE;
 }
 
+PyObject* attribute(const char* module, const char* name) {
+  PyObject* m = PyImport_ImportModule(module);
+  PyObject* a = m ? PyObject_GetAttrString(m, name) : nullptr;
+  Py_XDECREF(m);
+  return a;
+}
+
 template <PyObject* (*FN)(PyObject* const*), int ARGS>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
   if (count != ARGS) {
@@ -357,15 +367,17 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
   try {
     return FN(args);
   } catch (const Refused& r) {
-    PyObject* module = PyImport_ImportModule("pyb2vx");
-    PyObject* type = module ? PyObject_GetAttrString(module, "B2vxError") : nullptr;
+    PyObject* type = attribute("pyb2vx", "B2vxError");
     PyObject* error = type ? PyObject_CallFunction(type, "is", r.status, r.message.c_str()) : nullptr;
     if (error) PyErr_SetObject(type, error);
     Py_XDECREF(error);
     Py_XDECREF(type);
-    Py_XDECREF(module);
   } catch (const std::invalid_argument& e) {
     PyErr_SetString(PyExc_ValueError, e.what());
+  } catch (const c10::OutOfMemoryError& e) {
+    PyObject* type = attribute("torch", "OutOfMemoryError");
+    if (type) PyErr_SetString(type, e.what_without_backtrace());
+    Py_XDECREF(type);
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());
   }

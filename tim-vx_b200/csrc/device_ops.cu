@@ -1,6 +1,7 @@
 // The entry points of the operators on device tensors: argument checks, workspace layout, launches.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <climits>
 #include <cstdio>
 #include <cstring>
@@ -20,14 +21,13 @@ constexpr uint64_t kMaxStride = 1ull << 40;     // elements or bytes; keeps byte
 // Status words the products write a code to when they give up on a barrier, one per GPU, in page-locked memory of the library's own.
 alignas(4096) int g_status[4096 / sizeof(int)];
 struct PerDevice {
-  std::once_flag once;
-  cudaError_t error = cudaSuccess;
+  std::atomic<bool> ready{false};
   int* status = nullptr;
   int sm_count = 0;
 };
 PerDevice g_devices[kMaxDevices];
-std::once_flag g_registered;
-cudaError_t g_register_error = cudaSuccess;
+std::mutex g_mutex;          // of the first call on each GPU
+bool g_registered = false;
 
 b2vx_status fail(char* err, size_t err_len, b2vx_status st, const char* msg) {
   if (err && err_len) std::snprintf(err, err_len, "%s", msg);
@@ -53,16 +53,26 @@ b2vx_status device(PerDevice** out, char* err, size_t err_len) {
     cudaGetLastError();
     return fail(err, err_len, B2VX_CUDA_ERROR, "no CUDA device");
   }
-  std::call_once(g_registered, [] { g_register_error = cudaHostRegister(g_status, sizeof(g_status), cudaHostRegisterPortable | cudaHostRegisterMapped); });
   PerDevice& d = g_devices[dev];
-  std::call_once(d.once, [&] {
-    d.error = g_register_error;
-    void* p = nullptr;
-    if (d.error == cudaSuccess) d.error = cudaHostGetDevicePointer(&p, g_status, 0);
-    if (d.error == cudaSuccess) d.error = cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, dev);
-    d.status = static_cast<int*>(p) + dev;
-  });
-  if (d.error != cudaSuccess) return fail(err, err_len, B2VX_CUDA_ERROR, cudaGetErrorString(d.error));
+  if (!d.ready.load(std::memory_order_acquire)) {
+    std::lock_guard<std::mutex> lock(g_mutex);
+    // the first call may be one that is being captured, where registering memory is refused in other modes
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e == cudaSuccess) {
+      if (!g_registered) e = cudaHostRegister(g_status, sizeof(g_status), cudaHostRegisterPortable | cudaHostRegisterMapped);
+      void* p = nullptr;
+      if (e == cudaSuccess) {
+        g_registered = true;
+        e = cudaHostGetDevicePointer(&p, g_status, 0);
+      }
+      if (e == cudaSuccess) e = cudaDeviceGetAttribute(&d.sm_count, cudaDevAttrMultiProcessorCount, dev);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      d.status = static_cast<int*>(p) + dev;
+    }
+    if (e != cudaSuccess) return launched(e, err, err_len);
+    d.ready.store(true, std::memory_order_release);
+  }
   *out = &d;
   return B2VX_OK;
 }
@@ -148,7 +158,7 @@ extern "C" b2vx_status b2vx_fp4_quantize_noalloc(const b2vx_fp4_quantize_desc* d
   B2VX_NEED(row_index || d->rows <= d->x_rows, "more rows than x has, and no row_index");
   if (d->rows == 0 || d->k == 0) return B2VX_OK;
   B2VX_NEED(codes && scales && (x || d->x_rows == 0), "null argument");
-  B2VX_NEED(aligned(x, size_of(d->x_dtype)) && aligned(codes, 4), "a pointer is not aligned");
+  B2VX_NEED(aligned(x, size_of(d->x_dtype)) && aligned(codes, 4) && aligned(row_index, 4) && aligned(tensor_scale, 4), "a pointer is not aligned");
   PerDevice* pd;
   b2vx_status st = device(&pd, err, err_len);
   if (st != B2VX_OK) return st;
@@ -175,7 +185,7 @@ extern "C" b2vx_status b2vx_fp4_dequantize_noalloc(const b2vx_fp4_dequantize_des
   B2VX_NEED((tensor_scale != nullptr) == (d->format == B2VX_FP4_BLOCK16), "a tensor scale belongs to B2VX_FP4_BLOCK16 and only to it");
   if (d->rows == 0 || d->k == 0) return B2VX_OK;
   B2VX_NEED(codes && scales && y, "null argument");
-  B2VX_NEED(aligned(y, size_of(d->y_dtype)) && aligned(codes, 4), "a pointer is not aligned");
+  B2VX_NEED(aligned(y, size_of(d->y_dtype)) && aligned(codes, 4) && aligned(tensor_scale, 4), "a pointer is not aligned");
   PerDevice* pd;
   b2vx_status st = device(&pd, err, err_len);
   if (st != B2VX_OK) return st;
@@ -225,6 +235,7 @@ extern "C" b2vx_status b2vx_linear_noalloc(const b2vx_linear_desc* d, const b2vx
   if (d->rows == 0 || d->n == 0) return B2VX_OK;
   B2VX_NEED(a->w && a->y && (a->x || d->x_rows == 0) && (!fp4 || a->w_scales), "null argument");
   B2VX_NEED(aligned(a->w, 16) && aligned(a->w_scales, 16) && aligned(a->x, size_of(d->x_dtype)) && aligned(a->y, size_of(d->y_dtype)), "a pointer is not aligned");
+  B2VX_NEED(aligned(a->bias, 4) && aligned(a->x_scale, 4) && aligned(a->w_scale, 4) && aligned(a->offsets, 4) && aligned(a->row_index, 4), "a pointer is not aligned");
   const Workspace ws = workspace_of(*d);
   // 16-bit rows that TMA can read where they lie need no workspace
   const bool direct = !fp4 && !a->row_index && aligned(a->x, 16) && d->x_stride % 8 == 0;
@@ -296,6 +307,7 @@ extern "C" b2vx_status b2vx_route_noalloc(const b2vx_route_desc* d, const void* 
   B2VX_NEED(d->normalize == 0 || d->normalize == 1, "normalize must be 0 or 1");
   B2VX_NEED(d->logits_stride >= d->experts && d->logits_stride <= kMaxStride, "logits_stride is smaller than a row or out of range");
   B2VX_NEED(offsets, "null argument");
+  B2VX_NEED(aligned(offsets, 4) && aligned(ids, 4) && aligned(weights, 4) && aligned(row_index, 4) && aligned(slots, 4), "a pointer is not aligned");
   cudaStream_t s = static_cast<cudaStream_t>(cuda_stream);
   PerDevice* pd;
   if (d->tokens == 0) {   // no rows: every expert starts at 0
@@ -320,7 +332,7 @@ extern "C" b2vx_status b2vx_combine_noalloc(const b2vx_combine_desc* d, const vo
   B2VX_NEED(d->z_stride <= kMaxStride && d->y_stride <= kMaxStride && d->residual_stride <= kMaxStride, "a stride is out of range");
   if (d->tokens == 0 || d->n == 0) return B2VX_OK;
   B2VX_NEED(y && (d->top_k == 0 || (slots && weights)) && (z || d->z_rows == 0), "null argument");
-  B2VX_NEED(aligned(z, size_of(d->dtype)) && aligned(y, size_of(d->dtype)) && aligned(residual, size_of(d->dtype)), "a pointer is not aligned");
+  B2VX_NEED(aligned(z, size_of(d->dtype)) && aligned(y, size_of(d->dtype)) && aligned(residual, size_of(d->dtype)) && aligned(slots, 4) && aligned(weights, 4), "a pointer is not aligned");
   PerDevice* pd;
   b2vx_status st = device(&pd, err, err_len);
   if (st != B2VX_OK) return st;

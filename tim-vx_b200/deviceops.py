@@ -20,7 +20,6 @@ import deviceops_native as _native
 
 FORMATS = {"block32": 1, "block16": 2}
 BLOCK = {"block32": 32, "block16": 16}
-MAX_EXPERTS = 1024
 
 # codes uint8 [rows][(k rounded up to 32) / 2], scales uint8 [rows][blocks]; scale: the tensor's scale (block16) or None
 Fp4Rows = collections.namedtuple("Fp4Rows", "codes scales k format scale")
@@ -110,5 +109,6 @@ def combine_experts(z, slots, weights, residual=None, out=None):
 
 
 def check(device=None):
-    """Waits for the current stream; raises where a product on that GPU gave up on a barrier."""
-    _native.check(torch.cuda.current_device() if device is None else torch.device(device).index or 0)
+    """Waits for the current stream of a GPU (the current one, unless device names another); raises where a product there gave up on a barrier."""
+    index = None if device is None else torch.device(device).index
+    _native.check(torch.cuda.current_device() if index is None else index)
