@@ -336,11 +336,8 @@ __device__ __forceinline__ void quantize_part(const LinearParams& p, int kb, int
 #pragma unroll
       for (int i = 0; i < 16; ++i) t.v[i] = c + i < p.k ? row[c + i] : from_float<X>(0.0f);
     }
-    float v[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = to_float(t.v[i]);
     uint32_t byte;
-    const uint2 code = quantize_16<KIND>(v, top_of(t), scale, byte, [&](int i) { return to_float(row[c + i]); });
+    const uint2 code = quantize_16<KIND>(t, scale, byte, [&](int i) { return to_float(row[c + i]); });
     if (c >= p.k) byte = 0;
     const uint32_t word = scale_word<KIND>(byte);
     if (block >= blocks) continue;

@@ -14,7 +14,7 @@
 namespace b2vx {
 
 // Eight floats to e2m1 codes (nearest even, cut to +-6), element i in bits 4 i.
-__device__ __forceinline__ uint32_t e2m1_codes(const float (&v)[8]) {
+__device__ __forceinline__ uint32_t e2m1_codes(const float* v) {
   uint32_t r;
   asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
       "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
@@ -116,6 +116,13 @@ __device__ __forceinline__ Sixteen<T> load_16(const T* row, int c, int k, uint4*
   }
   return t;
 }
+template <typename T>
+__device__ __forceinline__ Sixteen<T> load_whole(const T* from) {
+  Sixteen<T> t;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(t) / 16); ++i) reinterpret_cast<uint4*>(&t)[i] = __ldg(reinterpret_cast<const uint4*>(from) + i);
+  return t;
+}
 // The largest magnitude, as float bits.
 template <typename T>
 __device__ __forceinline__ uint32_t top_of(const Sixteen<T>& t) {
@@ -202,55 +209,61 @@ __device__ __forceinline__ uint32_t settle_codes(uint32_t codes, uint32_t diff, 
 }
 
 // The block's scale byte and the codes of this lane's sixteen numbers: a block of block16, or half of one of block32, whose other half is
-// the neighbouring lane's.  top: the largest magnitude of the lane's numbers, as bits (NaN is above infinity is above everything else).
-// number(i): the lane's i-th number once more, for the few that need it.
-template <int FORMAT, typename F>
-__device__ __forceinline__ uint2 quantize_16(const float (&v)[16], uint32_t top, const TensorScale& t, uint32_t& byte, F number) {
-  if (FORMAT == B2VX_FP4_BLOCK32) {
+// the neighbouring lane's.  number(i): the lane's i-th number once more, for the few that need it.
+template <int FORMAT, typename T, typename F>
+__device__ __forceinline__ uint2 quantize_16(const Sixteen<T>& x, const TensorScale& t, uint32_t& byte, F number) {
+  uint32_t top = top_of(x);         // as bits: NaN is above infinity is above everything else
+  float v[16];
+  if constexpr (FORMAT == B2VX_FP4_BLOCK32) {
     top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     const int e = static_cast<int>(top >> 23) - 2;            // biased exponent of 2^(floor(log2 amax) - 2)
     byte = static_cast<uint32_t>(max(e, 0));
     const float f = __uint_as_float((254u - min(byte, 253u)) << 23);   // a power of two: the products are exact
-    uint2 codes = make_uint2(e2m1_codes_times(v, f), e2m1_codes_times(v + 8, f));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = to_float(x.v[i]) * f;
+    uint2 codes = make_uint2(e2m1_codes(v), e2m1_codes(v + 8));
     if (top >= 0x7f800000u) {
       byte = 255u;
       codes = make_uint2(0u, 0u);
     }
     return codes;
-  }
-  // amax / (6 g) as a product of three roundings is off by less than 2^-22 of itself: where a little less and a little more round to
-  // the same byte, that is the answer, else the border between them, as in settle_codes.
-  constexpr float kLess = 1.0f - 0x1p-20f, kMore = 1.0f + 0x1p-20f;
-  const float amax = __uint_as_float(top) * t.lift;
-  const float q = amax * t.over_6g;
-  const uint32_t two = e4m3_bytes(q * kLess, q * kMore);
-  byte = two >> 8;
-  if ((two & 0xff) != byte) {
-    const float border6 = 3.0f * (e4m3_value(two & 0xff) + e4m3_value(byte));
-    const float r = fmaf(border6, t.g, -amax);
-    if (r > 0.0f || (r == 0.0f && (byte & 1u))) byte = two & 0xff;
-  }
-  const float s = e4m3_value(byte);
-  float over_s;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(over_s) : "f"(s));   // off by 2^-23; s = 0 is dealt with below
-  // The numbers over s g: the approximate reciprocal, two products and 1 / g are off by less than 2^-21 together.
-  const float inv = over_s * t.over_g * t.lift, less = inv * kLess, more = inv * kMore;
-  const uint32_t near = __shfl_sync(0xffffffffu, t.near, (__float_as_uint(s) >> 20) & 7);
-  const float f = near == 2u ? more : less;
-  uint2 codes = make_uint2(e2m1_codes_times(v, f), e2m1_codes_times(v + 8, f));
-  if (near == 3u) {
-    const uint2 up = make_uint2(e2m1_codes_times(v, more), e2m1_codes_times(v + 8, more));
-    if ((codes.x != up.x || codes.y != up.y) && byte != 0) {
-      codes.x = settle_codes(codes.x, codes.x ^ up.x, s, t.g, t.lift, number);
-      codes.y = settle_codes(codes.y, codes.y ^ up.y, s, t.g, t.lift, [&](int i) { return number(8 + i); });
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = to_float(x.v[i]);
+    // amax / (6 g) as a product of three roundings is off by less than 2^-22 of itself: where a little less and a little more round to
+    // the same byte, that is the answer, else the border between them, as in settle_codes.
+    constexpr float kLess = 1.0f - 0x1p-20f, kMore = 1.0f + 0x1p-20f;
+    const float amax = __uint_as_float(top) * t.lift;
+    const float q = amax * t.over_6g;
+    const uint32_t two = e4m3_bytes(q * kLess, q * kMore);
+    byte = two >> 8;
+    if ((two & 0xff) != byte) {
+      const float border6 = 3.0f * (e4m3_value(two & 0xff) + e4m3_value(byte));
+      const float r = fmaf(border6, t.g, -amax);
+      if (r > 0.0f || (r == 0.0f && (byte & 1u))) byte = two & 0xff;
     }
+    const float s = e4m3_value(byte);
+    float over_s;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(over_s) : "f"(s));   // off by 2^-23; s = 0 is dealt with below
+    // The numbers over s g: the approximate reciprocal, two products and 1 / g are off by less than 2^-21 together.
+    const float inv = over_s * t.over_g * t.lift, less = inv * kLess, more = inv * kMore;
+    const uint32_t near = __shfl_sync(0xffffffffu, t.near, (__float_as_uint(s) >> 20) & 7);
+    const float f = near == 2u ? more : less;
+    uint2 codes = make_uint2(e2m1_codes_times(v, f), e2m1_codes_times(v + 8, f));
+    if (near == 3u) {
+      const uint2 up = make_uint2(e2m1_codes_times(v, more), e2m1_codes_times(v + 8, more));
+      if ((codes.x != up.x || codes.y != up.y) && byte != 0) {
+        codes.x = settle_codes(codes.x, codes.x ^ up.x, s, t.g, t.lift, number);
+        codes.y = settle_codes(codes.y, codes.y ^ up.y, s, t.g, t.lift, [&](int i) { return number(8 + i); });
+      }
+    }
+    if (byte == 0) codes = make_uint2(0u, 0u);                  // every number rounds to zero
+    if (top >= 0x7f800000u || !t.ok) {
+      byte = 127u;
+      codes = make_uint2(0u, 0u);
+    }
+    return codes;
   }
-  if (byte == 0) codes = make_uint2(0u, 0u);                  // every number rounds to zero
-  if (top >= 0x7f800000u || !t.ok) {
-    byte = 127u;
-    codes = make_uint2(0u, 0u);
-  }
-  return codes;
 }
 
 // Four neighbouring blocks' bytes as a word, in the first of their lanes.

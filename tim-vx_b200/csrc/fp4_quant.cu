@@ -1,9 +1,10 @@
 // Rows of numbers to 4-bit block floating point and back, packing of scales, gathering of rows.
 //
-// Quantization reads every number once and writes half a byte and a scale's share for it; memory bounds block32, the instructions of
-// the two-sided rounding block16.  Sixteen columns a lane: a block of block16, so that its scale, some forty instructions, is worked out
-// once, or half a block of block32.
+// Quantization reads every number once and writes half a byte and a scale's share for it: 8192 x 8192 bfloat16 numbers to block32 in 34 us,
+// to block16 in 38 (26 are the bytes'), 32-bit numbers in 49 (46), bound by instructions between rounding and memory.
+// Sixteen columns a lane: a block of block16, so that its scale, some forty instructions, is worked out once, or half a block of block32.
 #include <algorithm>
+#include <climits>
 
 #include "block_linear.cuh"
 #include "fp4.cuh"
@@ -13,9 +14,9 @@ namespace b2vx {
 namespace {
 
 constexpr int kWarps = 8;
-// Blocks of a quantization kernel an SM: what 64 registers a thread leave (block16, which works longer on a chunk and asks for two ahead)
-// or 48.  8192 x 8192 16-bit numbers to block32 41 us with five, 46 with four and two chunks ahead; to block16 46 and 46 - 54.
-constexpr int quantize_blocks(int format) { return format == B2VX_FP4_BLOCK16 ? 4 : 5; }
+// Blocks of a quantization kernel an SM: what 48 registers a thread leave, or 64 where 32-bit numbers would not fit beside block16's
+// rounding (8192 x 8192 to block16: 50 us with four, 58 with five).  8192 x 8192 bfloat16 numbers with five / four: to block32 34 / 42 us, to block16 38 / 42.
+constexpr int quantize_blocks(int format, size_t elem) { return format == B2VX_FP4_BLOCK16 && elem == 4 ? 4 : 5; }
 // Rows that several rows of an operand refer to (a token's, for each of its experts) are quantized once and then copied, where that saves
 // more than the second launch costs: measured at 8192 rows of 1408 columns taken four times each.
 constexpr long long kTwiceElements = 1 << 22;
@@ -46,7 +47,7 @@ __device__ __forceinline__ uint8_t* packed_place(const QuantizeArgs& a, uint32_t
 
 // `split` warps share a row, each taking every split-th chunk.
 template <typename T, int FORMAT, bool VEC, bool PACKED>
-__global__ void __launch_bounds__(kWarps * 32, quantize_blocks(FORMAT)) quantize_kernel(const QuantizeArgs a, int chunks, int split) {
+__global__ void __launch_bounds__(kWarps * 32, quantize_blocks(FORMAT, sizeof(T))) quantize_kernel(const QuantizeArgs a, int chunks, int split) {
   constexpr int B = fp4_block(FORMAT), LANES = B / 16, PER = scale_words_per_stage(FORMAT);   // lanes to a block, words to a k-block
   pdl_wait();
   pdl_trigger();   // after the wait: a product behind this kernel may read its weights before its own wait
@@ -66,37 +67,42 @@ __global__ void __launch_bounds__(kWarps * 32, quantize_blocks(FORMAT)) quantize
     const int k_here = there ? k : 0;
     uint8_t* codes_row = a.codes + row * a.codes_pitch;
     int c = part * kChunk + lane * 16;
-    // one or two chunks are under way while one is worked on
-    constexpr bool kTwo = FORMAT == B2VX_FP4_BLOCK16 && sizeof(T) == 2;
-    const int step = split * kChunk;
-    Sixteen<T> t = load_16<T, VEC>(from, c, k_here, staging, lane), ahead = t;
-    if (kTwo && part + split < chunks) ahead = load_16<T, VEC>(from, c + step, k_here, staging, lane);
-    uint8_t* tile = PACKED ? packed_place<FORMAT>(a, row, lane) : nullptr;
+    const int step = split * kChunk, whole = k_here / kChunk;      // chunks with no column behind the row's end
+    auto load = [&](int chunk, int at) {
+      return VEC && chunk < whole ? load_whole(from + at) : load_16<T, VEC>(from, at, k_here, staging, lane);
+    };
+    Sixteen<T> t = load(part, c);
+    uint8_t* tile = nullptr;
+    long long tile_step = 0;
+    if (PACKED) {       // this lane's word of its first chunk's scales; a chunk is two k-blocks
+      const long long block = static_cast<long long>(a.scale_tiles) * (PER * kScaleTile);
+      tile = packed_place<FORMAT>(a, row, lane);
+      if (lane % (4 * LANES) != 0) tile = nullptr;
+      if (tile) tile += (2 * part + lane / 16) * block + lane % 16 / (4 * LANES) * kScaleTile;
+      tile_step = 2 * split * block;
+    }
     for (int chunk = part; chunk < chunks; chunk += split) {
       Sixteen<T> next = t;
-      if (chunk + (kTwo ? 2 : 1) * split < chunks) next = load_16<T, VEC>(from, c + (kTwo ? 2 : 1) * step, k_here, staging, lane);
-      float v[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = to_float(t.v[i]);
+      if (chunk + split < chunks) next = load(chunk + split, c + step);
       uint32_t byte;
-      const uint2 codes = quantize_16<FORMAT>(v, top_of(t), scale, byte, [&](int i) { return to_float(from[c + i]); });
-      if (c < k32) {
-        // k32 is a multiple of 32, c of 16: all sixteen codes lie inside the row
+      const uint2 codes = quantize_16<FORMAT>(t, scale, byte, [&](int i) { return to_float(from[c + i]); });
+      // k32 is a multiple of 32, c of 16: all sixteen codes lie inside the row or none; an operand's k is a multiple of 32
+      if (chunk < whole || c < k32) {
         uint32_t* to = reinterpret_cast<uint32_t*>(codes_row + c / 2);
-        if (a.codes_pitch % 8 == 0) *reinterpret_cast<uint2*>(to) = codes;
+        if (PACKED || a.codes_pitch % 8 == 0) *reinterpret_cast<uint2*>(to) = codes;
         else { to[0] = codes.x; to[1] = codes.y; }
       }
       if (PACKED) {
-        if (c >= k) byte = 0;
+        if (chunk >= whole && c >= k) byte = 0;
         const uint32_t word = scale_word<FORMAT>(byte);
-        const int k_block = c / 256, w = lane % 16 / (4 * LANES);
-        if (lane % (4 * LANES) == 0 && tile && k_block * 256 < k)
-          *reinterpret_cast<uint32_t*>(tile + (static_cast<long long>(k_block) * a.scale_tiles * PER + w) * kScaleTile) = word;
+        if (tile) {
+          if (c / 256 * 256 < k) *reinterpret_cast<uint32_t*>(tile) = word;
+          tile += tile_step;
+        }
       } else if (lane % LANES == 0 && c / B < blocks) {
         a.scales[row * a.scales_pitch + c / B] = static_cast<uint8_t>(byte);
       }
-      t = kTwo ? ahead : next;
-      ahead = next;
+      t = next;
       c += step;
     }
   }
@@ -246,13 +252,30 @@ int split_of(long long rows, int chunks) {
   const long long fill = 4 * 148 * 40;
   return static_cast<int>(std::max<long long>(1, std::min<long long>(chunks, fill / std::max<long long>(1, rows))));
 }
+// The same for a product's operand, where a row's start costs about as much as a chunk (the place of its scales): rounds of `warps` units, each
+// as long as its chunks and one more; of the splits that fill 1 to 8 rounds the one whose rounds together are shortest.  2048 x 8192 numbers
+// and a product with 128 features: 27 us by the rule above, 24 by this one.
+int operand_split_of(long long rows, int chunks, int warps) {
+  long long best = 1, least = LLONG_MAX;
+  for (int round = 1; round <= 8; ++round) {
+    const long long split = std::max<long long>(1, std::min<long long>(chunks, static_cast<long long>(warps) * round / rows));
+    const long long cost = (rows * split + warps - 1) / warps * ((chunks + split - 1) / split + 1);
+    if (cost < least) {
+      least = cost;
+      best = split;
+    }
+  }
+  return static_cast<int>(best);
+}
 
 template <typename T, int FORMAT, bool VEC>
 cudaError_t quantize(const QuantizeArgs& a, cudaStream_t s) {
   const int chunks = static_cast<int>((a.k + kChunk - 1) / kChunk);
-  const int split = split_of(a.rows, chunks);
-  const int grid = blocks_for(a.rows * split, kWarps, quantize_blocks(FORMAT));
-  if (a.scales_pitch == 0) return launch_pdl(quantize_kernel<T, FORMAT, VEC, true>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
+  constexpr int kBlocks = quantize_blocks(FORMAT, sizeof(T));
+  const bool operand = a.scales_pitch == 0;
+  const int split = operand ? operand_split_of(a.rows, chunks, 148 * kBlocks * kWarps) : split_of(a.rows, chunks);
+  const int grid = blocks_for(a.rows * split, kWarps, kBlocks);
+  if (operand) return launch_pdl(quantize_kernel<T, FORMAT, VEC, true>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
   return launch_pdl(quantize_kernel<T, FORMAT, VEC, false>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
 }
 template <typename T, int FORMAT>
