@@ -4,7 +4,7 @@
 // pairs are one 32-bit mask: the number of a pair among those of its 32 tokens is a population count, and neither it nor the
 // order of the result depends on the order in which masks were put together.
 // A warp chooses for one token; 32 tokens to a block.  Up to 128 tokens one block does everything (16 tokens, 8 of 128 experts: one
-// launch of 4 us instead of three); else
+// launch, 3.2 us, instead of three); else
 //   choose   ids, weights, masks [32-token block][expert]
 //   before   a lane per expert, the blocks shared by 32 warps: pairs before each block, pairs of each expert
 //   place    first rows of the experts from those, then a thread per pair
