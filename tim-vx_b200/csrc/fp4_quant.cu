@@ -16,7 +16,8 @@ namespace {
 constexpr int kWarps = 8;
 // Blocks of a quantization kernel an SM: what 48 registers a thread leave, or 64 where 32-bit numbers would not fit beside block16's
 // rounding (8192 x 8192 to block16: 50 us with four, 58 with five).  8192 x 8192 bfloat16 numbers with five / four: to block32 34 / 42 us, to block16 38 / 42.
-constexpr int quantize_blocks(int format, size_t elem) { return format == B2VX_FP4_BLOCK16 && elem == 4 ? 4 : 5; }
+// A product's operand in block16 is most often a few rows, where the registers count: 24 rows through 8192 x 8192 13.2 us with five, 12.8 with four.
+constexpr int quantize_blocks(int format, size_t elem, bool packed) { return format == B2VX_FP4_BLOCK16 && (elem == 4 || packed) ? 4 : 5; }
 // Rows that several rows of an operand refer to (a token's, for each of its experts) are quantized once and then copied, where that saves
 // more than the second launch costs: measured at 8192 rows of 1408 columns taken four times each.
 constexpr long long kTwiceElements = 1 << 22;
@@ -47,7 +48,7 @@ __device__ __forceinline__ uint8_t* packed_place(const QuantizeArgs& a, uint32_t
 
 // `split` warps share a row, each taking every split-th chunk.
 template <typename T, int FORMAT, bool VEC, bool PACKED>
-__global__ void __launch_bounds__(kWarps * 32, quantize_blocks(FORMAT, sizeof(T))) quantize_kernel(const QuantizeArgs a, int chunks, int split) {
+__global__ void __launch_bounds__(kWarps * 32, quantize_blocks(FORMAT, sizeof(T), PACKED)) quantize_kernel(const QuantizeArgs a, int chunks, int split) {
   constexpr int B = fp4_block(FORMAT), LANES = B / 16, PER = scale_words_per_stage(FORMAT);   // lanes to a block, words to a k-block
   pdl_wait();
   pdl_trigger();   // after the wait: a product behind this kernel may read its weights before its own wait
@@ -271,8 +272,8 @@ int operand_split_of(long long rows, int chunks, int warps) {
 template <typename T, int FORMAT, bool VEC>
 cudaError_t quantize(const QuantizeArgs& a, cudaStream_t s) {
   const int chunks = static_cast<int>((a.k + kChunk - 1) / kChunk);
-  constexpr int kBlocks = quantize_blocks(FORMAT, sizeof(T));
   const bool operand = a.scales_pitch == 0;
+  const int kBlocks = quantize_blocks(FORMAT, sizeof(T), operand);
   const int split = operand ? operand_split_of(a.rows, chunks, 148 * kBlocks * kWarps) : split_of(a.rows, chunks);
   const int grid = blocks_for(a.rows * split, kWarps, kBlocks);
   if (operand) return launch_pdl(quantize_kernel<T, FORMAT, VEC, true>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
