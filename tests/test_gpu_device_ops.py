@@ -847,3 +847,22 @@ def test_no_memory_is_torchs_own_error():
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     assert not D.linear(x, w[:64]).any()
+
+
+@pytest.mark.parametrize("rows,k", [(3, 1024), (40, 64)])
+def test_gate_far_below_zero(rows, k):
+    """silu of numbers around -88, whose exponentials leave float32's normal range, times numbers that bring the result back into it."""
+    # Sums are of one product, exact.  The exponential is off by two steps or half the smallest float32, the division by two steps, two products
+    # and a sum by half a step each or half the smallest float32.
+    gates = [-126.0, -103.5, -100.0, -90.0, -88.75, -88.5, -88.0, -87.5, -87.0, -20.0, -0.5, 0.0, 0.5, 20.0, 88.5, 126.0]
+    n = len(gates)
+    u = 2.0 ** 100
+    w = torch.zeros(1, 2 * n, k, dtype=torch.bfloat16, device="cuda")
+    w[0, :n, 0], w[0, n:, 0] = torch.tensor(gates), u
+    g = f64(w[0, :n, 0])                           # -88.75 is -89 in bfloat16
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = 1.0
+    y = D.expert_linear(x, w, torch.tensor([0, rows], dtype=torch.int32, device="cuda"), gated=True, out_dtype=torch.float32)
+    want = silu(g) * u
+    off = (4 * 2.0 ** -23 + 3 * 2.0 ** -24) * np.abs(want) + (np.abs(g) + 1) * 2.0 ** -150 * u
+    assert (np.abs(f64(y) - want) <= off).all()

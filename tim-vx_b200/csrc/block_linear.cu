@@ -316,7 +316,12 @@ __device__ __noinline__ void store_elements(T* to, long long step, uint32_t from
       reinterpret_cast<uint16_t*>(to)[k] = v;
     }
 }
-__device__ __forceinline__ float gate(float g, float u) { return __fdividef(g, 1.0f + expf(-g)) * u; }
+// silu(g) u.  The exponential is at most 1, so the divisor lies in [1, 2]: that of -g leaves __fdividef's range from g = -87.4 on, where 0 came out
+// for results that a large u makes ordinary numbers.
+__device__ __forceinline__ float gate(float g, float u) {
+  const float t = expf(-fabsf(g));
+  return __fdividef(g < 0.0f ? g * t : g, 1.0f + t) * u;
+}
 
 // RAW: k-blocks kb .. kb + blocks - 1 of the rows of x into shared memory, as the loads of a quantized x would put them there (16-byte pieces
 // exchanged by the row's number: the 128-byte swizzle).  A warp takes two k-blocks of a row at a time.  Rows up to 15 that do not
