@@ -341,7 +341,7 @@ b2vx_status b2vx_conv2d_first_layer_noalloc(const b2vx_conv2d_noalloc_desc* d, c
 enum { B2VX_FP4_BLOCK32 = 1, B2VX_FP4_BLOCK16 = 2 };
 
 /* x [x_rows][x_stride] (float32, float16 or bfloat16) to codes [rows][codes_pitch]
- * and scales.  codes_pitch (bytes): a multiple of 4, at least k rounded up to 32,
+ * (4-byte aligned) and scales.  codes_pitch (bytes): a multiple of 4, at least k rounded up to 32,
  * over 2; columns from k to there get code 0.  scales_pitch (bytes): at
  * least ceil(k / block).  row_index (int32 [rows], may be NULL): output row i is
  * row row_index[i] of x, a row of zeros where that is outside 0..x_rows-1.

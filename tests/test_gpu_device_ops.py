@@ -866,3 +866,29 @@ def test_gate_far_below_zero(rows, k):
     want = silu(g) * u
     off = (4 * 2.0 ** -23 + 3 * 2.0 ** -24) * np.abs(want) + (np.abs(g) + 1) * 2.0 ** -150 * u
     assert (np.abs(f64(y) - want) <= off).all()
+
+
+@pytest.mark.parametrize("fmt", ["block32", "block16"])
+@pytest.mark.parametrize("k,pitch,offset", [(96, 48, 4), (96, 48, 0), (96, 52, 4), (1100, 560, 4), (1100, 564, 0)])
+def test_codes_at_any_four_byte_address(fmt, k, pitch, offset):
+    """Codes that start on 4 bytes but not on 8, and pitches that are a multiple of 4 but not of 8: what quantize_fp4 stores at 256, between bytes that stay."""
+    rows = 9
+    x = gaussian(rows, k, torch.bfloat16, k, 2.0)
+    s = scale_for(f64(x), fmt)
+    want = D.quantize_fp4(x, fmt, scale=s)
+    width, blocks = want.codes.shape[1], want.scales.shape[1]
+    buf = torch.full((rows * pitch + 8,), 0xCD, dtype=torch.uint8, device="cuda")
+    scales = torch.empty(rows, blocks, dtype=torch.uint8, device="cuda")
+    d = ABI.QuantizeDesc(D.FORMATS[fmt], 16, rows, rows, k, k, pitch, blocks)
+    ABI.call(ABI.library().b2vx_fp4_quantize_noalloc, C.byref(d), x.data_ptr(), None, None if s is None else s.data_ptr(), buf.data_ptr() + offset, scales.data_ptr(), None)
+    torch.cuda.synchronize()
+    at = buf.as_strided((rows, width), (pitch, 1), offset)
+    assert torch.equal(at, want.codes) and torch.equal(scales, want.scales)
+    at.fill_(0xCD)
+    assert (buf == 0xCD).all()
+    d = ABI.DequantizeDesc(D.FORMATS[fmt], 9, rows, k, pitch, blocks, k)
+    buf.as_strided((rows, width), (pitch, 1), offset).copy_(want.codes)
+    y = torch.empty(rows, k, device="cuda")
+    ABI.call(ABI.library().b2vx_fp4_dequantize_noalloc, C.byref(d), buf.data_ptr() + offset, scales.data_ptr(), None if s is None else s.data_ptr(), y.data_ptr(), None)
+    torch.cuda.synchronize()
+    assert torch.equal(y, D.dequantize_fp4(want))

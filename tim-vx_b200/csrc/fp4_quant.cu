@@ -59,6 +59,8 @@ __global__ void __launch_bounds__(kWarps * 32, quantize_blocks(FORMAT, sizeof(T)
   const TensorScale scale = tensor_scale<FORMAT, T>(a.tensor_scale);
   const int k = static_cast<int>(a.k), k32 = (k + 31) / 32 * 32, blocks = (k + B - 1) / B;
   const T* x = static_cast<const T*>(a.x);
+  // rows of codes start on 8 bytes; an operand's always do
+  const bool wide = PACKED || ((reinterpret_cast<uintptr_t>(a.codes) | static_cast<uintptr_t>(a.codes_pitch)) & 7) == 0;
   for (uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5); unit < units; unit += warps) {
     const uint32_t row = split == 1 ? unit : unit / split;
     const int part = static_cast<int>(unit - row * split);
@@ -90,7 +92,7 @@ __global__ void __launch_bounds__(kWarps * 32, quantize_blocks(FORMAT, sizeof(T)
       // k32 is a multiple of 32, c of 16: all sixteen codes lie inside the row or none; an operand's k is a multiple of 32
       if (chunk < whole || c < k32) {
         uint32_t* to = reinterpret_cast<uint32_t*>(codes_row + c / 2);
-        if (PACKED || a.codes_pitch % 8 == 0) *reinterpret_cast<uint2*>(to) = codes;
+        if (wide) *reinterpret_cast<uint2*>(to) = codes;
         else { to[0] = codes.x; to[1] = codes.y; }
       }
       if (PACKED) {
