@@ -892,3 +892,26 @@ def test_codes_at_any_four_byte_address(fmt, k, pitch, offset):
     ABI.call(ABI.library().b2vx_fp4_dequantize_noalloc, C.byref(d), buf.data_ptr() + offset, scales.data_ptr(), None if s is None else s.data_ptr(), y.data_ptr(), None)
     torch.cuda.synchronize()
     assert torch.equal(y, D.dequantize_fp4(want))
+
+
+@pytest.mark.parametrize("fmt", ["block32", "block16"])
+@pytest.mark.parametrize("offsets", [[0, 50, 20, 70], [-5, 10, 1 << 30, 70], [70, 60, 50, 0], [90, 90, 90, 90], [-1, -7, 33, -2, 12, 40], [5, 5, 0, 64, 63, 65, 70], [0, 69, 40, 70]])
+def test_bad_offsets_of_4_bit_products(fmt, offsets):
+    """Rows and their scales belong to the groups of the offsets after these are cut; memory that was used before holds NaN."""
+    experts, rows, n, k = len(offsets) - 1, 70, 40, 96
+    w, wv = weight_of(experts, n, k, fmt, 4)
+    x = gaussian(rows, k, torch.bfloat16, 3, 1.0)
+    xv, s = operand(x, fmt)
+    cut = np.maximum.accumulate(np.clip(offsets, 0, rows))
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    buf = torch.full((rows + 2, n), -77.0, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.empty_cache()
+    torch.empty(1 << 21, dtype=torch.uint8, device="cuda").fill_(0x7F)
+    D.expert_linear(x, w, off, x_scale=s, out=buf[1:-1])
+    seen = np.zeros(rows + 2, bool)
+    for e in range(experts):
+        lo, hi = int(cut[e]), int(cut[e + 1])
+        seen[lo + 1:hi + 1] = True
+        if hi > lo:
+            close(buf[lo + 1:hi + 1], *expected(xv[lo:hi], wv[e], None, False))
+    assert (buf[torch.from_numpy(~seen).cuda()] == -77.0).all()

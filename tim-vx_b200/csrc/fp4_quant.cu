@@ -23,24 +23,40 @@ constexpr int quantize_blocks(int format, size_t elem, bool packed) { return for
 constexpr long long kTwiceElements = 1 << 22;
 constexpr int kChunk = 512;   // columns of a warp per step, two k-blocks of the products
 
-// The group of a row: how many groups end at or before it.
-__device__ __forceinline__ int group_of(const int32_t* offsets, int experts, long long row, int lane) {
-  int n = 0;
-  for (int e = lane; e < experts; e += 32) n += offsets[e + 1] <= row;
-  return __reduce_add_sync(0xffffffffu, n);
-}
-
 // Where the words of a row's scales lie in the first k-block's scale tiles of a product's operand; null: the row belongs to no group.
+// Groups follow the product's rule, offsets cut to rising values among the rows: the first offset behind the row ends its group, and the largest of
+// those before that one (the last, where they rise) begins it.
 template <int FORMAT>
 __device__ __forceinline__ uint8_t* packed_place(const QuantizeArgs& a, uint32_t row, int lane) {
   int e = 0, lo = 0, count = static_cast<int>(a.rows);
   if (a.offsets) {
-    e = group_of(a.offsets, a.experts, row, lane);
-    lo = e < a.experts ? a.offsets[e] : -1;
-    count = e < a.experts ? min(a.offsets[e + 1], static_cast<int>(a.rows)) - lo : 0;
+    int end = a.experts + 1, begun = 0;                      // the first offset behind the row; how many are not
+    for (int top = a.experts - lane; top >= 0; top -= 4 * 32) {
+      int v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = top - u * 32 >= 0 ? a.offsets[top - u * 32] : INT_MIN;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (v[u] > static_cast<int>(row)) {
+          end = top - u * 32;
+        } else {
+          lo = max(lo, v[u]);
+          begun += top - u * 32 >= 0;
+        }
+      }
+    }
+    end = __reduce_min_sync(0xffffffffu, end);
+    begun = __reduce_add_sync(0xffffffffu, begun);
+    if (end == 0 || end > a.experts) return nullptr;
+    if (begun != end) {                                      // some behind the end are lower again
+      lo = 0;
+      for (int j = lane; j < end; j += 32) lo = max(lo, a.offsets[j]);
+    }
+    lo = __reduce_max_sync(0xffffffffu, lo);
+    e = end - 1;
+    count = min(a.offsets[end], count) - lo;
   }
   const int in = static_cast<int>(row) - lo;            // row inside its group
-  if (lo < 0 || in < 0 || in >= count) return nullptr;
   const int per = rows_of_tile(count, a.bn), i = in / per, r = in - i * per;
   const int at = expert_scale_tile(lo, e, a.bn) + i * ((a.bn + 127) / 128) + r / 128;
   return a.scales + static_cast<long long>(at) * (scale_words_per_stage(FORMAT) * kScaleTile) + (r % 32) * 16 + (r % 128 / 32) * 4;
