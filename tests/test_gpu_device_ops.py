@@ -915,3 +915,41 @@ def test_bad_offsets_of_4_bit_products(fmt, offsets):
         if hi > lo:
             close(buf[lo + 1:hi + 1], *expected(xv[lo:hi], wv[e], None, False))
     assert (buf[torch.from_numpy(~seen).cuda()] == -77.0).all()
+
+
+@pytest.mark.parametrize("fmt", ["block32", "none"])
+@pytest.mark.parametrize("rows", [40, 70])
+@pytest.mark.parametrize("tiles", [0.5, 1, 1.5, 2, 2.5, 3, 5])
+def test_tiles_of_a_cta(fmt, rows, tiles):
+    """One to five tiles for each CTA or pair of CTAs, some with one more than others: accumulators are handed back for the tiles that come, and only for those."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    n, k = int(128 * sms * tiles) - 9, 96                # 128 features of a tile and SM
+    x = gaussian(rows, k, torch.bfloat16, 2, 1.0)
+    if fmt == "none":
+        w = (gaussian(n, k, torch.float32, 4, 1.0) / k ** 0.5).bfloat16()
+        wv = f64(w)
+    else:
+        w, wv = weight_of(0, n, k, fmt, 4)
+        wv = wv[0]
+    y = D.linear(x, w)
+    close(y, *expected(operand(x, fmt)[0], wv, None, False))
+    for _ in range(5):
+        assert torch.equal(D.linear(x, w), y)
+
+
+@pytest.mark.parametrize("fmt", ["block32", "block16"])
+def test_bad_offsets_of_rows_taken_several_times(fmt):
+    """Rows that are quantized once and copied to where falling offsets put them, in tiles of two CTAs."""
+    tokens, rows, n, k = 300, 5000, 72, 1056
+    offsets = [-3, 2000, 900, 3500, 3400, 1 << 30, 4000]
+    experts = len(offsets) - 1
+    x = gaussian(tokens, k, torch.bfloat16, 12, 1.0)
+    index = np.random.default_rng(3).integers(0, tokens, rows).astype(np.int32)
+    w, wv = weight_of(experts, n, k, fmt, 6)
+    xv, s = operand(x, fmt)
+    y = D.expert_linear(x, w, torch.tensor(offsets, dtype=torch.int32, device="cuda"), row_index=torch.from_numpy(index).cuda(), x_scale=s)
+    cut = np.maximum.accumulate(np.clip(offsets, 0, rows))
+    for e in range(experts):
+        lo, hi = int(cut[e]), int(cut[e + 1])
+        if hi > lo:
+            close(y[lo:hi], *expected(xv[index[lo:hi]], wv[e], None, False))

@@ -516,6 +516,12 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
         if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
       }
     }
+    // The last use of each stage: what the issuer's instructions still tell this CTA's barriers has to arrive while it exists.
+    for (int i = 0; i < p.stages; ++i) {
+      if (elect_one()) ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 101);
+      __syncwarp();
+      if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
+    }
   } else if (!RAW && warp == 2) {
     // ------------------------------------------------------------ producer of x
     pdl_wait();
@@ -720,8 +726,11 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const bool ok = set_all(set, mbar_wait(smem_u32(&h->acc_full[buf]), buf_ph, abort_flag, p.status, 104));
       if (!ok) break;
       fence_after();
-      // The accumulator is free for the tile after the next one once everything of it is in registers, before any row is stored.
+      // The accumulator is free for the tile after the next one once everything of it is in registers, before any row is stored.  Where there is no
+      // such tile nobody waits for that, and an arrival at the first CTA could come when it has left.
+      const bool again = t + 2 * tile_step < num_tiles;
       auto release = [&] {
+        if (!again) return;
         fence_before();
         __syncwarp();
         if (lane == 0) {
@@ -877,7 +886,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   __syncwarp();
   fence_before();
   if constexpr (CG == 1) __syncthreads();
-  else asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");   // the other CTA's instructions and arrivals reach into this one's memory; stores need not be waited for
+  else asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");   // the other CTA's instructions reach into this one's memory (its arrivals and loads have all been waited for); stores need not be waited for
   if (*abort_flag) {          // copies in flight land within microseconds
     const long long began = clock64();
     while (clock64() - began < 200000) {}
