@@ -433,7 +433,7 @@ typedef struct b2vx_combine_desc {
 b2vx_status b2vx_combine_noalloc(const b2vx_combine_desc* d, const void* z, const int32_t* slots, const float* weights,
                                  const void* residual, void* y, void* cuda_stream, char* err, size_t err_len);
 /* Waits for the stream and tells whether a product on the current GPU gave up on a barrier since the last such call
- * (B2VX_DEVICE_TIMEOUT; its y is incomplete).  Later calls on that GPU are refused until this one is made. */
+ * (B2VX_DEVICE_TIMEOUT; its y is incomplete).  Later products on that GPU are refused until this one is made. */
 b2vx_status b2vx_device_check_noalloc(void* cuda_stream, char* err, size_t err_len);
 
 /* Measurement aid with no counterpart in the reference: the dense int8 rate of

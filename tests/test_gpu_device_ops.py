@@ -3,6 +3,7 @@
 Quantization is compared code by code and byte by byte.  Products: a kernel adds float32 partial sums, one for every 16 to 64 columns of K, each
 rounded (or cut) to 2^-23 of at most S = sum |x w| |alpha| + |bias|, so a result may be off by (k / 16 + 4) 2^-23 S and half a step of its type."""
 import ctypes as C
+import os
 import subprocess
 import sys
 
@@ -953,3 +954,65 @@ def test_bad_offsets_of_rows_taken_several_times(fmt):
         lo, hi = int(cut[e]), int(cut[e + 1])
         if hi > lo:
             close(y[lo:hi], *expected(xv[index[lo:hi]], wv[e], None, False))
+
+
+STALL = """
+import sys
+sys.path[:0] = %r
+import torch, deviceops as D, pyb2vx as B
+g = torch.Generator(device="cuda").manual_seed(1)
+E2M1 = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64, device="cuda")
+
+def case(fmt, rows, n, k, gated=False):
+    # numbers that 4 bits hold with a scale of 1, so that sums are exact
+    x = torch.tensor([-6.0, -3.0, 0.0, 1.0, 6.0], device="cuda")[torch.randint(0, 5, (rows, k), generator=g, device="cuda")]
+    x[:, ::16] = 6.0
+    x = x.bfloat16()
+    lead, s, off = (2 * n if gated else n,), None, None
+    if gated:
+        lead, off = (2,) + lead, torch.tensor([0, rows // 3, rows], dtype=torch.int32, device="cuda")
+    if fmt == "none":
+        w = torch.randint(-3, 4, lead + (k,), generator=g, device="cuda").bfloat16()
+        v = w.double()
+    else:
+        codes = torch.randint(0, 256, lead + (k // 2,), dtype=torch.uint8, generator=g, device="cuda")
+        one = 127 if fmt == "block32" else 0x38
+        scale = None if fmt == "block32" else torch.ones(2 if gated else 1, device="cuda")
+        s = None if fmt == "block32" else torch.ones(1, device="cuda")
+        w = D.Fp4Weight(codes, torch.full(lead + (k // D.BLOCK[fmt],), one, dtype=torch.uint8, device="cuda"), fmt, scale, gated)
+        v = torch.stack([E2M1[(codes & 15).long()], E2M1[(codes >> 4).long()]], dim=-1).flatten(-2)
+    if not gated:
+        return lambda: D.linear(x, w, x_scale=s, out_dtype=torch.float32), x.double() @ v.T
+    h = torch.cat([x[:rows // 3].double() @ v[0].T, x[rows // 3:].double() @ v[1].T])
+    return lambda: D.expert_linear(x, w, off, gated=True, x_scale=s, out_dtype=torch.float32), torch.nn.functional.silu(h[:, :n]) * h[:, n:]
+
+cases = [case("none", 40, 40000, 96), case("none", 3, 300, 1024), case("block32", 2, 512, 2048), case("block16", 24, 2048, 4096),
+         case("block16", 300, 5000, 1056), case("none", 300, 21000, 160), case("block32", 400, 1024, 512, True), case("block32", 40, 512, 544, True)]
+assert len(cases) == %d
+torch.cuda.synchronize()
+for run, _ in cases:
+    run()
+    torch.cuda.synchronize()
+    for again in (run, D.check):
+        try:
+            again()
+            print("no error")
+        except B.B2vxError as e:
+            assert e.status == 7 and "gave up waiting on a barrier" in str(e), str(e)
+    D.check()
+for _ in range(3):
+    for i, (run, want) in enumerate(cases):
+        got = run().double()
+        # of a gated product 16 steps of float32 at most, as in expected() above; sums are exact
+        assert ((got - want).abs() <= (16 * 2.0 ** -24 * want.abs() + 2.0 ** -126 if i >= 6 else 0 * want)).all(), i
+D.check()
+print("same")
+"""
+
+
+def test_a_wait_that_runs_out_is_reported_and_the_context_stays_usable():
+    """B2VX_TEST_STALL: the first products of the process announce 16 bytes more than they load and give up after a millisecond, in every form of the kernel:
+    one CTA to a tile, a cluster that shares K, with x quantized by the product and before it, and two CTAs to a tile, also by expert."""
+    env = dict(os.environ, B2VX_TEST_STALL="8")
+    out = subprocess.run([sys.executable, "-c", STALL % (sys.path, 8)], capture_output=True, text=True, env=env, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip() == "same", out.stdout + out.stderr

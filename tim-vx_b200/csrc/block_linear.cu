@@ -30,13 +30,15 @@
 // into shared memory, where it stays; the ring then holds W alone.  Every tile's CTAs repeat that work, but it saves a launch
 // and what the products wait for it.
 //
-// Every wait is bounded as in gemm_tc.cu: on a time-out the CTA records a code and leaves through its common exit.
+// Every wait is bounded as in gemm_tc.cu: on a time-out the CTA records a code, tells the other CTA of its tiles, and both leave through their common
+// exit: producers load nothing more, the issuer issues and announces nothing more.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <algorithm>
 #include <atomic>
+#include <cstdlib>
 
 #include "block_linear.cuh"
 #include "fp4.cuh"
@@ -89,6 +91,8 @@ struct LinearParams {
   int y_dtype;
   int y_vec;                  // rows of y start on 16 bytes
   int* status;
+  long long wait_limit;       // cycles
+  uint32_t tx_extra;          // bytes announced and never loaded (B2VX_TEST_STALL)
 };
 
 struct Maps {
@@ -139,7 +143,7 @@ __device__ __forceinline__ void arrive_remote(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 // A wait for arrivals that may come from the other CTA.
-__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code) {
+__device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status, int code, long long limit) {
   const long long began = clock64();
   while (true) {
     uint32_t ok;
@@ -150,12 +154,16 @@ __device__ __forceinline__ bool wait_cluster(uint32_t bar, uint32_t parity, vola
         : "=r"(ok) : "r"(bar), "r"(parity), "r"(100u) : "memory");
     if (ok) return true;
     if (*abort_flag) return false;
-    if (clock64() - began > kWaitLimitCycles) {
+    if (clock64() - began > limit) {
       *abort_flag = 1;
       atomicCAS(status, 0, code);
       return false;
     }
   }
+}
+// Sets the abort flag of the other CTA of a pair; ordered before this thread's arrival at the exit's barrier, until which that CTA stays.
+__device__ __forceinline__ void abort_other(uint32_t flag) {
+  asm volatile("st.relaxed.cluster.shared::cluster.u32 [%0], %1;\n\tfence.acq_rel.cluster;" ::"r"(in_cta(flag, static_cast<int>(cluster_rank() ^ 1u))), "r"(1u) : "memory");
 }
 // Arrives on the barrier (CG = 2: of both CTAs) when the instructions issued so far are done.
 template <int CG>
@@ -483,11 +491,16 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   fence_after();
   const int num_tiles = h->num_tiles;
 
+  // A bounded wait; false: given up, here or elsewhere in the CTA or its pair.
+  auto wait = [&](uint32_t bar, uint32_t parity, int code) {
+    if (mbar_wait(bar, parity, abort_flag, p.status, code, p.wait_limit)) return true;
+    if constexpr (CG == 2) abort_other(smem_u32(&h->abort_flag));
+    return false;
+  };
   // The control warps run their loops with all lanes, so that what feeds a copy or an instruction is the same in all of them and can live
   // in uniform registers, and elect one (always the same) for the issue.  What a stage costs the issuing thread besides
   // its instructions, some 300 cycles of waiting and bookkeeping, is why a stage holds two k-blocks, and why nothing votes on a wait
-  // that gave up: a producer's lane then loads nothing more, the issuer runs out on whatever lies there, and the exit waits for
-  // copies in flight.
+  // that gave up: the elected lane then does nothing more in its rounds, and the exit waits for copies in flight.
   const uint32_t full0 = smem_u32(h->full), empty0 = smem_u32(h->empty);
   if (warp == 0) {
     // ------------------------------------------------------------ producer of W
@@ -500,12 +513,12 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const int ft = tile.f * CG + static_cast<int>(rank);
       for (int kb = kb_first; kb < kb_end; kb += kGroup) {
         if (elect_one()) {
-          ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 101);
+          ok = ok && wait(empty0 + 8 * s, ph ^ 1, 101);
           if (ok) {
             uint32_t dst = ring + s * p.stage_bytes;
             const uint32_t full = announce + 8 * s;
             const int end = min(kb + kGroup, kb_end);
-            if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (end - kb) * CG * kWTile);
+            if (rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (end - kb) * CG * kWTile + p.tx_extra);
             for (int k = kb; k < end; ++k, dst += p.block_bytes) {
               if (GATED) load_5d<CG>(dst, &maps.w, k * kStageBytes, ft * 8, tile.e, full);
               else load_3d<CG>(dst, &maps.w, k * kStageBytes, ft * 128, tile.e, full);
@@ -518,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     }
     // The last use of each stage: what the issuer's instructions still tell this CTA's barriers has to arrive while it exists.
     for (int i = 0; i < p.stages; ++i) {
-      if (elect_one()) ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 101);
+      if (elect_one()) ok = ok && wait(empty0 + 8 * s, ph ^ 1, 101);
       __syncwarp();
       if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
     }
@@ -538,7 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const uint32_t tx = CG * (large ? p.x_box : boxes * kBoxRows) * kStageBytes;
       for (int kb = kb_first; kb < kb_end; kb += kGroup) {
         if (elect_one()) {
-          ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 105);
+          ok = ok && wait(empty0 + 8 * s, ph ^ 1, 105);
           if (ok) {
             uint32_t dst = ring + s * p.stage_bytes;
             const uint32_t full = announce + 8 * s;
@@ -573,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       for (int kb = kb_first; kb < kb_end; kb += kGroup) {
         const int blocks = min(kGroup, kb_end - kb);
         if (elect_one()) {
-          ok = ok && mbar_wait(empty0 + 8 * s, ph ^ 1, abort_flag, p.status, 106);
+          ok = ok && wait(empty0 + 8 * s, ph ^ 1, 106);
           if (ok) {
             uint32_t dst = ring + s * p.stage_bytes;
             const uint32_t full = announce + 8 * s;
@@ -596,6 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
     int j = 0;
     const uint32_t ring_low = (ring >> 4) | kDescLow, stage_low = p.stage_bytes >> 4, block_low = p.block_bytes >> 4;
     uint32_t low = ring_low;                               // of the stage's first operand
+    bool ok = true;
     Tile tile = {};
     if (first_tile < num_tiles) tile = tile_of<CG>(groups, p, first_tile, 0);
     for (int t = first_tile; t < num_tiles; t += tile_step, ++j) {
@@ -603,8 +617,12 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const int atoms = NW ? (tile.n_mma + 127) >> 7 : 0;
       const int buf = j & 1;
       const uint32_t buf_ph = (j >> 1) & 1;
-      if (CG == 1) mbar_wait(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102);
-      else wait_cluster(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102);
+      if constexpr (CG == 1) {
+        ok = ok && wait(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, 102);
+      } else if (ok && !wait_cluster(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102, p.wait_limit)) {
+        ok = false;
+        abort_other(smem_u32(&h->abort_flag));
+      }
       __syncwarp();
       fence_after();
       const uint32_t d = buf * kBufferColumns;
@@ -636,9 +654,10 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       for (int kb = kb_first; kb < kb_end; kb += kGroup) {
         // the next tile is worked out while the instructions of this one's last stages run
         if (kb + kGroup >= kb_end && t + tile_step < num_tiles) tile = tile_of<CG>(groups, p, t + tile_step, tile.e);
-        if (RAW && kb == kb_first) mbar_wait(smem_u32(&h->x_ready), 0, abort_flag, p.status, 107);
-        mbar_wait(full0 + 8 * s, ph, abort_flag, p.status, 103);
-        if (elect_one()) {
+        if (RAW && kb == kb_first) ok = ok && wait(smem_u32(&h->x_ready), 0, 107);
+        ok = ok && wait(full0 + 8 * s, ph, 103);
+        __syncwarp();
+        if (elect_one() && ok) {
           fence_after();
           k_block(low, 0, kb, kb == kb_first);
           if (kb + 1 < kb_end) k_block(low + block_low, 1, kb + 1, false);
@@ -648,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
         low += stage_low;
         if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; low = ring_low; }
       }
-      if (elect_one()) commit<CG>(smem_u32(&h->acc_full[buf]));
+      if (elect_one() && ok) commit<CG>(smem_u32(&h->acc_full[buf]));
       __syncwarp();
     }
   } else if (SPLIT && warp >= kFirstEpilogueWarp) {
@@ -666,7 +685,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const Tile tile = tile_of<CG>(groups, p, first_tile, 0);
       const int width = 128 / p.split, l = quarter * 32 + lane, owner = l / width;
       const uint32_t to = in_cta(staging + (part * tile.rows * width + l - owner * width) * 4, owner), step = width * 4;
-      mbar_wait(smem_u32(&h->acc_full[0]), 0, abort_flag, p.status, 104);
+      wait(smem_u32(&h->acc_full[0]), 0, 104);             // given up: the sums are of no use, y is incomplete
       __syncwarp();
       fence_after();
       for (int c0 = set * 16; c0 < tile.rows; c0 += 32) {
@@ -723,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const uint32_t taddr = buf * kBufferColumns + lanes;
       const int row0 = tile.lo + tile.r0;
       const int f0 = (tile.f * CG + static_cast<int>(rank)) * width;       // first feature of the CTA's tile
-      const bool ok = set_all(set, mbar_wait(smem_u32(&h->acc_full[buf]), buf_ph, abort_flag, p.status, 104));
+      const bool ok = set_all(set, wait(smem_u32(&h->acc_full[buf]), buf_ph, 104));
       if (!ok) break;
       fence_after();
       // The accumulator is free for the tile after the next one once everything of it is in registers, before any row is stored.  Where there is no
@@ -887,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   fence_before();
   if constexpr (CG == 1) __syncthreads();
   else asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");   // the other CTA's instructions reach into this one's memory (its arrivals and loads have all been waited for); stores need not be waited for
-  if (*abort_flag) {          // copies in flight land within microseconds
+  if (*abort_flag) {          // copies and instructions in flight end within microseconds; both CTAs of a pair wait for them
     const long long began = clock64();
     while (clock64() - began < 200000) {}
     __syncwarp();
@@ -1056,6 +1075,14 @@ cudaError_t launch_linear(const LinearArgs& a, cudaStream_t s, const char** why)
   p.y_stride = a.y_stride;
   p.y_dtype = a.y_dtype;
   p.status = a.status;
+  p.wait_limit = kWaitLimitCycles;
+  // Test aid, as in gemm_tc.cu: B2VX_TEST_STALL=<n> makes the first n products of the process announce 16 bytes more than their loads deliver and give
+  // up after about a millisecond.
+  static std::atomic<int> stall_left([] { const char* v = std::getenv("B2VX_TEST_STALL"); return v ? std::atoi(v) : 0; }());
+  if (stall_left.load(std::memory_order_relaxed) > 0 && stall_left.fetch_sub(1) > 0) {
+    p.wait_limit = 2000000LL;
+    p.tx_extra = 16;
+  }
   p.x_scale_tiles = fp4 ? static_cast<int>(expert_scale_tiles(a.rows, a.experts, p.bn)) : 0;
   p.after_operand = a.after_operand;
 
