@@ -1016,3 +1016,34 @@ def test_a_wait_that_runs_out_is_reported_and_the_context_stays_usable():
     env = dict(os.environ, B2VX_TEST_STALL="8")
     out = subprocess.run([sys.executable, "-c", STALL % (sys.path, 8)], capture_output=True, text=True, env=env, timeout=300)
     assert out.returncode == 0 and out.stdout.strip() == "same", out.stdout + out.stderr
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("g", [2.0 ** -149, 3e-39, 1e-37, 2.0 ** -126, 1e-30, 2.0 ** -61, 2.0 ** -60, 2.0 ** 60, 2.0 ** 61, 3e38])
+def test_quantize_at_the_ends_of_float_range(dtype, g):
+    """Tensor scales whose blocks' units are subnormal or below, or near float's largest; zeros, tiny and large numbers side by side."""
+    g = float(np.float32(g))
+    rng = np.random.default_rng(5)
+    rows = [np.zeros(16), np.full(16, 2.0 ** -149), np.where(np.arange(16) % 3 == 0, 3.4e38, 1e-40)]
+    for unit in (2.0 ** -9, 2.0 ** -8, 2.0 ** -6, 0.40625, 1.0, 13.0, 448.0):
+        for spread in (0.0, 1.0, 6.0):
+            r = 6 * unit * g * np.exp2(-spread * rng.random(16)) * rng.choice([-1.0, 1.0], 16)
+            r[rng.integers(0, 16, 4)] = 0.0
+            rows.append(r)
+        rows.append(np.append((E2M1[1:] + E2M1[:-1]) / 2, np.append(E2M1, 6.0)) * unit * g)
+    with np.errstate(over="ignore"):
+        x = torch.from_numpy(np.nan_to_num(np.stack(rows).astype(np.float32), posinf=3.3e38, neginf=-3.3e38)).to(dtype).cuda()
+    same_quantized(D.quantize_fp4(x, "block16", scale=torch.tensor([g], device="cuda")), x, g)
+
+
+def test_linear_with_a_tiny_scale_of_x():
+    """A product that quantizes x itself, x and its scale near float's smallest."""
+    n, k = 128, 2048
+    x = gaussian(1, k, torch.float32, 8, 0.5) * 1e-37
+    x[:, ::5] = 0.0
+    g = float(np.float32(1e-38))
+    w, wv = weight_of(0, n, k, "block16", 9)
+    w.scale.mul_(1e30)
+    y = D.linear(x, w, x_scale=torch.tensor([g], device="cuda"), out_dtype=torch.float32)
+    xv = values(*quantized(f64(x), "block16", g), "block16", g)
+    close(y, *expected(xv, wv[0] * (float(w.scale) / float(np.float32(0.0007))), None, False))

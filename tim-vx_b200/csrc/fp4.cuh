@@ -230,6 +230,10 @@ __device__ __forceinline__ uint2 quantize_16(const Sixteen<T>& x, const TensorSc
   } else {
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = to_float(x.v[i]);
+    if (t.lift != 1.0f) {             // else the factor below could overflow: s g may be less than 2^-128
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] *= t.lift;
+    }
     // amax / (6 g) as a product of three roundings is off by less than 2^-22 of itself: where a little less and a little more round to
     // the same byte, that is the answer, else the border between them, as in settle_codes.
     constexpr float kLess = 1.0f - 0x1p-20f, kMore = 1.0f + 0x1p-20f;
@@ -246,7 +250,7 @@ __device__ __forceinline__ uint2 quantize_16(const Sixteen<T>& x, const TensorSc
     float over_s;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(over_s) : "f"(s));   // off by 2^-23; s = 0 is dealt with below
     // The numbers over s g: the approximate reciprocal, two products and 1 / g are off by less than 2^-21 together.
-    const float inv = over_s * t.over_g * t.lift, less = inv * kLess, more = inv * kMore;
+    const float inv = over_s * t.over_g, less = inv * kLess, more = inv * kMore;
     const uint32_t near = __shfl_sync(0xffffffffu, t.near, (__float_as_uint(s) >> 20) & 7);
     const float f = near == 2u ? more : less;
     uint2 codes = make_uint2(e2m1_codes_times(v, f), e2m1_codes_times(v + 8, f));
