@@ -231,3 +231,35 @@ def test_addresses_of_words_must_be_aligned():
     d = C.byref(desc(ABI.CombineDesc, COMBINE))
     for args in ((PTR, odd, PTR, PTR, PTR), (PTR, PTR, odd, PTR, PTR)):
         assert "aligned" in refused(lib.b2vx_combine_noalloc, d, *args, None)
+
+
+def test_derivatives_are_refused_and_not_dropped():
+    torch = pytest.importorskip("torch")
+    import torch.autograd.forward_ad as forward
+    with forward.dual_level():
+        dual = forward.make_dual(torch.ones(2, 32), torch.ones(2, 32))
+        with pytest.raises(ValueError, match="forward-mode"):
+            D.quantize_fp4(dual)
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            D.linear(dual.bfloat16(), torch.zeros(8, 32, dtype=torch.bfloat16))
+        with pytest.raises(ValueError, match="forward-mode"):
+            D.combine_experts(torch.zeros(4, 8), torch.zeros(4, 1, dtype=torch.int32), forward.make_dual(torch.ones(4, 1), torch.ones(4, 1)))
+        assert forward.unpack_dual(dual).tangent is not None
+    with torch.no_grad(), pytest.raises(ValueError, match="GPU"):       # a gradient that nobody asks for is no obstacle
+        D.quantize_fp4(torch.zeros(2, 32, requires_grad=True))
+
+
+def test_transformed_tensors_are_refused():
+    """torch.func's wrappers have no memory of their own."""
+    torch = pytest.importorskip("torch")
+    for transformed in (lambda f: torch.func.grad(lambda x: f(x).sum()), lambda f: torch.func.vmap(f), lambda f: (lambda x: torch.func.jvp(f, (x,), (x,)))):
+        with pytest.raises(ValueError, match="memory of its own"):
+            transformed(lambda x: D.quantize_fp4(x).scales.float())(torch.ones(3, 32))
+    with pytest.raises(ValueError, match="memory of its own"):
+        D.quantize_fp4(torch.ones(2, 32).to_sparse())
+
+
+def test_traces_are_refused():
+    torch = pytest.importorskip("torch")
+    with pytest.raises(ValueError, match="traced"):
+        torch.jit.trace(lambda x: D.quantize_fp4(x).codes, torch.ones(2, 32))

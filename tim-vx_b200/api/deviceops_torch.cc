@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cstdint>
 #include <stdexcept>
@@ -43,7 +44,11 @@ int dtype_code(at::ScalarType t) {
 const at::Tensor& tensor(PyObject* o, const char* what) {
   if (!THPVariable_Check(o)) wrong(std::string(what) + " must be a tensor");
   const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.has_storage()) wrong(std::string(what) + " has no memory of its own (a wrapper of torch.func, or not strided)");
   if (c10::GradMode::is_enabled() && t.requires_grad()) wrong(std::string(what) + " requires a gradient, which these operators do not have");
+  if (t._fw_grad(0).defined()) wrong(std::string(what) + " carries a forward-mode gradient, which these operators do not have");
+  // calls do not pass torch's dispatcher: a trace would keep their outputs as constants
+  need(!torch::jit::tracer::isTracing(), "these operators cannot be traced");
   return t;
 }
 std::string shape_of(at::IntArrayRef s) {
