@@ -1047,3 +1047,60 @@ def test_linear_with_a_tiny_scale_of_x():
     y = D.linear(x, w, x_scale=torch.tensor([g], device="cuda"), out_dtype=torch.float32)
     xv = values(*quantized(f64(x), "block16", g), "block16", g)
     close(y, *expected(xv, wv[0] * (float(w.scale) / float(np.float32(0.0007))), None, False))
+
+
+def test_outputs_must_not_overlap_any_input():
+    pool = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+
+    def at(offset, shape, dtype):
+        return pool[offset:].view(dtype)[:int(np.prod(shape))].view(shape)
+
+    x = torch.zeros(8, 64, dtype=torch.bfloat16, device="cuda")
+    codes, scales = at(0, (3, 64, 32), torch.uint8), at(8192, (3, 64, 4), torch.uint8)
+    scales.fill_(0x38)
+    w_scale, x_scale, bias = at(16384, (3,), torch.float32), at(16400, (1,), torch.float32), at(16416, (3, 64), torch.float32)
+    offsets, index = at(20480, (4,), torch.int32), at(20512, (8,), torch.int32)
+    w_scale.fill_(1.0), x_scale.fill_(1.0)
+    w = D.Fp4Weight(codes, scales, "block16", w_scale)
+    args = dict(row_index=index, bias=bias, x_scale=x_scale)
+    for offset in (0, 6143 // 16 * 16, 16384, 16400, 16416 + 512, 20480, 20512):        # over each of them
+        with pytest.raises(ValueError, match="overlaps"):
+            D.expert_linear(x, w, offsets, out=at(offset, (8, 64), torch.bfloat16), **args)
+    with pytest.raises(ValueError, match="overlaps"):
+        D.expert_linear(x, w, offsets, out=w.packed[:1024].view(torch.bfloat16).view(8, 64), **args)
+    D.expert_linear(x, w, offsets, out=at(65536, (8, 64), torch.bfloat16), **args)
+
+    q = D.Fp4Rows(at(0, (4, 32), torch.uint8), at(128, (4, 4), torch.uint8), 64, "block16", at(256, (1,), torch.float32))
+    for offset in (0, 64, 128, 256):
+        with pytest.raises(ValueError, match="overlaps"):
+            D.dequantize_fp4(q, torch.float16, out=at(offset, (4, 64), torch.float16))
+    assert D.dequantize_fp4(q, torch.float16, out=at(512, (4, 64), torch.float16)).shape == (4, 64)
+
+    z, slots, weights = torch.zeros(4, 64, device="cuda"), at(0, (4, 2), torch.int32), at(32, (4, 2), torch.float32)
+    for offset in (0, 32):
+        with pytest.raises(ValueError, match="overlaps"):
+            D.combine_experts(z, slots, weights, out=at(offset, (4, 64), torch.float32))
+    wide = torch.zeros(9, 64, device="cuda")
+    for residual, out in ((wide[:4], wide[1:5]), (wide[1:5], wide[:4]), (wide[:4], wide[:8:2]), (wide.view(-1)[:256].view(4, 64), wide.view(-1)[4:260].view(4, 64))):
+        with pytest.raises(ValueError, match="overlaps"):
+            D.combine_experts(z, slots, weights, residual=residual, out=out)
+    D.combine_experts(z, slots, weights, residual=wide[:4], out=wide[:4])
+    D.combine_experts(z, slots, weights, residual=wide[:4], out=wide[4:8])
+
+
+def test_columns_of_one_tensor_may_be_input_and_output():
+    wide = torch.zeros(30, 256, dtype=torch.bfloat16, device="cuda")
+    wide[:, 32:128] = gaussian(30, 96, torch.bfloat16, 1, 0.0)
+    w = gaussian(64, 96, torch.bfloat16, 2, 0.0)
+    want = D.linear(wide[:, 32:128].contiguous(), w)
+    for first in (128, 192):
+        assert torch.equal(D.linear(wide[:, 32:128], w, out=wide[:, first:first + 64]), want)
+    assert not wide[:, :32].any()
+    for first in (0, 64, 127):
+        with pytest.raises(ValueError, match="overlaps"):
+            D.linear(wide[:, 32:128], w, out=wide[:, first:first + 64])
+    narrow = wide.view(60, 128)                          # rows of another pitch over the same memory
+    with pytest.raises(ValueError, match="overlaps"):
+        D.linear(narrow[:, 32:128], w, out=wide.view(60, 128)[:, 64:])
+    with pytest.raises(ValueError, match="overlaps"):
+        D.linear(wide[:, 32:128], w, out=wide.view(-1)[:30 * 64].view(30, 64))

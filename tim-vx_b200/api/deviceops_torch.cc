@@ -15,6 +15,7 @@
 #include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 
@@ -124,15 +125,37 @@ at::Tensor output(PyObject* out, at::IntArrayRef shape, at::ScalarType type, con
   need(t.size(0) <= 1 || t.stride(0) >= t.size(1), "out has rows that overlap");
   return t;
 }
-// Whether the memory from a's first to its last element meets b's.
-bool overlap(const at::Tensor& a, const at::Tensor& b) {
-  if (!a.numel() || !b.numel()) return false;
-  auto end = [](const at::Tensor& t) {
-    int64_t last = 0;
-    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-    return static_cast<const char*>(t.data_ptr()) + (last + 1) * static_cast<int64_t>(t.element_size());
-  };
-  return static_cast<const char*>(a.data_ptr()) < end(b) && static_cast<const char*>(b.data_ptr()) < end(a);
+// A tensor's memory: rows of `width` bytes, `pitch` apart.
+struct Memory {
+  explicit Memory(const at::Tensor& t) : at(static_cast<const char*>(t.data_ptr())) {
+    const int64_t size = static_cast<int64_t>(t.element_size());
+    if (t.dim() == 2 && !t.is_contiguous()) {
+      rows = t.size(0);
+      pitch = t.stride(0) * size;
+      width = t.size(1) * size;
+    } else {
+      width = t.numel() * size;
+    }
+  }
+  const char* end() const { return at + (rows - 1) * pitch + width; }
+  const char* at;
+  int64_t rows = 1, pitch = 0, width;
+};
+// Rows of one pitch, such as columns of a larger tensor, may lie between one another; else the first to the last byte count.
+bool overlap(const at::Tensor& ta, const at::Tensor& tb) {
+  if (!ta.numel() || !tb.numel()) return false;
+  const Memory a(ta), b(tb);
+  if (a.at >= b.end() || b.at >= a.end()) return false;
+  const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+  if (pitch == 0 || (a.rows > 1 && b.rows > 1 && a.pitch != b.pitch)) return true;
+  const int64_t apart = ((b.at - a.at) % pitch + pitch) % pitch;       // columns of b behind those of a
+  return apart < a.width || apart + b.width > pitch;
+}
+// Refuses an output of the caller's that overlaps one of these arguments.
+void apart(const at::Tensor& y, PyObject* out, PyObject* const* a, std::initializer_list<int> inputs) {
+  if (out == Py_None) return;
+  for (int i : inputs)
+    if (a[i] != Py_None && overlap(y, tensor(a[i], "an input"))) wrong("out overlaps an input");
 }
 uint64_t row_stride(const at::Tensor& t) { return static_cast<uint64_t>(t.size(0) > 1 ? t.stride(0) : t.size(1)); }
 
@@ -205,6 +228,7 @@ PyObject* dequantize(PyObject* const* a) {
   void* scale = tensor_scale(a[4], format, 1, device, "scale");
   Call call(device);
   at::Tensor y = output(a[6], {rows, k}, scalar_type(a[5]), device);
+  apart(y, a[6], a, {0, 1, 4});
   const b2vx_fp4_dequantize_desc d = {static_cast<int32_t>(format), dtype_code(y.scalar_type()), static_cast<uint64_t>(rows), static_cast<uint64_t>(k),
                                       static_cast<uint64_t>(codes.size(1)), static_cast<uint64_t>((k + block - 1) / block), row_stride(y)};
   call(b2vx_fp4_dequantize_noalloc(&d, c, s, static_cast<const float*>(scale), y.data_ptr(), call.stream, call.err, sizeof(call.err)));
@@ -258,7 +282,7 @@ PyObject* product(PyObject* const* a) {
   p.bias = static_cast<const float*>(experts ? dense(a[8], "bias", at::kFloat, {experts, w_rows}, device) : dense(a[8], "bias", at::kFloat, {w_rows}, device));
   Call call(device);
   at::Tensor y = output(a[11], {rows, n}, a[10] == Py_None ? x.scalar_type() : scalar_type(a[10]), device);
-  if (a[11] != Py_None) need(!overlap(y, x), "out overlaps x");
+  apart(y, a[11], a, {0, 1, 2, 3, 6, 7, 8, 9});
   b2vx_linear_desc d = {};
   d.w_format = static_cast<int32_t>(format);
   d.x_dtype = dtype_code(x.scalar_type());
@@ -338,7 +362,9 @@ PyObject* combine(PyObject* const* a) {
   Call call(device);
   at::Tensor y = output(a[4], {tokens, n}, z.scalar_type(), device);
   need(y.scalar_type() == z.scalar_type(), "out must have z's type");
-  if (a[4] != Py_None) need(!overlap(y, z), "out overlaps z");
+  apart(y, a[4], a, {0, 1, 2});
+  if (residual && residual != y.data_ptr()) apart(y, a[4], a, {3});
+  else if (residual) need(r_stride == row_stride(y), "out overlaps the residual and has other rows");
   const b2vx_combine_desc d = {dtype_code(z.scalar_type()), static_cast<uint32_t>(top_k), static_cast<uint64_t>(tokens), static_cast<uint64_t>(n),
                                static_cast<uint64_t>(z.size(0)), stride, r_stride, row_stride(y)};
   call(b2vx_combine_noalloc(&d, z.data_ptr(), static_cast<const int32_t*>(s), static_cast<const float*>(w), residual, y.data_ptr(), call.stream, call.err, sizeof(call.err)));
