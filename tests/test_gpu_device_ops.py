@@ -1104,3 +1104,19 @@ def test_columns_of_one_tensor_may_be_input_and_output():
         D.linear(narrow[:, 32:128], w, out=wide.view(60, 128)[:, 64:])
     with pytest.raises(ValueError, match="overlaps"):
         D.linear(wide[:, 32:128], w, out=wide.view(-1)[:30 * 64].view(30, 64))
+
+
+def test_outputs_of_the_callers_count_as_changed():
+    """A graph that saved a tensor refuses its backward pass once one of these operators has written to it."""
+    x, w = torch.ones(4, 64, dtype=torch.bfloat16, device="cuda"), torch.ones(64, 64, dtype=torch.bfloat16, device="cuda")
+    q = D.quantize_fp4(x)
+    slots, weights = torch.zeros(4, 1, dtype=torch.int32, device="cuda"), torch.ones(4, 1, device="cuda")
+    for write in (lambda out: D.linear(x, w, out=out), lambda out: D.dequantize_fp4(q, torch.bfloat16, out=out),
+                  lambda out: D.combine_experts(x, slots, weights, out=out), lambda out: D.combine_experts(x, slots, weights, residual=out, out=out)):
+        leaf, out = torch.ones(4, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True), torch.ones(4, 64, dtype=torch.bfloat16, device="cuda")
+        loss = (leaf * out).sum()
+        write(out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        D.linear(x, w, out=torch.empty(4, 64, dtype=torch.bfloat16, device="cuda"))

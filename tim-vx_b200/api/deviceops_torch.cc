@@ -125,6 +125,12 @@ at::Tensor output(PyObject* out, at::IntArrayRef shape, at::ScalarType type, con
   need(t.size(0) <= 1 || t.stride(0) >= t.size(1), "out has rows that overlap");
   return t;
 }
+// An output of the caller's has been written: a graph that saved it for a backward pass notices.
+void written(PyObject* out) {
+  if (out == Py_None) return;
+  const at::Tensor& t = THPVariable_Unpack(out);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 // A tensor's memory: rows of `width` bytes, `pitch` apart.
 struct Memory {
   explicit Memory(const at::Tensor& t) : at(static_cast<const char*>(t.data_ptr())) {
@@ -232,6 +238,7 @@ PyObject* dequantize(PyObject* const* a) {
   const b2vx_fp4_dequantize_desc d = {static_cast<int32_t>(format), dtype_code(y.scalar_type()), static_cast<uint64_t>(rows), static_cast<uint64_t>(k),
                                       static_cast<uint64_t>(codes.size(1)), static_cast<uint64_t>((k + block - 1) / block), row_stride(y)};
   call(b2vx_fp4_dequantize_noalloc(&d, c, s, static_cast<const float*>(scale), y.data_ptr(), call.stream, call.err, sizeof(call.err)));
+  written(a[6]);
   return THPVariable_Wrap(std::move(y));
 }
 
@@ -304,6 +311,7 @@ PyObject* product(PyObject* const* a) {
   p.workspace = workspace.data_ptr();
   p.workspace_bytes = bytes;
   call(b2vx_linear_noalloc(&d, &p, call.stream, call.err, sizeof(call.err)));
+  written(a[11]);
   return THPVariable_Wrap(std::move(y));
 }
 
@@ -368,6 +376,7 @@ PyObject* combine(PyObject* const* a) {
   const b2vx_combine_desc d = {dtype_code(z.scalar_type()), static_cast<uint32_t>(top_k), static_cast<uint64_t>(tokens), static_cast<uint64_t>(n),
                                static_cast<uint64_t>(z.size(0)), stride, r_stride, row_stride(y)};
   call(b2vx_combine_noalloc(&d, z.data_ptr(), static_cast<const int32_t*>(s), static_cast<const float*>(w), residual, y.data_ptr(), call.stream, call.err, sizeof(call.err)));
+  written(a[4]);
   return THPVariable_Wrap(std::move(y));
 }
 
