@@ -405,6 +405,8 @@ typedef struct b2vx_linear_args {
   size_t workspace_bytes;
 } b2vx_linear_args;
 b2vx_status b2vx_linear_workspace_size_noalloc(const b2vx_linear_desc* d, size_t* bytes, char* err, size_t err_len);
+/* 1 where the product reads x where it lies and needs no workspace: 16-bit weights, no row_index, rows of x on 16 bytes. */
+int32_t b2vx_linear_in_place_noalloc(const b2vx_linear_desc* d, const b2vx_linear_args* a);
 b2vx_status b2vx_linear_noalloc(const b2vx_linear_desc* d, const b2vx_linear_args* a, void* cuda_stream, char* err, size_t err_len);
 
 /* The experts of each token: ids[t][j] (int32) = the top_k largest of logits[t][0..experts-1], largest first, ties to the

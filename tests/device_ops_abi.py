@@ -41,6 +41,7 @@ _SIGNATURES = {
     "b2vx_fp4_packed_scales_size_noalloc": [_i32, _u64, _u64, _i32, _u64, C.POINTER(_sz)],
     "b2vx_fp4_pack_scales_noalloc": [_i32, _u64, _u64, _i32, _u64, _vp, _vp, _vp] + _err,
     "b2vx_linear_workspace_size_noalloc": [C.POINTER(LinearDesc), C.POINTER(_sz)] + _err,
+    "b2vx_linear_in_place_noalloc": [C.POINTER(LinearDesc), C.POINTER(LinearArgs)],
     "b2vx_linear_noalloc": [C.POINTER(LinearDesc), C.POINTER(LinearArgs), _vp] + _err,
     "b2vx_route_workspace_size_noalloc": [C.POINTER(RouteDesc), C.POINTER(_sz)] + _err,
     "b2vx_route_noalloc": [C.POINTER(RouteDesc)] + [_vp] * 7 + [_sz, _vp] + _err,

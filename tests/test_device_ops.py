@@ -263,3 +263,13 @@ def test_traces_are_refused():
     torch = pytest.importorskip("torch")
     with pytest.raises(ValueError, match="traced"):
         torch.jit.trace(lambda x: D.quantize_fp4(x).codes, torch.ones(2, 32))
+
+
+@pytest.mark.parametrize("change,args,told", [
+    (dict(), dict(), 1), (dict(w_format=1), dict(), 0), (dict(), dict(row_index=PTR), 0), (dict(), dict(x=PTR + 2), 0), (dict(x_stride=100), dict(), 0),
+    (dict(x_stride=104), dict(x=PTR + 16), 1)])
+def test_products_that_need_no_workspace(change, args, told):
+    d = desc(ABI.LinearDesc, dict(LINEAR, w_format=0), **change)
+    a = desc(ABI.LinearArgs, dict(x=PTR, w=PTR, y=PTR), **args)
+    assert ABI.library().b2vx_linear_in_place_noalloc(C.byref(d), C.byref(a)) == told
+    assert ABI.library().b2vx_linear_in_place_noalloc(None, C.byref(a)) == 0

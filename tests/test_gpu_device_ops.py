@@ -1120,3 +1120,21 @@ def test_outputs_of_the_callers_count_as_changed():
             loss.backward()
     with torch.inference_mode():
         D.linear(x, w, out=torch.empty(4, 64, dtype=torch.bfloat16, device="cuda"))
+
+
+def test_no_workspace_where_x_is_read_in_place():
+    x, w = gaussian(4096, 4096, torch.bfloat16, 1, 0.0), gaussian(64, 4096, torch.bfloat16, 2, 0.0)
+    out = torch.empty(4096, 64, dtype=torch.bfloat16, device="cuda")
+    D.linear(x, w, out=out)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    D.linear(x, w, out=out)
+    assert torch.cuda.max_memory_allocated() == before
+    D.linear(x[1:, :], w, out=out[1:])                   # rows of another place on 16 bytes
+    assert torch.cuda.max_memory_allocated() == before
+    odd = torch.empty(4096 * 4096 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(4096, 4096)
+    odd.copy_(x)
+    want = out.clone()
+    assert torch.equal(D.linear(odd, w), want)
+    assert torch.cuda.max_memory_allocated() >= before + 2 * x.numel() * 2

@@ -302,14 +302,15 @@ PyObject* product(PyObject* const* a) {
   d.k = k;
   d.x_stride = stride;
   d.y_stride = row_stride(y);
-  size_t bytes = 0;
-  call(b2vx_linear_workspace_size_noalloc(&d, &bytes, call.err, sizeof(call.err)));
-  at::Tensor workspace = empty({static_cast<int64_t>(bytes)}, at::kByte, device);
   p.x = x.data_ptr();
   p.w = w.data_ptr();
   p.y = y.data_ptr();
-  p.workspace = workspace.data_ptr();
-  p.workspace_bytes = bytes;
+  at::Tensor workspace;
+  if (!b2vx_linear_in_place_noalloc(&d, &p)) {
+    call(b2vx_linear_workspace_size_noalloc(&d, &p.workspace_bytes, call.err, sizeof(call.err)));
+    workspace = empty({static_cast<int64_t>(p.workspace_bytes)}, at::kByte, device);
+    p.workspace = workspace.data_ptr();
+  }
   call(b2vx_linear_noalloc(&d, &p, call.stream, call.err, sizeof(call.err)));
   written(a[11]);
   return THPVariable_Wrap(std::move(y));

@@ -224,6 +224,10 @@ extern "C" b2vx_status b2vx_linear_workspace_size_noalloc(const b2vx_linear_desc
   return B2VX_OK;
 }
 
+extern "C" int32_t b2vx_linear_in_place_noalloc(const b2vx_linear_desc* d, const b2vx_linear_args* a) {
+  return d && a && d->w_format == 0 && !a->row_index && aligned(a->x, 16) && d->x_stride % 8 == 0;
+}
+
 extern "C" b2vx_status b2vx_linear_noalloc(const b2vx_linear_desc* d, const b2vx_linear_args* a, void* cuda_stream, char* err, size_t err_len) {
   b2vx_status st = check_linear(d, err, err_len);
   if (st != B2VX_OK) return st;
@@ -237,8 +241,7 @@ extern "C" b2vx_status b2vx_linear_noalloc(const b2vx_linear_desc* d, const b2vx
   B2VX_NEED(aligned(a->w, 16) && aligned(a->w_scales, 16) && aligned(a->x, size_of(d->x_dtype)) && aligned(a->y, size_of(d->y_dtype)), "a pointer is not aligned");
   B2VX_NEED(aligned(a->bias, 4) && aligned(a->x_scale, 4) && aligned(a->w_scale, 4) && aligned(a->offsets, 4) && aligned(a->row_index, 4), "a pointer is not aligned");
   const Workspace ws = workspace_of(*d);
-  // 16-bit rows that TMA can read where they lie need no workspace
-  const bool direct = !fp4 && !a->row_index && aligned(a->x, 16) && d->x_stride % 8 == 0;
+  const bool direct = b2vx_linear_in_place_noalloc(d, a);
   if (!direct) {
     B2VX_NEED(a->workspace && aligned(a->workspace, 256), "a 256-byte aligned workspace is needed");
     B2VX_NEED(a->workspace_bytes >= ws.total, "the workspace is too small");
