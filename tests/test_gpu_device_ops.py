@@ -1138,3 +1138,19 @@ def test_no_workspace_where_x_is_read_in_place():
     want = out.clone()
     assert torch.equal(D.linear(odd, w), want)
     assert torch.cuda.max_memory_allocated() >= before + 2 * x.numel() * 2
+
+
+def test_route_as_many_pairs_as_32_bits_count():
+    tokens, experts = (2 ** 31 - 1) // 32, 32
+    z = torch.empty(tokens, experts, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    r = D.route_experts(z, experts)                      # every token to every expert: rows are known
+    assert torch.equal(r.offsets, torch.arange(experts + 1, dtype=torch.int64, device="cuda").mul_(tokens).int())
+    step = 1 << 21
+    for t in range(0, tokens, step):
+        ids, m = r.ids[t:t + step].long(), min(step, tokens - t)
+        assert torch.equal(ids.sort(dim=1).values, torch.arange(experts, device="cuda").expand(m, -1))
+        assert torch.equal(r.slots[t:t + step].long(), ids * tokens + torch.arange(t, t + m, device="cuda")[:, None])
+        assert torch.equal(z[t:t + step].gather(1, ids), z[t:t + step].sort(dim=1, descending=True).values)
+    for e in range(experts):
+        assert torch.equal(r.row_index[e * tokens:(e + 1) * tokens], torch.arange(tokens, dtype=torch.int32, device="cuda"))
+    assert ((r.weights[-5:].sum(dim=1) - 1).abs() <= 32 * 2.0 ** -24).all()
