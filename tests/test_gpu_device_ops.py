@@ -1154,3 +1154,11 @@ def test_route_as_many_pairs_as_32_bits_count():
     for e in range(experts):
         assert torch.equal(r.row_index[e * tokens:(e + 1) * tokens], torch.arange(tokens, dtype=torch.int32, device="cuda"))
     assert ((r.weights[-5:].sum(dim=1) - 1).abs() <= 32 * 2.0 ** -24).all()
+
+
+def test_weights_of_no_features():
+    x = torch.ones(3, 32, dtype=torch.bfloat16, device="cuda")
+    w = D.Fp4Weight(torch.zeros(0, 16, dtype=torch.uint8, device="cuda"), torch.zeros(0, 1, dtype=torch.uint8, device="cuda"))
+    assert D.linear(x, w).shape == (3, 0)
+    w = D.Fp4Weight(torch.zeros(2, 0, 16, dtype=torch.uint8, device="cuda"), torch.zeros(2, 0, 1, dtype=torch.uint8, device="cuda"), gated=True)
+    assert D.expert_linear(x, w, torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda"), gated=True).shape == (3, 0)

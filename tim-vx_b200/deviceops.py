@@ -66,7 +66,7 @@ class Fp4Weight:
         if (scale is not None) != (format == "block16"):
             raise ValueError("scale belongs to block16 and only to it")
         self.codes, self.scale, self.format = codes, scale, format
-        self.packed = _native.pack(scales.reshape(-1, rows, k // BLOCK[format]), self.code, self.gated)
+        self.packed = _native.pack(scales.reshape(codes.shape[0] if codes.dim() == 3 else 1, rows, k // BLOCK[format]), self.code, self.gated)
 
 
 def _product(x, weight, offsets, row_index, bias, gated, x_scale, out_dtype, out):
