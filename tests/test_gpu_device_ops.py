@@ -13,6 +13,7 @@ import torch
 
 import device_ops_abi as ABI
 import deviceops as D
+import pyb2vx
 
 pytestmark = pytest.mark.gpu
 E2M1 = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
@@ -1162,3 +1163,8 @@ def test_weights_of_no_features():
     assert D.linear(x, w).shape == (3, 0)
     w = D.Fp4Weight(torch.zeros(2, 0, 16, dtype=torch.uint8, device="cuda"), torch.zeros(2, 0, 1, dtype=torch.uint8, device="cuda"), gated=True)
     assert D.expert_linear(x, w, torch.tensor([0, 1, 3], dtype=torch.int32, device="cuda"), gated=True).shape == (3, 0)
+
+
+def test_weights_of_too_many_experts():
+    with pytest.raises(pyb2vx.B2vxError, match="1024 matrices"):
+        D.Fp4Weight(torch.zeros(1025, 8, 16, dtype=torch.uint8, device="cuda"), torch.zeros(1025, 8, 1, dtype=torch.uint8, device="cuda"))

@@ -252,7 +252,8 @@ PyObject* pack(PyObject* const* a) {
   const int32_t gated = number(a[2]) != 0;
   const uint64_t matrices = scales.size(0), n = gated ? scales.size(1) / 2 : scales.size(1), k = scales.size(2) * block;
   size_t bytes = 0;
-  call(b2vx_fp4_packed_scales_size_noalloc(static_cast<int32_t>(format), matrices, n, gated, k, &bytes));
+  const b2vx_status st = b2vx_fp4_packed_scales_size_noalloc(static_cast<int32_t>(format), matrices, n, gated, k, &bytes);
+  if (st != B2VX_OK) throw Refused{st, "more than 1024 matrices, or an extent out of range"};
   at::Tensor packed = empty({static_cast<int64_t>(bytes)}, at::kByte, scales.device());
   call(b2vx_fp4_pack_scales_noalloc(static_cast<int32_t>(format), matrices, n, gated, k, scales.data_ptr(), packed.data_ptr(), call.stream, call.err, sizeof(call.err)));
   return THPVariable_Wrap(std::move(packed));
