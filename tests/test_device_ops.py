@@ -2,11 +2,15 @@
 
 Every refusal comes before the first CUDA call, so the pointers here are only numbers."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 
 import device_ops_abi as ABI
 import deviceops as D
+import pyb2vx
 
 PTR = 1 << 20   # an address that is aligned to everything; never read
 
@@ -273,3 +277,14 @@ def test_products_that_need_no_workspace(change, args, told):
     a = desc(ABI.LinearArgs, dict(x=PTR, w=PTR, y=PTR), **args)
     assert ABI.library().b2vx_linear_in_place_noalloc(C.byref(d), C.byref(a)) == told
     assert ABI.library().b2vx_linear_in_place_noalloc(None, C.byref(a)) == 0
+
+
+def test_the_libraries_are_made_without_torch():
+    def commands(python):
+        env = {k: v for k, v in os.environ.items() if k not in ("PYTHONPATH", "MAKEFLAGS")}
+        return subprocess.run(["make", "-n", "-B", "-C", os.path.dirname(pyb2vx.PRODUCT_LIB), "PYTHON=" + python], capture_output=True, text=True, check=True, env=env).stdout
+    with_torch, without = commands(sys.executable), commands(sys.executable + " -S")     # -S: no installed packages
+    for text in (with_torch, without):
+        assert "-o " + pyb2vx.PRODUCT_LIB in text and "libtim-vx.so" in text
+    assert "deviceops_torch.cc" in with_torch and "deviceops_torch.cc" not in without
+    assert "has no torch" in without
