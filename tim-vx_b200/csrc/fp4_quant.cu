@@ -15,8 +15,9 @@ namespace {
 
 constexpr int kWarps = 8;
 // Blocks of a quantization kernel an SM: what 48 registers a thread leave, or 64 where 32-bit numbers would not fit beside block16's
-// rounding (8192 x 8192 to block16: 50 us with four, 58 with five).  8192 x 8192 bfloat16 numbers with five / four: to block32 34 / 42 us, to block16 38 / 42.
-// A product's operand in block16 is most often a few rows, where the registers count: 24 rows through 8192 x 8192 13.2 us with five, 12.8 with four.
+// rounding (8192 x 8192 to block16: 50 us with four, 58 with five).  8192 x 8192 bfloat16 numbers by rows with five / four: to block32 34 / 42 us, to
+// block16 38 / 42.  As a product's operand, where the place of the scales takes registers too, block16 wants four at every number of rows: 24 / 512 / 2048 / 8192 rows
+// of 8192 columns and a product with 128 features 6.6 / 17.5 / 29.0 / 73.8 us with five, 6.5 / 16.3 / 24.8 / 62.4 with four.
 constexpr int quantize_blocks(int format, size_t elem, bool packed) { return format == B2VX_FP4_BLOCK16 && (elem == 4 || packed) ? 4 : 5; }
 // Rows that several rows of an operand refer to (a token's, for each of its experts) are quantized once and then copied, where that saves
 // more than the second launch costs: measured at 8192 rows of 1408 columns taken four times each.
