@@ -3,6 +3,7 @@
 Every refusal comes before the first CUDA call, so the pointers here are only numbers."""
 import ctypes as C
 import os
+import re
 import subprocess
 import sys
 
@@ -288,3 +289,10 @@ def test_the_libraries_are_made_without_torch():
         assert "-o " + pyb2vx.PRODUCT_LIB in text and "libtim-vx.so" in text
     assert "deviceops_torch.cc" in with_torch and "deviceops_torch.cc" not in without
     assert "has no torch" in without
+
+
+@pytest.mark.parametrize("name", ["block_linear.cu", "block_linear.cuh", "fp4_quant.cu", "fp4.cuh", "experts.cu", "device_ops.cu"])
+def test_launches_count_the_devices_sms(name):
+    """No number of SMs is written into the code of these operators; comments say which one figures were measured on."""
+    with open(os.path.join(os.path.dirname(pyb2vx.PRODUCT_LIB), name)) as f:
+        assert not re.findall(r"\b(?:148|132|160)\b", re.sub(r"//.*", "", f.read()))

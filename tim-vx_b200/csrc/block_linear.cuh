@@ -64,6 +64,7 @@ struct QuantizeArgs {
   int experts;
   int bn;                      // packed: rows of the product's tiles
   int scale_tiles;             // packed: expert_scale_tiles
+  int sm_count;
 };
 cudaError_t launch_fp4_quantize(const QuantizeArgs& a, cudaStream_t s);
 // The operand x of a product (packed scales; codes_pitch is k / 2, a multiple of 16): quantized in one step, or each row of x once and then
@@ -72,11 +73,12 @@ size_t fp4_twice_bytes(const QuantizeArgs& a);
 cudaError_t launch_fp4_operand(const QuantizeArgs& a, void* between, cudaStream_t s);
 cudaError_t launch_fp4_dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
                                   const float* tensor_scale, int format, long long rows, long long k, void* y, int y_dtype,
-                                  long long y_stride, cudaStream_t s);
-cudaError_t launch_fp4_pack_scales(const uint8_t* scales, int format, long long matrices, long long n, int gated, long long k, uint8_t* packed, cudaStream_t s);
+                                  long long y_stride, int sm_count, cudaStream_t s);
+cudaError_t launch_fp4_pack_scales(const uint8_t* scales, int format, long long matrices, long long n, int gated, long long k, uint8_t* packed, int sm_count,
+                                   cudaStream_t s);
 // rows of 16-bit numbers, gathered: y[i] = x[row_index[i]] (zeros where the index is out of range), K contiguous in y
 cudaError_t launch_gather_rows(const void* x, long long x_stride, long long x_rows, const int32_t* row_index, long long rows, long long k,
-                               void* y, cudaStream_t s);
+                               void* y, int sm_count, cudaStream_t s);
 
 struct LinearArgs {
   int format;                  // 0: 16-bit numbers of x_dtype, else B2VX_FP4_*

@@ -169,6 +169,7 @@ extern "C" b2vx_status b2vx_fp4_quantize_noalloc(const b2vx_fp4_quantize_desc* d
   a.row_index = row_index; a.tensor_scale = tensor_scale; a.format = d->format;
   a.codes = static_cast<uint8_t*>(codes); a.codes_pitch = static_cast<long long>(d->codes_pitch);
   a.scales = static_cast<uint8_t*>(scales); a.scales_pitch = static_cast<long long>(d->scales_pitch);
+  a.sm_count = pd->sm_count;
   return launched(launch_fp4_quantize(a, static_cast<cudaStream_t>(cuda_stream)), err, err_len);
 }
 
@@ -191,7 +192,7 @@ extern "C" b2vx_status b2vx_fp4_dequantize_noalloc(const b2vx_fp4_dequantize_des
   if (st != B2VX_OK) return st;
   return launched(launch_fp4_dequantize(static_cast<const uint8_t*>(codes), static_cast<long long>(d->codes_pitch), static_cast<const uint8_t*>(scales),
                                         static_cast<long long>(d->scales_pitch), tensor_scale, d->format, static_cast<long long>(d->rows),
-                                        static_cast<long long>(d->k), y, d->y_dtype, static_cast<long long>(d->y_stride), static_cast<cudaStream_t>(cuda_stream)),
+                                        static_cast<long long>(d->k), y, d->y_dtype, static_cast<long long>(d->y_stride), pd->sm_count, static_cast<cudaStream_t>(cuda_stream)),
                   err, err_len);
 }
 
@@ -212,7 +213,7 @@ extern "C" b2vx_status b2vx_fp4_pack_scales_noalloc(int32_t format, uint64_t mat
   b2vx_status st = device(&pd, err, err_len);
   if (st != B2VX_OK) return st;
   return launched(launch_fp4_pack_scales(static_cast<const uint8_t*>(scales), format, static_cast<long long>(matrices), static_cast<long long>(n), gated,
-                                         static_cast<long long>(k), static_cast<uint8_t*>(packed), static_cast<cudaStream_t>(cuda_stream)),
+                                         static_cast<long long>(k), static_cast<uint8_t*>(packed), pd->sm_count, static_cast<cudaStream_t>(cuda_stream)),
                   err, err_len);
 }
 
@@ -277,12 +278,13 @@ extern "C" b2vx_status b2vx_linear_noalloc(const b2vx_linear_desc* d, const b2vx
     q.offsets = a->offsets; q.experts = l.experts;
     q.bn = tile_rows(l.rows, l.experts, l.format);
     q.scale_tiles = static_cast<int>(expert_scale_tiles(l.rows, l.experts, q.bn));
+    q.sm_count = pd->sm_count;
     e = launch_fp4_operand(q, codes + ws.codes + ws.scales, s);
     l.x = codes; l.x_pitch = static_cast<long long>(ws.codes_pitch); l.x_scales = q.scales;
   } else if (direct) {
     l.x = a->x; l.x_pitch = static_cast<long long>(d->x_stride) * 2;
   } else {
-    e = launch_gather_rows(a->x, static_cast<long long>(d->x_stride), static_cast<long long>(d->x_rows), a->row_index, l.rows, l.k, codes, s);
+    e = launch_gather_rows(a->x, static_cast<long long>(d->x_stride), static_cast<long long>(d->x_rows), a->row_index, l.rows, l.k, codes, pd->sm_count, s);
     l.x = codes; l.x_pitch = static_cast<long long>(ws.codes_pitch);
   }
   if (e != cudaSuccess) return launched(e, err, err_len);
@@ -323,7 +325,7 @@ extern "C" b2vx_status b2vx_route_noalloc(const b2vx_route_desc* d, const void* 
   B2VX_NEED(need == 0 || (workspace && aligned(workspace, 256) && workspace_bytes >= need), "a 256-byte aligned workspace of the told size is needed");
   st = device(&pd, err, err_len);
   if (st != B2VX_OK) return st;
-  return launched(launch_route(*d, logits, ids, weights, offsets, row_index, slots, workspace, s), err, err_len);
+  return launched(launch_route(*d, logits, ids, weights, offsets, row_index, slots, workspace, pd->sm_count, s), err, err_len);
 }
 
 extern "C" b2vx_status b2vx_combine_noalloc(const b2vx_combine_desc* d, const void* z, const int32_t* slots, const float* weights, const void* residual,
@@ -339,7 +341,7 @@ extern "C" b2vx_status b2vx_combine_noalloc(const b2vx_combine_desc* d, const vo
   PerDevice* pd;
   b2vx_status st = device(&pd, err, err_len);
   if (st != B2VX_OK) return st;
-  return launched(launch_combine(*d, z, slots, weights, residual, y, static_cast<cudaStream_t>(cuda_stream)), err, err_len);
+  return launched(launch_combine(*d, z, slots, weights, residual, y, pd->sm_count, static_cast<cudaStream_t>(cuda_stream)), err, err_len);
 }
 
 extern "C" b2vx_status b2vx_device_check_noalloc(void* cuda_stream, char* err, size_t err_len) {

@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(1024) place_kernel(const int32_t* ids, const u
 
 template <typename T, int PER>
 cudaError_t route(const b2vx_route_desc& d, const T* logits, int32_t* ids, float* weights, int32_t* offsets, int32_t* row_index, int32_t* slots,
-                  void* workspace, cudaStream_t s) {
+                  void* workspace, int sm_count, cudaStream_t s) {
   const int tokens = static_cast<int>(d.tokens), experts = static_cast<int>(d.experts), top_k = static_cast<int>(d.top_k);
   const int blocks = (tokens + kBlockTokens - 1) / kBlockTokens;
   const long long stride = static_cast<long long>(d.logits_stride);
@@ -254,19 +254,19 @@ cudaError_t route(const b2vx_route_desc& d, const T* logits, int32_t* ids, float
   e = launch_pdl(before_kernel, dim3((experts + 31) / 32), dim3(1024), 0, s, static_cast<const uint32_t*>(masks), blocks, experts, before, totals);
   if (e != cudaSuccess) return e;
   const int pairs = tokens * top_k;      // up to 2^31 - 1, so no sum with it in 32 bits
-  return launch_pdl(place_kernel, dim3(std::min(pairs / 1024 + 1, 148 * 2)), dim3(1024), 0, s, static_cast<const int32_t*>(ids),
+  return launch_pdl(place_kernel, dim3(std::min(pairs / 1024 + 1, sm_count * 2)), dim3(1024), 0, s, static_cast<const int32_t*>(ids),
                     static_cast<const uint32_t*>(masks), static_cast<const int32_t*>(before), static_cast<const int32_t*>(totals), pairs, experts, top_k, offsets,
                     row_index, slots);
 }
 template <typename T>
 cudaError_t route_typed(const b2vx_route_desc& d, const void* logits, int32_t* ids, float* weights, int32_t* offsets, int32_t* row_index, int32_t* slots,
-                        void* workspace, cudaStream_t s) {
+                        void* workspace, int sm_count, cudaStream_t s) {
   const T* z = static_cast<const T*>(logits);
-  if (d.experts <= 64) return route<T, 2>(d, z, ids, weights, offsets, row_index, slots, workspace, s);
-  if (d.experts <= 128) return route<T, 4>(d, z, ids, weights, offsets, row_index, slots, workspace, s);
-  if (d.experts <= 256) return route<T, 8>(d, z, ids, weights, offsets, row_index, slots, workspace, s);
-  if (d.experts <= 512) return route<T, 16>(d, z, ids, weights, offsets, row_index, slots, workspace, s);
-  return route<T, 32>(d, z, ids, weights, offsets, row_index, slots, workspace, s);
+  if (d.experts <= 64) return route<T, 2>(d, z, ids, weights, offsets, row_index, slots, workspace, sm_count, s);
+  if (d.experts <= 128) return route<T, 4>(d, z, ids, weights, offsets, row_index, slots, workspace, sm_count, s);
+  if (d.experts <= 256) return route<T, 8>(d, z, ids, weights, offsets, row_index, slots, workspace, sm_count, s);
+  if (d.experts <= 512) return route<T, 16>(d, z, ids, weights, offsets, row_index, slots, workspace, sm_count, s);
+  return route<T, 32>(d, z, ids, weights, offsets, row_index, slots, workspace, sm_count, s);
 }
 
 // The sum is bound by memory: z once.  blockDim.x threads share a token, each with 16 bytes of neighbouring columns (VEC) or one column at a
@@ -325,14 +325,15 @@ __global__ void __launch_bounds__(256) combine_kernel(const T* z, long long z_st
 }
 
 template <typename T>
-cudaError_t combine(const b2vx_combine_desc& d, const void* z, const int32_t* slots, const float* weights, const void* residual, void* y, cudaStream_t s) {
+cudaError_t combine(const b2vx_combine_desc& d, const void* z, const int32_t* slots, const float* weights, const void* residual, void* y, int sm_count,
+                    cudaStream_t s) {
   constexpr uint64_t N = 16 / sizeof(T);
   const bool vec = d.n % N == 0 && d.z_stride % N == 0 && d.y_stride % N == 0 && reinterpret_cast<uintptr_t>(z) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(y) % 16 == 0 && (!residual || (d.residual_stride % N == 0 && reinterpret_cast<uintptr_t>(residual) % 16 == 0));
   const int pieces = static_cast<int>(vec ? d.n / N : d.n), tokens = static_cast<int>(d.tokens);
   int x = 8;                                     // threads to a token
   while (x < 256 && x < pieces) x *= 2;
-  const int y_dim = 256 / x, grid = std::min((tokens + y_dim - 1) / y_dim, 148 * 8);
+  const int y_dim = 256 / x, grid = std::min((tokens + y_dim - 1) / y_dim, sm_count * 8);
   auto* kernel = vec ? combine_kernel<T, true> : combine_kernel<T, false>;
   return launch_pdl(kernel, dim3(grid), dim3(x, y_dim), 0, s, static_cast<const T*>(z), static_cast<long long>(d.z_stride), static_cast<int>(d.z_rows), slots,
                     weights, static_cast<const T*>(residual), static_cast<long long>(d.residual_stride), static_cast<T*>(y),
@@ -347,17 +348,17 @@ size_t route_workspace_bytes(long long tokens, int experts) {
 }
 
 cudaError_t launch_route(const b2vx_route_desc& d, const void* logits, int32_t* ids, float* weights, int32_t* offsets, int32_t* row_index,
-                         int32_t* slots, void* workspace, cudaStream_t s) {
-  if (d.logits_dtype == B2VX_DT_FLOAT32) return route_typed<float>(d, logits, ids, weights, offsets, row_index, slots, workspace, s);
-  if (d.logits_dtype == B2VX_DT_FLOAT16) return route_typed<__half>(d, logits, ids, weights, offsets, row_index, slots, workspace, s);
-  return route_typed<__nv_bfloat16>(d, logits, ids, weights, offsets, row_index, slots, workspace, s);
+                         int32_t* slots, void* workspace, int sm_count, cudaStream_t s) {
+  if (d.logits_dtype == B2VX_DT_FLOAT32) return route_typed<float>(d, logits, ids, weights, offsets, row_index, slots, workspace, sm_count, s);
+  if (d.logits_dtype == B2VX_DT_FLOAT16) return route_typed<__half>(d, logits, ids, weights, offsets, row_index, slots, workspace, sm_count, s);
+  return route_typed<__nv_bfloat16>(d, logits, ids, weights, offsets, row_index, slots, workspace, sm_count, s);
 }
 
 cudaError_t launch_combine(const b2vx_combine_desc& d, const void* z, const int32_t* slots, const float* weights, const void* residual, void* y,
-                           cudaStream_t s) {
-  if (d.dtype == B2VX_DT_FLOAT32) return combine<float>(d, z, slots, weights, residual, y, s);
-  if (d.dtype == B2VX_DT_FLOAT16) return combine<__half>(d, z, slots, weights, residual, y, s);
-  return combine<__nv_bfloat16>(d, z, slots, weights, residual, y, s);
+                           int sm_count, cudaStream_t s) {
+  if (d.dtype == B2VX_DT_FLOAT32) return combine<float>(d, z, slots, weights, residual, y, sm_count, s);
+  if (d.dtype == B2VX_DT_FLOAT16) return combine<__half>(d, z, slots, weights, residual, y, sm_count, s);
+  return combine<__nv_bfloat16>(d, z, slots, weights, residual, y, sm_count, s);
 }
 
 }  // namespace b2vx

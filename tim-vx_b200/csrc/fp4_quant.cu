@@ -262,14 +262,14 @@ __global__ void __launch_bounds__(256) gather_rows_kernel(const uint16_t* x, lon
   }
 }
 
-int blocks_for(long long units, int per_block, int per_sm) {
-  return static_cast<int>(std::max<long long>(1, std::min<long long>((units + per_block - 1) / per_block, 148 * per_sm)));
+int blocks_for(long long units, int per_block, int most) {
+  return static_cast<int>(std::max<long long>(1, std::min<long long>((units + per_block - 1) / per_block, most)));
 }
 
 // Warps that share a row: up to as many as it has chunks, so that there are about four units of work for each warp that fits the GPU and an
 // uneven last round costs little.
-int split_of(long long rows, int chunks) {
-  const long long fill = 4 * 148 * 40;
+int split_of(long long rows, int chunks, int sm_count) {
+  const long long fill = 4ll * sm_count * 40;
   return static_cast<int>(std::max<long long>(1, std::min<long long>(chunks, fill / std::max<long long>(1, rows))));
 }
 // The same for a product's operand, where a row's start costs about as much as a chunk (the place of its scales): rounds of `warps` units, each
@@ -293,8 +293,8 @@ cudaError_t quantize(const QuantizeArgs& a, cudaStream_t s) {
   const int chunks = static_cast<int>((a.k + kChunk - 1) / kChunk);
   const bool operand = a.scales_pitch == 0;
   const int kBlocks = quantize_blocks(FORMAT, sizeof(T), operand);
-  const int split = operand ? operand_split_of(a.rows, chunks, 148 * kBlocks * kWarps) : split_of(a.rows, chunks);
-  const int grid = blocks_for(a.rows * split, kWarps, kBlocks);
+  const int split = operand ? operand_split_of(a.rows, chunks, a.sm_count * kBlocks * kWarps) : split_of(a.rows, chunks, a.sm_count);
+  const int grid = blocks_for(a.rows * split, kWarps, a.sm_count * kBlocks);
   if (operand) return launch_pdl(quantize_kernel<T, FORMAT, VEC, true>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
   return launch_pdl(quantize_kernel<T, FORMAT, VEC, false>, dim3(grid), dim3(kWarps * 32), 0, s, a, chunks, split);
 }
@@ -309,13 +309,13 @@ cudaError_t quantize_format(const QuantizeArgs& a, cudaStream_t s) {
 }
 template <typename T>
 cudaError_t dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch, const float* tensor_scale, int format,
-                       long long rows, long long k, void* y, long long y_stride, cudaStream_t s) {
+                       long long rows, long long k, void* y, long long y_stride, int sm_count, cudaStream_t s) {
   const int chunks = static_cast<int>((k + 255) / 256);
-  const int split = split_of(rows, (chunks + 3) / 4);
+  const int split = split_of(rows, (chunks + 3) / 4, sm_count);
   const bool vec = reinterpret_cast<uintptr_t>(y) % 16 == 0 && (y_stride * sizeof(T)) % 16 == 0;
   auto* kernel = format == B2VX_FP4_BLOCK32 ? (vec ? dequantize_kernel<T, B2VX_FP4_BLOCK32, true> : dequantize_kernel<T, B2VX_FP4_BLOCK32, false>)
                                             : (vec ? dequantize_kernel<T, B2VX_FP4_BLOCK16, true> : dequantize_kernel<T, B2VX_FP4_BLOCK16, false>);
-  return launch_pdl(kernel, dim3(blocks_for(rows * split, kWarps, 6)), dim3(kWarps * 32), 0, s, codes, codes_pitch, scales, scales_pitch, tensor_scale,
+  return launch_pdl(kernel, dim3(blocks_for(rows * split, kWarps, sm_count * 6)), dim3(kWarps * 32), 0, s, codes, codes_pitch, scales, scales_pitch, tensor_scale,
                     static_cast<uint32_t>(rows), static_cast<int>(k), static_cast<T*>(y), y_stride, chunks, split);
 }
 
@@ -343,28 +343,28 @@ cudaError_t launch_fp4_operand(const QuantizeArgs& a, void* between, cudaStream_
   cudaError_t e = launch_fp4_quantize(once, s);
   if (e != cudaSuccess) return e;
   auto* kernel = a.format == B2VX_FP4_BLOCK32 ? gather_fp4_kernel<B2VX_FP4_BLOCK32> : gather_fp4_kernel<B2VX_FP4_BLOCK16>;
-  return launch_pdl(kernel, dim3(blocks_for(a.rows, kWarps, 8)), dim3(kWarps * 32), 0, s, a, static_cast<const uint8_t*>(once.codes),
+  return launch_pdl(kernel, dim3(blocks_for(a.rows, kWarps, a.sm_count * 8)), dim3(kWarps * 32), 0, s, a, static_cast<const uint8_t*>(once.codes),
                     static_cast<const uint8_t*>(once.scales), once.scales_pitch);
 }
 cudaError_t launch_fp4_dequantize(const uint8_t* codes, long long codes_pitch, const uint8_t* scales, long long scales_pitch,
                                   const float* tensor_scale, int format, long long rows, long long k, void* y, int y_dtype,
-                                  long long y_stride, cudaStream_t s) {
-  if (y_dtype == B2VX_DT_FLOAT32) return dequantize<float>(codes, codes_pitch, scales, scales_pitch, tensor_scale, format, rows, k, y, y_stride, s);
-  if (y_dtype == B2VX_DT_FLOAT16) return dequantize<__half>(codes, codes_pitch, scales, scales_pitch, tensor_scale, format, rows, k, y, y_stride, s);
-  return dequantize<__nv_bfloat16>(codes, codes_pitch, scales, scales_pitch, tensor_scale, format, rows, k, y, y_stride, s);
+                                  long long y_stride, int sm_count, cudaStream_t s) {
+  if (y_dtype == B2VX_DT_FLOAT32) return dequantize<float>(codes, codes_pitch, scales, scales_pitch, tensor_scale, format, rows, k, y, y_stride, sm_count, s);
+  if (y_dtype == B2VX_DT_FLOAT16) return dequantize<__half>(codes, codes_pitch, scales, scales_pitch, tensor_scale, format, rows, k, y, y_stride, sm_count, s);
+  return dequantize<__nv_bfloat16>(codes, codes_pitch, scales, scales_pitch, tensor_scale, format, rows, k, y, y_stride, sm_count, s);
 }
 cudaError_t launch_fp4_pack_scales(const uint8_t* scales, int format, long long matrices, long long n, int gated, long long k, uint8_t* packed,
-                                   cudaStream_t s) {
+                                   int sm_count, cudaStream_t s) {
   const long long blocks = (k + fp4_block(format) - 1) / fp4_block(format), words = scale_words(k, format);
   const long long total = static_cast<long long>(packed_scale_bytes(matrices, n, gated, k, format) / 4);
-  return launch_pdl(pack_scales_kernel, dim3(blocks_for(total, 256, 8)), dim3(256), 0, s, scales, matrices, n, gated, blocks, words,
+  return launch_pdl(pack_scales_kernel, dim3(blocks_for(total, 256, sm_count * 8)), dim3(256), 0, s, scales, matrices, n, gated, blocks, words,
                     scale_words_per_stage(format), reinterpret_cast<uint32_t*>(packed));
 }
 cudaError_t launch_gather_rows(const void* x, long long x_stride, long long x_rows, const int32_t* row_index, long long rows, long long k, void* y,
-                               cudaStream_t s) {
+                               int sm_count, cudaStream_t s) {
   const int pieces = static_cast<int>(k / 8);
   const int vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && x_stride % 8 == 0;
-  return launch_pdl(gather_rows_kernel, dim3(blocks_for(rows * pieces, 256, 8)), dim3(256), 0, s, static_cast<const uint16_t*>(x), x_stride, x_rows,
+  return launch_pdl(gather_rows_kernel, dim3(blocks_for(rows * pieces, 256, sm_count * 8)), dim3(256), 0, s, static_cast<const uint16_t*>(x), x_stride, x_rows,
                     row_index, rows, k, pieces, static_cast<uint4*>(y), vec);
 }
 
