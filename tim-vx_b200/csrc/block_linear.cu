@@ -502,6 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   // its instructions, some 300 cycles of waiting and bookkeeping, is why a stage holds two k-blocks, and why nothing votes on a wait
   // that gave up: the elected lane then does nothing more in its rounds, and the exit waits for copies in flight.
   const uint32_t full0 = smem_u32(h->full), empty0 = smem_u32(h->empty);
+  uint32_t next_stage = 0, next_phase = 0;         // of the producer of W, at its end
   if (warp == 0) {
     // ------------------------------------------------------------ producer of W
     const uint32_t announce = CG == 1 ? full0 : in_first_cta(full0);
@@ -529,12 +530,8 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
         if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
       }
     }
-    // The last use of each stage: what the issuer's instructions still tell this CTA's barriers has to arrive while it exists.
-    for (int i = 0; i < p.stages; ++i) {
-      if (elect_one()) ok = ok && wait(empty0 + 8 * s, ph ^ 1, 101);
-      __syncwarp();
-      if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; }
-    }
+    next_stage = s;
+    next_phase = ph;
   } else if (!RAW && warp == 2) {
     // ------------------------------------------------------------ producer of x
     pdl_wait();
@@ -618,8 +615,8 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       const int buf = j & 1;
       const uint32_t buf_ph = (j >> 1) & 1;
       if constexpr (CG == 1) {
-        ok = ok && wait(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, 102);
-      } else if (ok && !wait_cluster(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102, p.wait_limit)) {
+        ok &= wait(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, 102);
+      } else if (!wait_cluster(smem_u32(&h->acc_empty[buf]), buf_ph ^ 1, abort_flag, p.status, 102, p.wait_limit)) {
         ok = false;
         abort_other(smem_u32(&h->abort_flag));
       }
@@ -654,10 +651,10 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
       for (int kb = kb_first; kb < kb_end; kb += kGroup) {
         // the next tile is worked out while the instructions of this one's last stages run
         if (kb + kGroup >= kb_end && t + tile_step < num_tiles) tile = tile_of<CG>(groups, p, t + tile_step, tile.e);
-        if (RAW && kb == kb_first) ok = ok && wait(smem_u32(&h->x_ready), 0, 107);
-        ok = ok && wait(full0 + 8 * s, ph, 103);
-        __syncwarp();
-        if (elect_one() && ok) {
+        // given up, the waits of the rounds that are left return at once; a branch around them would cost every round
+        if (RAW && kb == kb_first) ok &= wait(smem_u32(&h->x_ready), 0, 107);
+        ok &= wait(full0 + 8 * s, ph, 103);
+        if (elect_one() & ok) {
           fence_after();
           k_block(low, 0, kb, kb == kb_first);
           if (kb + 1 < kb_end) k_block(low + block_low, 1, kb + 1, false);
@@ -667,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
         low += stage_low;
         if (++s == static_cast<uint32_t>(p.stages)) { s = 0; ph ^= 1; low = ring_low; }
       }
-      if (elect_one() && ok) commit<CG>(smem_u32(&h->acc_full[buf]));
+      if (elect_one() & ok) commit<CG>(smem_u32(&h->acc_full[buf]));
       __syncwarp();
     }
   } else if (SPLIT && warp >= kFirstEpilogueWarp) {
@@ -902,6 +899,9 @@ __global__ void __launch_bounds__(kThreads, 1) block_linear_kernel(const __grid_
   }
 
   // ---------------------------------------------------------------- common exit
+  // What the other CTA's instructions still tell this one's barriers, the last use of each stage, has to arrive while it exists: a lane waits for each.
+  // (Within a CTA the epilogue has seen a later word of the same issuer.  Waiting there too cost one row through 4096 x 4096 0.2 us.)
+  if (CG == 2 && warp == 0 && lane < p.stages) wait(empty0 + 8 * lane, static_cast<uint32_t>(lane) < next_stage ? next_phase : next_phase ^ 1, 101);
   __syncwarp();
   fence_before();
   if constexpr (CG == 1) __syncthreads();
