@@ -31,29 +31,33 @@ template <int FORMAT>
 __device__ __forceinline__ uint8_t* packed_place(const QuantizeArgs& a, uint32_t row, int lane) {
   int e = 0, lo = 0, count = static_cast<int>(a.rows);
   if (a.offsets) {
-    int end = a.experts + 1, begun = 0;                      // the first offset behind the row; how many are not
-    for (int top = a.experts - lane; top >= 0; top -= 4 * 32) {
+    // of the offsets behind the first: the first that is behind the row, and how many are not
+    int end = a.experts + 1, begun = 0;
+    const int begin = a.offsets[0];
+    for (int top = a.experts - lane; top > 0; top -= 4 * 32) {
       int v[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = top - u * 32 >= 0 ? a.offsets[top - u * 32] : INT_MIN;
+      for (int u = 0; u < 4; ++u) v[u] = top - u * 32 > 0 ? a.offsets[top - u * 32] : INT_MIN;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         if (v[u] > static_cast<int>(row)) {
           end = top - u * 32;
         } else {
           lo = max(lo, v[u]);
-          begun += top - u * 32 >= 0;
+          begun += top - u * 32 > 0;
         }
       }
     }
     end = __reduce_min_sync(0xffffffffu, end);
     begun = __reduce_add_sync(0xffffffffu, begun);
-    if (end == 0 || end > a.experts) return nullptr;
-    if (begun != end) {                                      // some behind the end are lower again
+    lo = __reduce_max_sync(0xffffffffu, lo);
+    if (begin > static_cast<int>(row) || end > a.experts) return nullptr;
+    if (begun != end - 1) {                                  // some behind the end are lower again
       lo = 0;
       for (int j = lane; j < end; j += 32) lo = max(lo, a.offsets[j]);
+      lo = __reduce_max_sync(0xffffffffu, lo);
     }
-    lo = __reduce_max_sync(0xffffffffu, lo);
+    lo = max(lo, begin);
     e = end - 1;
     count = min(a.offsets[end], count) - lo;
   }
