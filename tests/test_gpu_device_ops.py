@@ -1168,3 +1168,30 @@ def test_weights_of_no_features():
 def test_weights_of_too_many_experts():
     with pytest.raises(pyb2vx.B2vxError, match="1024 matrices"):
         D.Fp4Weight(torch.zeros(1025, 8, 16, dtype=torch.uint8, device="cuda"), torch.zeros(1025, 8, 1, dtype=torch.uint8, device="cuda"))
+
+
+@pytest.mark.parametrize("fmt", ["block32", "block16", "none"])
+@pytest.mark.parametrize("rows,n,k", [(1, 8, 32), (1, 72, 2048), (2, 200, 4096), (16, 4104, 512), (5, 1000, 8192), (17, 136, 1056), (100, 264, 288), (300, 1032, 544)])
+def test_one_gated_matrix(fmt, rows, n, k):
+    """A gated product without experts, in every form: x quantized by the product and by a launch before it, K shared, two CTAs to a tile."""
+    dtype = torch.bfloat16
+    x = gaussian(rows, k, dtype, rows + n, 1.0)
+    xv, s = operand(x, fmt)
+    if fmt == "none":
+        w = (gaussian(2 * n, k, torch.float32, n, 1.0) / k ** 0.5).to(dtype)
+        wv, packed, scale, codes = f64(w), None, None, w
+    else:
+        w, wv = weight_of(0, 2 * n, k, fmt, n, True)
+        wv, packed, scale, codes = wv[0], w.packed, w.scale, w.codes
+    bias = gaussian(1, 2 * n, torch.float32, 6, 0.0)[0] if rows != 2 else None
+    d = ABI.LinearDesc(D.FORMATS.get(fmt, 0), 16, 9, 1, 0, rows, rows, n, k, k, n + 3)
+    size = C.c_size_t()
+    ABI.call(ABI.library().b2vx_linear_workspace_size_noalloc, C.byref(d), C.byref(size))
+    work = torch.full((max(1, size.value),), 0x7F, dtype=torch.uint8, device="cuda")
+    y = torch.full((rows, n + 3), -77.0, device="cuda")
+    at = lambda t: None if t is None else t.data_ptr()
+    a = ABI.LinearArgs(at(x), at(codes), at(packed), at(s), at(scale), at(bias), None, None, at(y), at(work), size.value)
+    ABI.call(ABI.library().b2vx_linear_noalloc, C.byref(d), C.byref(a), torch.cuda.current_stream().cuda_stream)
+    close(y[:, :n], *expected(xv, wv, None if bias is None else f64(bias), True))
+    assert (y[:, n:] == -77.0).all()
+    assert torch.equal(D.expert_linear(x, w, None, bias=bias, gated=True, x_scale=s, out_dtype=torch.float32), y[:, :n])
