@@ -319,7 +319,7 @@ b2vx_status b2vx_conv2d_first_layer_noalloc(const b2vx_conv2d_noalloc_desc* d, c
  * current device, results are queued on `cuda_stream` (NULL: the default stream)
  * and the call returns without waiting.  Nothing is allocated: intermediates go to
  * a workspace of the caller's, whose size the _workspace_ calls tell.  A call may
- * be captured into a CUDA graph, after the first call on that GPU; calls or
+ * be captured into a CUDA graph, the first one on a GPU too; calls or
  * captured graphs that may overlap need a workspace each.  Arguments are checked
  * before anything is launched; refusals return a status and write a message to err
  * (err may be NULL).  Counts of zero are fine: nothing is launched.  Outputs must not

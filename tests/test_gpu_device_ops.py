@@ -1195,3 +1195,43 @@ def test_one_gated_matrix(fmt, rows, n, k):
     close(y[:, :n], *expected(xv, wv, None if bias is None else f64(bias), True))
     assert (y[:, n:] == -77.0).all()
     assert torch.equal(D.expert_linear(x, w, None, bias=bias, gated=True, x_scale=s, out_dtype=torch.float32), y[:, :n])
+
+
+FIRST_OF_EACH = """
+import sys
+sys.path[:0] = %r
+import torch, deviceops as D
+torch.manual_seed(0)
+dev = "cuda"
+x, xs = torch.randn(300, 256, device=dev).bfloat16(), torch.full((1,), 0.01, device=dev)
+codes = torch.randint(0, 256, (6, 128, 128), device=dev).byte()
+scales = torch.randint(118, 124, (6, 128, 8), device=dev).byte()
+plain = torch.randn(6, 128, 256, device=dev).bfloat16()
+logits = torch.randn(300, 6, device=dev)
+odd = torch.randn(301, 257, device=dev).bfloat16()[1:, 1:]
+torch.cuda.synchronize()
+
+def everything():
+    w, one = D.Fp4Weight(codes, scales, gated=True), D.Fp4Weight(codes[0], scales[0])
+    r, few = D.route_experts(logits, 2), D.route_experts(logits[:9], 2)
+    h = D.expert_linear(x, w, r.offsets, row_index=r.row_index, gated=True)
+    outs = [*r, *few, h, D.expert_linear(x, plain, r.offsets, row_index=r.row_index), D.combine_experts(h, r.slots, r.weights)]
+    outs += [D.linear(x[:n], one) for n in (1, 20, 300)] + [D.linear(odd, plain[0]), D.linear(odd[:3], one)]
+    for q in (D.quantize_fp4(x), D.quantize_fp4(odd, "block16", scale=xs)):
+        outs += [q.codes, q.scales, D.dequantize_fp4(q)]
+    return outs
+
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    captured = everything()
+g.replay()
+D.check("cuda")
+for a, b in zip(captured, everything()):
+    assert torch.equal(a, b)
+print("same")
+"""
+
+
+def test_the_first_call_of_each_operator_may_be_captured():
+    out = subprocess.run([sys.executable, "-c", FIRST_OF_EACH % sys.path], capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip() == "same", out.stderr
