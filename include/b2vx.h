@@ -356,7 +356,8 @@ typedef struct b2vx_fp4_quantize_desc {
 b2vx_status b2vx_fp4_quantize_noalloc(const b2vx_fp4_quantize_desc* d, const void* x, const int32_t* row_index,
                                       const float* tensor_scale, void* codes, void* scales,
                                       void* cuda_stream, char* err, size_t err_len);
-/* The values that codes and scales stand for, times the tensor scale, rounded once to y_dtype. */
+/* The values that codes and scales stand for, times the tensor scale: float32 products, then rounded to y_dtype.  In BLOCK32 only the last step
+ * rounds; in BLOCK16 the tensor scale's product does too, so a 16-bit y may be off by 2^-24 of itself more than half its step. */
 typedef struct b2vx_fp4_dequantize_desc {
   int32_t format, y_dtype;
   uint64_t rows, k;
