@@ -253,8 +253,8 @@ cudaError_t route(const b2vx_route_desc& d, const T* logits, int32_t* ids, float
   if (e != cudaSuccess) return e;
   e = launch_pdl(before_kernel, dim3((experts + 31) / 32), dim3(1024), 0, s, static_cast<const uint32_t*>(masks), blocks, experts, before, totals);
   if (e != cudaSuccess) return e;
-  const int pairs = tokens * top_k;      // up to 2^31 - 1, so no sum with it in 32 bits
-  return launch_pdl(place_kernel, dim3(std::min(pairs / 1024 + 1, sm_count * 2)), dim3(1024), 0, s, static_cast<const int32_t*>(ids),
+  const int pairs = tokens * top_k;      // 1 to 2^31 - 1: no sum with it in 32 bits
+  return launch_pdl(place_kernel, dim3(std::min((pairs - 1) / 1024 + 1, sm_count * 2)), dim3(1024), 0, s, static_cast<const int32_t*>(ids),
                     static_cast<const uint32_t*>(masks), static_cast<const int32_t*>(before), static_cast<const int32_t*>(totals), pairs, experts, top_k, offsets,
                     row_index, slots);
 }
