@@ -1,7 +1,7 @@
 // Rows of numbers to 4-bit block floating point and back, packing of scales, gathering of rows.
 //
 // Quantization reads every number once and writes half a byte and a scale's share for it: 8192 x 8192 bfloat16 numbers to block32 in 34 us,
-// to block16 in 38 (26 are the bytes'), 32-bit numbers in 49 (46), bound by instructions between rounding and memory.
+// to block16 in 38 (26 are the bytes'), 32-bit numbers in 49 (46).  From 16 bits instructions bind, 65 - 68 % of the issue slots at 55 % of the warps; from 32 bits memory.
 // Sixteen columns a lane: a block of block16, so that its scale, some forty instructions, is worked out once, or half a block of block32.
 #include <algorithm>
 #include <climits>
