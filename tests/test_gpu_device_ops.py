@@ -1143,6 +1143,8 @@ def test_no_workspace_where_x_is_read_in_place():
 
 def test_route_as_many_pairs_as_32_bits_count():
     tokens, experts = (2 ** 31 - 1) // 32, 32
+    if torch.cuda.mem_get_info()[0] < 56 << 30:
+        pytest.skip("needs 56 GB")
     z = torch.empty(tokens, experts, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
     r = D.route_experts(z, experts)                      # every token to every expert: rows are known
     assert torch.equal(r.offsets, torch.arange(experts + 1, dtype=torch.int64, device="cuda").mul_(tokens).int())
